@@ -66,6 +66,12 @@ SIGNATURES = {
                                              _u32, _vp]),
     "fa_window_attention_bias_noalloc": (_i32, [_i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64p, _vp,
                                                  _i64, _f32, _vp]),
+    "fa_window_attention_rel_bias_workspace": (_i64, [_i32, _i64, _i64, _i64, _i32]),
+    "fa_window_attention_rel_bias": (_i32, [_i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64p, _vp, _i32, _vp,
+                                            _u8p, _u8p, _i64, _f32, _vp, _vp, _i64, _vp]),
+    "fa_window_attention_rel_bias_backward": (_i32, [_i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                     _i64p, _vp, _i32, _vp, _u8p, _u8p, _i64, _f32, _vp, _vp, _vp,
+                                                     _i64, _vp, _vp, _i64, _vp]),
     "fa_layernorm_affine": (_i32, [_vp, _i32, _vp, _vp, _vp, _i32, _f32, _vp, _i64, _i64, _vp]),
     "fa_attention_status": (_i32, [ctypes.POINTER(ctypes.c_int)]),
     "fa_attention_status_reset": (_i32, [_vp]),

@@ -1693,6 +1693,8 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
   return fn;
 }
 
+}  // namespace
+
 // 4D map over (Dh, N, H, Bwin) of one operand, box (inner, 144, 1, 1), 128-byte swizzle,
 // out-of-range token rows read as zero.
 int make_map(CUtensorMap* map, const void* base, bool f32, int64_t Bwin, int64_t H, int64_t N,
@@ -1711,6 +1713,8 @@ int make_map(CUtensorMap* map, const void* base, bool f32, int64_t Bwin, int64_t
   FA_REQUIRE(r == CUDA_SUCCESS, FA_ERR_CUDA, "cuTensorMapEncodeTiled failed (code " + std::to_string((int)r) + ")");
   return FA_OK;
 }
+
+namespace {
 
 template <int kMask>
 int launch_tc_bf16(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,

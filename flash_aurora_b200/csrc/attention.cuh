@@ -1,6 +1,7 @@
 // Shared definitions of the window-attention kernels.
 #pragma once
 
+#include <cuda.h>
 #include <stdint.h>
 
 namespace fa {
@@ -27,6 +28,10 @@ struct Params {
 };
 
 int* status_ptr();
+
+// 4D tensor map over (Dh, N, H, Bwin) of one operand, box (inner, 144, 1, 1), 128-byte swizzle; token
+// rows past N read as zero and are dropped by stores. `strides`: window, head, token (elements).
+int make_map(CUtensorMap* map, const void* base, bool f32, int64_t Bwin, int64_t H, int64_t N, const int64_t* strides);
 
 // Argument checks of run() (shapes, precision, flags, pointers, strides, alignment), without
 // launching anything: FA_OK or the status run() would return for these arguments.

@@ -1,0 +1,331 @@
+// Window attention with a learned relative position bias, and its gradients (N <= 144, head_dim 64).
+//
+//   x_ij = scale q_i . k_j + T[index_ij, h] + mask_ij        mask: -100 where masked
+//   P = softmax_j(x),  o = P v
+//   dV = P^T dO,  dP = dO V^T,  dS_ij = P_ij (dP_ij - sum_j' P_ij' dP_ij')
+//   dQ = scale dS K,  dK = scale dS^T Q,  dT[b, h] = sum over windows and pairs with index_ij = b of dS_ij
+//
+// The backward pass recomputes P from q, k and the bias with the row statistics that the forward
+// pass kept, so nothing of size N x N per window ever reaches memory. The bias gradient is summed
+// over the windows of a head inside each block (one N x N partial per block and head), and a second
+// kernel adds the partials and the pairs of a bucket in a fixed order: no atomics, so the same call
+// gives the same bits.
+#include <cuda_bf16.h>
+
+#include "rel_bias.cuh"
+
+namespace fa {
+namespace relb {
+namespace {
+
+using attn::kGroups;
+using attn::kMaskedLog2;
+using attn::kMaskU8;
+using attn::kMaxN;
+using attn::kNoMask;
+
+constexpr int kThreads = 160;  // one thread per query row, then one per key row
+
+template <typename T>
+__device__ __forceinline__ void load_rows(float (*dst)[64], const void* src, const int64_t* st, int w, int h, int N) {
+  const T* base = reinterpret_cast<const T*>(src) + w * st[0] + h * st[1];
+  for (int e = threadIdx.x; e < N * 64; e += kThreads) dst[e >> 6][e & 63] = to_f32(base[(e >> 6) * st[2] + (e & 63)]);
+}
+
+__device__ __forceinline__ float dot64(const float* a, const float* b) {
+  float s = 0.f;
+#pragma unroll
+  for (int d = 0; d < 64; ++d) s = fmaf(a[d], b[d], s);
+  return s;
+}
+
+template <int kMask>
+__device__ __forceinline__ float logit_log2(const Params& p, int h, int w, int i, int j, float s) {
+  float x = fmaf(s, p.scale_log2, bias_log2(p, h, i, j));
+  const int64_t mw = w % p.nW;
+  if (kMask == kGroups && __ldg(p.mask + mw * p.N + i) != __ldg(p.mask + mw * p.N + j)) x += kMaskedLog2;
+  if (kMask == kMaskU8 && __ldg(p.mask + (mw * p.N + i) * p.N + j)) x += kMaskedLog2;
+  return x;
+}
+
+// One thread per query row: two passes over the keys (maximum, then sum and P v).
+template <typename T, int kMask>
+__global__ void __launch_bounds__(kThreads) rel_bias_fwd_kernel(const Params p) {
+  extern __shared__ float sm[];
+  auto sK = reinterpret_cast<float(*)[64]>(sm);
+  auto sV = sK + kMaxN;
+  const int i = threadIdx.x, t_end = tile_end(p.num_tiles);
+  for (int t = tile_begin(p.num_tiles); t < t_end; ++t) {
+    const int h = t / p.Bwin, w = t - h * p.Bwin;
+    __syncthreads();
+    load_rows<T>(sK, p.k, p.sk, w, h, p.N);
+    load_rows<T>(sV, p.v, p.sv, w, h, p.N);
+    __syncthreads();
+    if (i >= p.N) continue;
+    float q[64], o[64];
+    const T* qr = reinterpret_cast<const T*>(p.q) + w * p.sq[0] + h * p.sq[1] + i * p.sq[2];
+    for (int d = 0; d < 64; ++d) {
+      q[d] = to_f32(qr[d]);
+      o[d] = 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+    for (int j = 0; j < p.N; ++j) m = fmaxf(m, logit_log2<kMask>(p, h, w, i, j, dot64(q, sK[j])));
+    for (int j = 0; j < p.N; ++j) {
+      const float e = exp2f(logit_log2<kMask>(p, h, w, i, j, dot64(q, sK[j])) - m);
+      l += e;
+      for (int d = 0; d < 64; ++d) o[d] = fmaf(e, sV[j][d], o[d]);
+    }
+    T* orow = reinterpret_cast<T*>(p.out) + w * p.so[0] + h * p.so[1] + i * p.so[2];
+    for (int d = 0; d < 64; ++d) orow[d] = from_f32<T>(o[d] / l);
+    if (p.stats) p.stats[((int64_t)w * p.H + h) * p.N + i] = make_float2(m, log2f(l));
+  }
+}
+
+// One thread per query row for dQ and the bias gradient, then one per key row for dK and dV.
+template <typename T, int kMask>
+__global__ void __launch_bounds__(kThreads) rel_bias_bwd_kernel(const Params p) {
+  extern __shared__ float sm[];
+  auto sQ = reinterpret_cast<float(*)[64]>(sm);
+  auto sK = sQ + kMaxN;
+  auto sV = sK + kMaxN;
+  auto sG = sV + kMaxN;
+  float2* sStat = reinterpret_cast<float2*>(sG + kMaxN);
+  float* sDelta = reinterpret_cast<float*>(sStat + kMaxN);
+  const int i = threadIdx.x, t_begin = tile_begin(p.num_tiles), t_end = tile_end(p.num_tiles);
+  for (int t = t_begin; t < t_end; ++t) {
+    const int h = t / p.Bwin, w = t - h * p.Bwin;
+    const bool first = t == t_begin || w == 0;  // first window of this head in this block
+    float* slot = p.slots + (int64_t)(blockIdx.x + h) * p.N * p.N;
+    __syncthreads();
+    load_rows<T>(sQ, p.q, p.sq, w, h, p.N);
+    load_rows<T>(sK, p.k, p.sk, w, h, p.N);
+    load_rows<T>(sV, p.v, p.sv, w, h, p.N);
+    load_rows<T>(sG, p.dout, p.so, w, h, p.N);
+    if (i < p.N) sStat[i] = p.stats[((int64_t)w * p.H + h) * p.N + i];
+    __syncthreads();
+    if (i < p.N) {
+      float acc[64];
+      float delta = 0.f;
+      for (int d = 0; d < 64; ++d) acc[d] = 0.f;
+      const float2 st = sStat[i];
+      for (int j = 0; j < p.N; ++j)
+        delta += exp2f(logit_log2<kMask>(p, h, w, i, j, dot64(sQ[i], sK[j])) - st.x - st.y) * dot64(sG[i], sV[j]);
+      for (int j = 0; j < p.N; ++j) {
+        const float e = exp2f(logit_log2<kMask>(p, h, w, i, j, dot64(sQ[i], sK[j])) - st.x - st.y);
+        const float ds = e * (dot64(sG[i], sV[j]) - delta);
+        slot[i * p.N + j] = first ? ds : slot[i * p.N + j] + ds;
+        for (int d = 0; d < 64; ++d) acc[d] = fmaf(ds, sK[j][d], acc[d]);
+      }
+      sDelta[i] = delta;
+      T* row = reinterpret_cast<T*>(p.dq) + w * p.sdq[0] + h * p.sdq[1] + i * p.sdq[2];
+      for (int d = 0; d < 64; ++d) row[d] = from_f32<T>(acc[d] * p.scale);
+    }
+    __syncthreads();
+    if (i < p.N) {
+      const int j = i;
+      float gk[64], gv[64];
+      for (int d = 0; d < 64; ++d) gk[d] = gv[d] = 0.f;
+      for (int r = 0; r < p.N; ++r) {
+        const float e = exp2f(logit_log2<kMask>(p, h, w, r, j, dot64(sQ[r], sK[j])) - sStat[r].x - sStat[r].y);
+        const float ds = e * (dot64(sG[r], sV[j]) - sDelta[r]);
+        for (int d = 0; d < 64; ++d) {
+          gv[d] = fmaf(e, sG[r][d], gv[d]);
+          gk[d] = fmaf(ds, sQ[r][d], gk[d]);
+        }
+      }
+      T* kr = reinterpret_cast<T*>(p.dk) + w * p.sdk[0] + h * p.sdk[1] + j * p.sdk[2];
+      T* vr = reinterpret_cast<T*>(p.dv) + w * p.sdv[0] + h * p.sdv[1] + j * p.sdv[2];
+      for (int d = 0; d < 64; ++d) {
+        kr[d] = from_f32<T>(gk[d] * p.scale);
+        vr[d] = from_f32<T>(gv[d]);
+      }
+    }
+  }
+}
+
+// dT[b, h] = sum over the pairs of bucket b (positions order[offsets[b]] .. in the N x N index) of
+// the head's partials. One block per (bucket, head); every thread adds its share in a fixed order.
+constexpr int kReduceThreads = 128;
+__global__ void __launch_bounds__(kReduceThreads)
+bias_grad_kernel(const float* slots, const int32_t* order, const int32_t* offsets, void* dtable, int dtable_bf16, int H,
+                 int NN, int Bwin, int num_tiles, int grid) {
+  const int b = blockIdx.x, h = blockIdx.y;
+  // Blocks of the main kernel whose tile range meets [h * Bwin, (h + 1) * Bwin): block c covers
+  // [c * T / G, (c + 1) * T / G).
+  float acc = 0.f;
+  if (num_tiles > 0) {
+    const int64_t lo = (int64_t)h * Bwin, hi = lo + Bwin;
+    int c0 = (int)(lo * grid / num_tiles), c1 = (int)((hi - 1) * grid / num_tiles);
+    while (c0 > 0 && (int64_t)c0 * num_tiles / grid > lo) --c0;
+    while (c0 + 1 < grid && (int64_t)(c0 + 1) * num_tiles / grid <= lo) ++c0;
+    while (c1 > 0 && (int64_t)c1 * num_tiles / grid > hi - 1) --c1;
+    while (c1 + 1 < grid && (int64_t)(c1 + 1) * num_tiles / grid <= hi - 1) ++c1;
+    const int p0 = offsets[b], p1 = offsets[b + 1];
+    for (int e = p0 + threadIdx.x; e < p1; e += kReduceThreads) {
+      const int pos = order[e];
+      for (int c = c0; c <= c1; ++c) acc += slots[(int64_t)(c + h) * NN + pos];
+    }
+  }
+  __shared__ float warp_acc[kReduceThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if ((threadIdx.x & 31) == 0) warp_acc[threadIdx.x >> 5] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float s = 0.f;
+    for (int i = 0; i < kReduceThreads / 32; ++i) s += warp_acc[i];
+    const int64_t e = (int64_t)b * H + h;
+    if (dtable_bf16) reinterpret_cast<__nv_bfloat16*>(dtable)[e] = __float2bfloat16_rn(s);
+    else reinterpret_cast<float*>(dtable)[e] = s;
+  }
+}
+
+template <typename T, int kMask>
+int launch_fwd(const Params& p, int grid, cudaStream_t s) {
+  auto kern = rel_bias_fwd_kernel<T, kMask>;
+  constexpr int smem = 2 * kMaxN * 64 * 4;
+  FA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kern<<<grid, kThreads, smem, s>>>(p);
+  return check_launch("rel_bias_fwd_kernel");
+}
+
+template <typename T, int kMask>
+int launch_bwd(const Params& p, int grid, cudaStream_t s) {
+  auto kern = rel_bias_bwd_kernel<T, kMask>;
+  constexpr int smem = 4 * kMaxN * 64 * 4 + kMaxN * 12;
+  FA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kern<<<grid, kThreads, smem, s>>>(p);
+  return check_launch("rel_bias_bwd_kernel");
+}
+
+int grid_of(int64_t tiles) { return (int)(tiles < num_sms() ? tiles : num_sms()); }
+
+// Checks shared by both directions; strides are {window, head, token} triples.
+int check_args(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, const void* const* ptrs, int n_ptrs,
+               const int64_t* strides, const void* table, int table_dtype, const int32_t* index, bool u8, bool ids,
+               int64_t nW) {
+  FA_REQUIRE(precision == FA_ATTN_BF16 || precision == FA_ATTN_FP32_3XTF32, FA_ERR_INVALID,
+             "precision must be FA_ATTN_BF16 or FA_ATTN_FP32_3XTF32");
+  FA_REQUIRE(strides, FA_ERR_INVALID, "null stride pointer");
+  FA_REQUIRE(Bwin >= 0 && H >= 1 && N >= 1, FA_ERR_INVALID, "invalid attention shape");
+  FA_REQUIRE(Dh == 64, FA_ERR_UNSUPPORTED, "window attention supports head_dim 64");
+  FA_REQUIRE(N <= kMaxN, FA_ERR_UNSUPPORTED, "window attention supports N <= 144 tokens");
+  FA_REQUIRE(!(u8 && ids), FA_ERR_INVALID, "pass at most one of mask_u8 / group_ids");
+  FA_REQUIRE(!(u8 || ids) || nW >= 1, FA_ERR_INVALID, "nW must be >= 1 with a mask");
+  FA_REQUIRE(nW < ((int64_t)1 << 31), FA_ERR_INVALID, "too many mask windows");
+  FA_REQUIRE(Bwin < ((int64_t)1 << 31) && H < ((int64_t)1 << 31) && Bwin * H < ((int64_t)1 << 31), FA_ERR_INVALID,
+             "too many (window, head) tiles");
+  FA_REQUIRE(table_dtype == FA_F32 || table_dtype == FA_BF16, FA_ERR_INVALID, "table dtype must be FA_F32 or FA_BF16");
+  FA_REQUIRE(table && index, FA_ERR_INVALID, "null bias table or index");
+  if (Bwin == 0) return FA_OK;
+  const int64_t es = precision == FA_ATTN_FP32_3XTF32 ? 4 : 2;
+  for (int i = 0; i < n_ptrs; ++i) {
+    FA_REQUIRE(ptrs[i], FA_ERR_INVALID, "null tensor pointer");
+    FA_REQUIRE(aligned16(ptrs[i]), FA_ERR_INVALID, "tensors must be 16-byte aligned");
+    for (int j = 0; j < 3; ++j)
+      FA_REQUIRE(strides[3 * i + j] > 0 && (strides[3 * i + j] * es) % 16 == 0, FA_ERR_INVALID,
+                 "strides must be positive multiples of 16 bytes");
+  }
+  return FA_OK;
+}
+
+void copy3(int64_t* dst, const int64_t* src) {
+  for (int i = 0; i < 3; ++i) dst[i] = src[i];
+}
+
+}  // namespace
+}  // namespace relb
+}  // namespace fa
+
+using namespace fa;
+using namespace fa::relb;
+
+extern "C" int64_t fa_window_attention_rel_bias_workspace(int precision, int64_t Bwin, int64_t H, int64_t N,
+                                                          int backward) {
+  if (precision != FA_ATTN_BF16 && precision != FA_ATTN_FP32_3XTF32)
+    return set_error(FA_ERR_INVALID, "precision must be FA_ATTN_BF16 or FA_ATTN_FP32_3XTF32");
+  if (Bwin < 0 || H < 1 || N < 1 || N > kMaxN || Bwin >= ((int64_t)1 << 31) || H >= ((int64_t)1 << 31) ||
+      Bwin * H >= ((int64_t)1 << 31))
+    return set_error(FA_ERR_INVALID, "invalid attention shape");
+  return backward ? (grid_of(Bwin * H) + H) * N * N * 4 : 0;
+}
+
+extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh,
+                                            const void* q, const void* k, const void* v, void* out,
+                                            const int64_t strides[12], const void* table, int table_dtype,
+                                            const int32_t* index, const uint8_t* mask_u8, const uint8_t* group_ids,
+                                            int64_t nW, float scale, float* stats, void* workspace,
+                                            int64_t workspace_bytes, void* stream) {
+  const void* ptrs[4] = {q, k, v, out};
+  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 4, strides, table, table_dtype, index, mask_u8 != nullptr,
+                      group_ids != nullptr, nW);
+  if (rc != FA_OK || Bwin == 0) return rc;
+  const int64_t need = fa_window_attention_rel_bias_workspace(precision, Bwin, H, N, 0);
+  FA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), FA_ERR_INVALID, "workspace too small");
+  Params p{};
+  p.Bwin = (int)Bwin; p.H = (int)H; p.N = (int)N; p.nW = (int)(nW > 0 ? nW : 1);
+  p.num_tiles = (int)(Bwin * H);
+  p.scale = scale; p.scale_log2 = scale * kLog2e;
+  p.q = q; p.k = k; p.v = v; p.out = out;
+  copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
+  p.table = table; p.table_bf16 = table_dtype == FA_BF16; p.index = index;
+  p.mask = mask_u8 ? mask_u8 : group_ids;
+  p.stats = reinterpret_cast<float2*>(stats);
+  cudaStream_t s = (cudaStream_t)stream;
+  const int grid = grid_of(p.num_tiles);
+  if (precision == FA_ATTN_BF16) {
+    if (mask_u8) return launch_fwd<__nv_bfloat16, kMaskU8>(p, grid, s);
+    if (group_ids) return launch_fwd<__nv_bfloat16, kGroups>(p, grid, s);
+    return launch_fwd<__nv_bfloat16, kNoMask>(p, grid, s);
+  }
+  if (mask_u8) return launch_fwd<float, kMaskU8>(p, grid, s);
+  if (group_ids) return launch_fwd<float, kGroups>(p, grid, s);
+  return launch_fwd<float, kNoMask>(p, grid, s);
+}
+
+extern "C" int fa_window_attention_rel_bias_backward(
+    int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, const void* q, const void* k, const void* v,
+    const void* dout, void* dq, void* dk, void* dv, const int64_t strides[21], const void* table, int table_dtype,
+    const int32_t* index, const uint8_t* mask_u8, const uint8_t* group_ids, int64_t nW, float scale,
+    const float* stats, const int32_t* order, const int32_t* offsets, int64_t num_buckets, void* dtable,
+    void* workspace, int64_t workspace_bytes, void* stream) {
+  const void* ptrs[7] = {q, k, v, dout, dq, dk, dv};
+  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 7, strides, table, table_dtype, index, mask_u8 != nullptr,
+                      group_ids != nullptr, nW);
+  if (rc != FA_OK) return rc;
+  FA_REQUIRE(stats || Bwin == 0, FA_ERR_INVALID, "null row statistics");
+  FA_REQUIRE(!dtable || (order && offsets && num_buckets >= 1 && num_buckets < ((int64_t)1 << 31) && H <= 65535),
+             FA_ERR_INVALID, "a bias gradient needs the bucket lists (and at most 65535 heads)");
+  cudaStream_t s = (cudaStream_t)stream;
+  const int64_t need = fa_window_attention_rel_bias_workspace(precision, Bwin, H, N, 1);
+  FA_REQUIRE(Bwin == 0 || (workspace && workspace_bytes >= need), FA_ERR_INVALID, "workspace too small");
+  const int grid = grid_of(Bwin * H);
+  if (Bwin > 0) {
+    Params p{};
+    p.Bwin = (int)Bwin; p.H = (int)H; p.N = (int)N; p.nW = (int)(nW > 0 ? nW : 1);
+    p.num_tiles = (int)(Bwin * H);
+    p.scale = scale; p.scale_log2 = scale * kLog2e;
+    p.q = q; p.k = k; p.v = v; p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
+    copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
+    copy3(p.sdq, strides + 12); copy3(p.sdk, strides + 15); copy3(p.sdv, strides + 18);
+    p.table = table; p.table_bf16 = table_dtype == FA_BF16; p.index = index;
+    p.mask = mask_u8 ? mask_u8 : group_ids;
+    p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats));
+    p.slots = reinterpret_cast<float*>(workspace);
+    if (precision == FA_ATTN_BF16) {
+      rc = mask_u8 ? launch_bwd<__nv_bfloat16, kMaskU8>(p, grid, s)
+                   : group_ids ? launch_bwd<__nv_bfloat16, kGroups>(p, grid, s)
+                               : launch_bwd<__nv_bfloat16, kNoMask>(p, grid, s);
+    } else {
+      rc = mask_u8 ? launch_bwd<float, kMaskU8>(p, grid, s)
+                   : group_ids ? launch_bwd<float, kGroups>(p, grid, s)
+                               : launch_bwd<float, kNoMask>(p, grid, s);
+    }
+    if (rc != FA_OK) return rc;
+  }
+  if (!dtable) return FA_OK;
+  bias_grad_kernel<<<dim3((unsigned)num_buckets, (unsigned)H), kReduceThreads, 0, s>>>(
+      reinterpret_cast<const float*>(workspace), order, offsets, dtable, table_dtype == FA_BF16, (int)H, (int)(N * N),
+      (int)Bwin, (int)(Bwin * H), grid);
+  return check_launch("bias_grad_kernel");
+}

@@ -1,0 +1,343 @@
+"""Window attention with a learned relative position bias by buckets, differentiable.
+
+    out = softmax(q k^T * scale + table[index[i, j], h] + mask) v
+
+beside :mod:`flash_aurora_b200.window_attn`, whose kernels take only the 0 / -100 mask. ``table``
+``(num_buckets, H)`` is the learned parameter (the ``relative_position_bias_table`` of Swin models);
+:class:`RelativeBuckets` says which bucket each (query, key) pair of a window reads. Gradients reach
+q, k, v (or the packed qkv) and the table. Windows hold 1 to 144 tokens, head_dim is 64, tensors are
+bfloat16 or float32 (3xTF32 products, fp32 accuracy); masks as in ``window_attn``: region ids or a
+float bias below -50, each adding -100 to a masked logit.
+
+Nothing is kept between calls: the backward pass recomputes the probabilities from q, k, the table
+and the row statistics of its own forward call. Sums run in a fixed order, so equal calls give equal
+bits. Gradients of gradients are not available.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .window_attn import _mask_args
+
+__all__ = ["RelativeBuckets", "window_attn_rel_bias", "window_attn_rel_bias_qkvpacked"]
+
+_MAX_TOKENS = 144
+_HEAD_DIM = 64
+
+
+class RelativeBuckets:
+    """The bucket of every (query, key) pair of a window: ``index (N, N)`` integers in
+    ``[0, num_buckets)``, with the pairs of each bucket listed for the table's gradient.
+
+    Built once per window shape and device (the range check reads the index on the host). The index
+    is copied: changing the given tensor later has no effect.
+    """
+
+    def __init__(self, index: torch.Tensor, num_buckets: int, device: Optional[torch.device] = None) -> None:
+        if index.ndim != 2 or index.shape[0] != index.shape[1] or not 1 <= index.shape[0] <= _MAX_TOKENS:
+            raise ValueError(f"index must be (N, N) with 1 <= N <= {_MAX_TOKENS}, got {tuple(index.shape)}")
+        if index.dtype not in (torch.uint8, torch.int16, torch.int32, torch.int64):
+            raise ValueError(f"index must hold integers, got {index.dtype}")
+        num_buckets = int(num_buckets)
+        if not 1 <= num_buckets <= 2 ** 31 - 1:
+            raise ValueError(f"num_buckets must be positive, got {num_buckets}")
+        flat = index.detach().reshape(-1).to("cpu", torch.int64)
+        if int(flat.min()) < 0 or int(flat.max()) >= num_buckets:
+            raise ValueError(f"index holds values outside [0, {num_buckets})")
+        dev = index.device if device is None else torch.device(device)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        offsets = torch.zeros(num_buckets + 1, dtype=torch.int64)
+        offsets[1:] = torch.cumsum(torch.bincount(flat, minlength=num_buckets), 0)
+        self.tokens = int(index.shape[0])
+        self.num_buckets = num_buckets
+        self.device = dev
+        self.index = flat.view(self.tokens, self.tokens).to(torch.int32).to(dev)
+        self.order = torch.argsort(flat, stable=True).to(torch.int32).to(dev)
+        self.offsets = offsets.to(torch.int32).to(dev)
+
+    def to(self, device) -> "RelativeBuckets":
+        """These buckets on ``device`` (this object if it is there already)."""
+        dev = torch.device(device)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        return self if dev == self.device else RelativeBuckets(self.index, self.num_buckets, dev)
+
+    @classmethod
+    def window(cls, window_size, device: Optional[torch.device] = None) -> "RelativeBuckets":
+        """One bucket per 3-D offset of a ``(wc, wh, ww)`` window, ``(2wc-1)(2wh-1)(2ww-1)`` in all, in
+        the order of Swin's ``relative_position_index``."""
+        w = tuple(int(v) for v in window_size)
+        if len(w) != 3 or min(w) < 1:
+            raise ValueError(f"window_size must be three positive integers, got {tuple(window_size)}")
+        pos = torch.cartesian_prod(*(torch.arange(v) for v in w)).view(-1, 3)
+        rel = pos[:, None, :] - pos[None, :, :] + torch.tensor([v - 1 for v in w])
+        span = [2 * v - 1 for v in w]
+        index = (rel[..., 0] * span[1] + rel[..., 1]) * span[2] + rel[..., 2]
+        return cls(index, span[0] * span[1] * span[2], device if device is not None else torch.device("cpu"))
+
+    @classmethod
+    def log_distance(cls, tokens: int, num_buckets: int = 32, max_distance: int = 128,
+                     device: Optional[torch.device] = None) -> "RelativeBuckets":
+        """Buckets of the signed distance ``j - i`` along one axis: half of them for keys after the
+        query; in each half the distances below ``num_buckets / 4`` have a bucket of their own and the
+        rest share logarithmically wider ones up to ``max_distance`` (and beyond)."""
+        if num_buckets < 4 or num_buckets % 4 or max_distance <= num_buckets // 4:
+            raise ValueError("num_buckets must be a multiple of 4 and max_distance above num_buckets / 4")
+        rel = torch.arange(tokens)[None, :] - torch.arange(tokens)[:, None]
+        half, exact = num_buckets // 2, num_buckets // 4
+        dist = rel.abs()
+        far = exact + (torch.log(dist.clamp(min=1).double() / exact) / math.log(max_distance / exact)
+                       * (half - exact)).long()
+        index = torch.where(dist < exact, dist, far.clamp(max=half - 1)) + torch.where(rel > 0, half, 0)
+        return cls(index, num_buckets, device if device is not None else torch.device("cpu"))
+
+
+def _check_bias(table: torch.Tensor, buckets: RelativeBuckets, H: int, N: int, device: torch.device) -> None:
+    if not isinstance(buckets, RelativeBuckets):
+        raise TypeError("buckets must be a RelativeBuckets")
+    if buckets.tokens != N:
+        raise ValueError(f"buckets are of a window of {buckets.tokens} tokens, the tensors hold {N}")
+    if tuple(table.shape) != (buckets.num_buckets, H):
+        raise ValueError(f"table must have shape (num_buckets, heads) = {(buckets.num_buckets, H)}, "
+                         f"got {tuple(table.shape)}")
+    if table.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"table must be float32 or bfloat16, got {table.dtype}")
+    if table.device != device or buckets.device != device:
+        raise ValueError(f"table ({table.device}) and buckets ({buckets.device}) must be on {device}")
+
+
+def _strided(t: torch.Tensor) -> torch.Tensor:
+    """``t (Bwin, H, N, Dh)`` as the kernels can read it: unit head-dim stride, positive strides of
+    whole 16-byte units, an aligned base; anything else is copied."""
+    unit = 16 // t.element_size()
+    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
+            and all(s > 0 and s % unit == 0 or n == 1 for s, n in zip(t.stride()[:3], t.shape[:3]))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _precision(dtype: torch.dtype) -> int:
+    return _lib.FA_ATTN_BF16 if dtype == torch.bfloat16 else _lib.FA_ATTN_FP32_3XTF32
+
+
+def _workspace(prec: int, Bwin: int, H: int, N: int, backward: int, device) -> Optional[torch.Tensor]:
+    n = _lib.load().fa_window_attention_rel_bias_workspace(prec, Bwin, H, N, backward)
+    if n < 0:
+        _lib.check(int(n), "window_attn_rel_bias")
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
+
+
+def _strides(*tensors: torch.Tensor):
+    """Window, head and token strides of each tensor; an axis of one entry gets a legal stride."""
+    flat = [s if n > 1 else _HEAD_DIM for t in tensors for s, n in zip(t.stride()[:3], t.shape[:3])]
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+class _Call:
+    """One attention call's arguments besides its tensors. ``kind``: None, "mask_u8" or "group_ids"."""
+
+    def __init__(self, buckets, kind, nW, scale) -> None:
+        self.buckets, self.kind, self.nW, self.scale = buckets, kind, nW, scale
+
+    def masks(self, mask: Optional[torch.Tensor]):
+        """The C arguments mask_u8, group_ids, nW, scale."""
+        return (_ptr(mask) if self.kind == "mask_u8" else None, _ptr(mask) if self.kind == "group_ids" else None,
+                self.nW, self.scale)
+
+
+def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool) -> Optional[torch.Tensor]:
+    """Launch the forward kernel into ``out``; returns the row statistics when asked for."""
+    Bwin, H, N, Dh = q.shape
+    dev = q.device
+    with torch.cuda.device(dev):
+        stats = torch.empty(Bwin, H, N, 2, device=dev, dtype=torch.float32) if want_stats else None
+        prec = _precision(q.dtype)
+        ws = _workspace(prec, Bwin, H, N, 0, dev)
+        rc = _lib.load().fa_window_attention_rel_bias(
+            prec, Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(q, k, v, out),
+            table.data_ptr(), _lib.dtype_code(table.dtype), call.buckets.index.data_ptr(), *call.masks(mask),
+            _ptr(stats), _ptr(ws), ws.numel() if ws is not None else 0, _lib.stream_ptr(dev))
+        _lib.check(rc, "window_attn_rel_bias")
+    return stats
+
+
+def _backward(q, k, v, dout, dq, dk, dv, table, mask, call: _Call, stats, want_table: bool) -> Optional[torch.Tensor]:
+    """Launch the backward kernels into ``dq``, ``dk``, ``dv``; returns the table's gradient when asked for."""
+    Bwin, H, N, Dh = q.shape
+    dev = q.device
+    b = call.buckets
+    with torch.cuda.device(dev):
+        dtable = torch.empty_like(table, memory_format=torch.contiguous_format) if want_table else None
+        prec = _precision(q.dtype)
+        ws = _workspace(prec, Bwin, H, N, 1, dev)
+        rc = _lib.load().fa_window_attention_rel_bias_backward(
+            prec, Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), _strides(q, k, v, dout, dq, dk, dv), table.data_ptr(),
+            _lib.dtype_code(table.dtype), b.index.data_ptr(), *call.masks(mask), stats.data_ptr(), b.order.data_ptr(),
+            b.offsets.data_ptr(), b.num_buckets, _ptr(dtable), _ptr(ws), ws.numel() if ws is not None else 0,
+            _lib.stream_ptr(dev))
+        _lib.check(rc, "window_attn_rel_bias backward")
+    return dtable
+
+
+def _same_heads(t: torch.Tensor, bnc: bool, H: int) -> torch.Tensor:
+    """``(Bwin, H, N, Dh)`` view of an output or its gradient in either layout."""
+    if bnc:
+        return t.view(t.shape[0], t.shape[1], H, _HEAD_DIM).permute(0, 2, 1, 3)
+    return t
+
+
+class _Attn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, mask, call):
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        stats = _forward(q, k, v, out, table, mask, call, True)
+        ctx.save_for_backward(q, k, v, table, mask, stats)
+        ctx.call = call
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, mask, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv = (torch.empty(q.shape, device=q.device, dtype=q.dtype) for _ in range(3))
+        dtable = _backward(q, k, v, _strided(dout), dq, dk, dv, table, mask, ctx.call, stats, need[3])
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None
+
+
+class _AttnPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, table, mask, call, H, bnc):
+        out, stats = _packed_forward(qkv, table, mask, call, H, bnc, True)
+        ctx.save_for_backward(qkv, table, mask, stats)
+        ctx.call, ctx.H, ctx.bnc = call, H, bnc
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv, table, mask, stats = ctx.saved_tensors
+        dqkv = torch.empty_like(qkv)
+        dout = _strided(_same_heads(dout.contiguous() if ctx.bnc else dout, ctx.bnc, ctx.H))
+        dtable = _backward(*_heads_of(qkv, ctx.H), dout, *_heads_of(dqkv, ctx.H), table, mask, ctx.call, stats,
+                           ctx.needs_input_grad[1])
+        return dqkv if ctx.needs_input_grad[0] else None, dtable, None, None, None, None
+
+
+def _heads_of(qkv: torch.Tensor, H: int):
+    """q, k, v as ``(Bwin, H, N, Dh)`` views of a packed ``(Bwin, N, 3 * H * Dh)`` tensor."""
+    Bwin, N, _ = qkv.shape
+    return qkv.view(Bwin, N, 3, H, _HEAD_DIM).permute(2, 0, 3, 1, 4).unbind(0)
+
+
+def _packed_forward(qkv, table, mask, call, H, bnc, want_stats):
+    Bwin, N, _ = qkv.shape
+    shape = (Bwin, N, H * _HEAD_DIM) if bnc else (Bwin, H, N, _HEAD_DIM)
+    out = torch.empty(shape, device=qkv.device, dtype=qkv.dtype)
+    return out, _forward(*_heads_of(qkv, H), _same_heads(out, bnc, H), table, mask, call, want_stats)
+
+
+def _check_window(N: int, Dh: int) -> None:
+    if Dh != _HEAD_DIM:
+        raise ValueError(f"window attention supports head_dim {_HEAD_DIM}, got {Dh}")
+    if not 1 <= N <= _MAX_TOKENS:
+        raise ValueError(f"window attention supports 1 to {_MAX_TOKENS} tokens per window, got {N}")
+
+
+def _call_args(t, N, H, table, buckets, bias, group_ids, scale_qk):
+    if bias is not None and group_ids is not None:
+        raise ValueError("pass at most one of bias / group_ids")
+    _check_bias(table, buckets, H, N, t.device)
+    with torch.cuda.device(t.device):
+        mask_u8, gids, nW, _ = _mask_args(bias, group_ids, t.device, N)
+    if (mask_u8 is not None or gids is not None) and nW < 1:
+        raise ValueError("a mask needs at least one window")
+    scale = 1.0 / math.sqrt(_HEAD_DIM) if scale_qk is None else float(scale_qk)
+    kind = "mask_u8" if mask_u8 is not None else "group_ids" if gids is not None else None
+    return table.contiguous(), mask_u8 if mask_u8 is not None else gids, _Call(buckets, kind, nW, scale)
+
+
+def window_attn_rel_bias(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    table: torch.Tensor,
+    buckets: RelativeBuckets,
+    bias: Optional[torch.Tensor] = None,
+    *,
+    scale_qk: Optional[float] = None,
+    group_ids: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention on ``q, k, v (Bwin, H, N, 64)`` (bfloat16 or float32, one dtype) with the bias
+    ``table[buckets.index, h]`` and an optional mask: ``bias (nW, N, N)`` (below -50 means masked) or
+    ``group_ids (nW, N)`` uint8. Window ``b`` reads mask ``b % nW``. Returns ``(Bwin, H, N, 64)``."""
+    if q.ndim != 4 or q.shape != k.shape or q.shape != v.shape:
+        raise ValueError("q, k, v must all be (Bwin, H, N, Dh)")
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"window_attn_rel_bias supports bfloat16 and float32; got {q.dtype}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must share a dtype")
+    Bwin, H, N, Dh = q.shape
+    _check_window(N, Dh)
+    if H < 1:
+        raise ValueError("at least one head is needed")
+    if not q.is_cuda:
+        raise RuntimeError("B200 window attention requires CUDA tensors.")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must be on one device")
+    table, mask, call = _call_args(q, N, H, table, buckets, bias, group_ids, scale_qk)
+    q, k, v = _strided(q), _strided(k), _strided(v)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table)):
+        return _Attn.apply(q, k, v, table, mask, call)
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    _forward(q, k, v, out, table, mask, call, False)
+    return out
+
+
+def window_attn_rel_bias_qkvpacked(
+    qkv: torch.Tensor,
+    num_heads: int,
+    table: torch.Tensor,
+    buckets: RelativeBuckets,
+    bias: Optional[torch.Tensor] = None,
+    *,
+    scale_qk: Optional[float] = None,
+    output_layout: str = "bhnd",
+    group_ids: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """:func:`window_attn_rel_bias` on the packed ``Linear(D, 3D)`` output ``(Bwin, N, 3 * H * 64)``,
+    contiguous. Returns ``(Bwin, H, N, 64)``, or ``(Bwin, N, H * 64)`` with ``output_layout="bnc"``."""
+    if qkv.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"qkv-packed path supports bfloat16 and float32; got {qkv.dtype}")
+    if qkv.ndim != 3:
+        raise ValueError(f"qkv must have shape (Bwin, N, 3*C); got {tuple(qkv.shape)}")
+    if not qkv.is_contiguous():
+        raise ValueError("qkv-packed path requires contiguous qkv linear output")
+    if num_heads < 1 or qkv.shape[-1] % (3 * num_heads) != 0:
+        raise ValueError(f"last dim {qkv.shape[-1]} must be divisible by 3*num_heads={3 * num_heads}")
+    if output_layout not in {"bhnd", "bnc"}:
+        raise ValueError(f"output_layout must be 'bhnd' or 'bnc', got {output_layout!r}")
+    Bwin, N, three_c = qkv.shape
+    H = int(num_heads)
+    _check_window(N, three_c // (3 * H))
+    if not qkv.is_cuda:
+        raise RuntimeError("B200 window attention requires CUDA tensors.")
+    table, mask, call = _call_args(qkv, N, H, table, buckets, bias, group_ids, scale_qk)
+    if qkv.data_ptr() % 16:
+        qkv = qkv.clone()
+    bnc = output_layout == "bnc"
+    if torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad):
+        return _AttnPacked.apply(qkv, table, mask, call, H, bnc)
+    return _packed_forward(qkv, table, mask, call, H, bnc, False)[0]
