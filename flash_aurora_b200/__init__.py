@@ -10,6 +10,7 @@ PyTorch host layer that mirrors the operator interface of upstream Flash-Aurora:
                      (upstream ``ops/triton_adaln.py``)
 * ``window_attn``    WinAttnPrecision, window_attn_fwd_cute, window_attn_fwd_cute_qkvpacked,
                      window_attn_dispatch (upstream ``ops/cute/window_attn_fwd.py``)
+* ``block_norm``     norms before / after / between blocks with gate and residual scale, differentiable
 * ``rel_bias``       window attention with a learned relative position bias by buckets, differentiable
 * ``swin3d``         Swin3DTransformerBlock / Swin3DTransformerBackbone with upstream state-dict
                      keys (upstream ``aurora/model/swin3d.py``, ``film.py``)
@@ -46,6 +47,7 @@ from .window_attn import (
     window_attn_fwd_cute,
     window_attn_fwd_cute_qkvpacked,
 )
+from .block_norm import block_postnorm_residual, block_postnorm_residual_prenorm, block_prenorm
 from .rel_bias import RelativeBuckets, window_attn_rel_bias, window_attn_rel_bias_qkvpacked
 from .workspace_pool import InferenceWorkspacePool
 from .status import DeviceStatusError, check_device_status, device_status, reset_device_status, watchdog_selftest
@@ -85,6 +87,9 @@ __all__ = [
     "window_attn_dispatch",
     "window_attn_fwd_cute",
     "window_attn_fwd_cute_qkvpacked",
+    "block_prenorm",
+    "block_postnorm_residual",
+    "block_postnorm_residual_prenorm",
     "RelativeBuckets",
     "window_attn_rel_bias",
     "window_attn_rel_bias_qkvpacked",

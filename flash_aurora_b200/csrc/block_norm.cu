@@ -1,0 +1,605 @@
+// The norms before and after a residual block, fused with the block's gate and residual scale, and
+// their gradients. With N(v) the layer norm (or RMS norm) of a row, without affine:
+//
+//   before   z = N(x) (c2 + s2) + t2                                       x -> the block's input
+//   after    y = a r + g (N(x) (c + s) + t)                                the block's output x, residual r
+//   between  y as in after, z = N(y) (c2 + s2) + t2                        one block's end, the next one's start
+//
+// s, t, g, a, s2, t2 are per channel, shared or one row per batch element. Everything is computed in
+// fp32 and rounded once per output; z of `between` is computed from the unrounded y.
+//
+// Backward, with n = N(x), p = n (c + s) + t, m = N(y) and the row statistics the forward pass kept:
+//   d = dy + rho2 (dm - mean(dm) - m mean(dm m)),  dm = dz (c2 + s2)       (no mean(dm) for RMS)
+//   dr = a d,  dx = rho (dn - mean(dn) - n mean(dn n)),  dn = g d (c + s)
+//   ds = sum g d n, dt = sum g d, dg = sum d p, da = sum d r, ds2 = sum dz m, dt2 = sum dz
+// The sums over rows are kept in registers by the threads that own the columns, added over a block's
+// row groups in shared memory, and over blocks by a second kernel in a fixed order (no atomics).
+//
+// All of it is bound by memory: a row is read once and held in registers by its group of `tpr` threads.
+// The variance is taken about the mean (two reductions), not as E[x^2] - mean^2.
+#include "fa_common.cuh"
+
+namespace fa {
+namespace {
+
+enum { kBefore = 0, kAfter = 1, kBetween = 2 };
+enum { kPostScale = 0, kPostShift, kGate, kResScale, kPreScale, kPreShift, kParams };
+constexpr int kMaxDim = 4096;
+constexpr int kFwdThreads = 128;
+
+struct NormArgs {
+  const void *x, *r, *dy, *dz;
+  void *y, *z, *dx, *dr;
+  const float* par[kParams];
+  int64_t par_stride[kParams];  // batch stride: 0 (shared) or D
+  float scale_bias, pre_scale_bias, res_scale, eps, inv_d;
+  int rms, D, tpr;
+  int64_t L;
+  int B;
+  float4* stats;  // per row: mean and 1 / deviation of x, and of y
+  float* ws;      // backward: (B, gridDim.x, sums, D) partial column sums
+};
+
+// ------------------------------------------------------------------------------------------
+// A row's elements of one thread: kVec: 8 consecutive ones per unit, units tpr apart; else single
+// elements tpr apart (both coalesced). kN elements per thread; columns past D read as zero.
+// ------------------------------------------------------------------------------------------
+template <bool kVec>
+__device__ __forceinline__ int col_of(int t, int tpr, int k) {
+  return kVec ? (t + tpr * (k >> 3)) * 8 + (k & 7) : t + tpr * k;
+}
+
+template <typename T, bool kVec, int kN>
+__device__ __forceinline__ void load_row(const T* row, int t, int tpr, int D, bool on, float (&v)[kN]) {
+#pragma unroll
+  for (int u = 0; u < kN; u += 8) {
+    if constexpr (kVec) {
+      const int c = col_of<true>(t, tpr, u);
+      if (on && c < D) {
+        Vec8<T>::load_stream(row + c, &v[u]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[u + k] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int c = col_of<false>(t, tpr, u + k);
+        v[u + k] = on && c < D ? to_f32(row[c]) : 0.f;
+      }
+    }
+  }
+}
+
+template <typename T, bool kVec, int kN>
+__device__ __forceinline__ void store_row(T* row, int t, int tpr, int D, bool on, const float (&v)[kN]) {
+  if (!on) return;
+#pragma unroll
+  for (int u = 0; u < kN; u += 8) {
+    if constexpr (kVec) {
+      const int c = col_of<true>(t, tpr, u);
+      if (c < D) Vec8<T>::store(row + c, &v[u]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int c = col_of<false>(t, tpr, u + k);
+        if (c < D) row[c] = from_f32<T>(v[u + k]);
+      }
+    }
+  }
+}
+
+// Columns u .. u+7 of this thread of a parameter row (null: `fill` everywhere).
+template <bool kVec>
+__device__ __forceinline__ void param8(const float* p, int t, int tpr, int D, int u, float add, float fill,
+                                       float (&v)[8]) {
+  if (!p) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = fill;
+  } else if constexpr (kVec) {
+    const int c = col_of<true>(t, tpr, u);
+    if (c < D) {
+      Vec8<float>::load(p + c, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += add;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = col_of<false>(t, tpr, u + k);
+      v[k] = c < D ? __ldg(p + c) + add : 0.f;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Sums over the threads of a row: shuffles inside a warp (rows narrower than a warp share one), and
+// one named barrier per sum across warps; `buf` alternates so that one barrier is enough.
+// ------------------------------------------------------------------------------------------
+struct Group {
+  int tpr, id, t;  // threads per row, row group in the block, thread in the group
+  float* buf;      // 2 x 2 x (tpr / 32) floats of this group
+  int par;
+};
+
+template <int kVals>
+__device__ __forceinline__ void group_sum(Group& g, float (&v)[kVals]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (o < g.tpr) {
+#pragma unroll
+      for (int i = 0; i < kVals; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+  }
+  if (g.tpr > 32) {
+    const int warps = g.tpr >> 5;
+    float* b = g.buf + g.par * kVals * warps;
+    g.par ^= 1;
+    if ((g.t & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < kVals; ++i) b[i * warps + (g.t >> 5)] = v[i];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(g.id + 1), "r"(g.tpr) : "memory");
+#pragma unroll
+    for (int i = 0; i < kVals; ++i) {
+      float s = 0.f;
+      for (int w = 0; w < warps; ++w) s += b[i * warps + w];
+      v[i] = s;
+    }
+  }
+}
+
+// Mean and 1 / deviation of a row held by a group; v becomes the normalised row.
+template <bool kVec, int kN>
+__device__ __forceinline__ float2 normalise(Group& g, const NormArgs& a, float (&v)[kN]) {
+  float s[1] = {0.f};
+  float mean = 0.f;
+  if (!a.rms) {
+#pragma unroll
+    for (int k = 0; k < kN; ++k) s[0] += v[k];
+    group_sum<1>(g, s);
+    mean = s[0] * a.inv_d;
+  }
+  s[0] = 0.f;
+#pragma unroll
+  for (int k = 0; k < kN; ++k) {
+    v[k] = col_of<kVec>(g.t, g.tpr, k) < a.D ? v[k] - mean : 0.f;
+    s[0] = fmaf(v[k], v[k], s[0]);
+  }
+  group_sum<1>(g, s);
+  const float rstd = rsqrtf(fmaf(s[0], a.inv_d, a.eps));
+#pragma unroll
+  for (int k = 0; k < kN; ++k) v[k] *= rstd;
+  return make_float2(mean, rstd);
+}
+
+// kVpt units of 8 elements per thread. YT: the type of r and y, or of z in the `before` form.
+template <typename XT, typename YT, int kForm, bool kVec, int kVpt>
+__global__ void __launch_bounds__(kFwdThreads) block_norm_kernel(const NormArgs a) {
+  constexpr int kN = 8 * kVpt;
+  __shared__ float buf[2 * kFwdThreads / 32];
+  Group g;
+  g.tpr = a.tpr;
+  g.id = threadIdx.x / a.tpr;
+  g.t = threadIdx.x - g.id * a.tpr;
+  g.buf = buf + 2 * (g.id * a.tpr >> 5);
+  g.par = 0;
+  const int groups = kFwdThreads / a.tpr;
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
+    const float* par[kParams];
+#pragma unroll
+    for (int i = 0; i < kParams; ++i) par[i] = a.par[i] ? a.par[i] + b * a.par_stride[i] : nullptr;
+    for (int64_t row0 = (int64_t)blockIdx.x * groups; row0 < a.L; row0 += (int64_t)gridDim.x * groups) {
+      const bool on = row0 + g.id < a.L;
+      const int64_t row = (int64_t)b * a.L + row0 + g.id, off = row * a.D;
+      float v[kN], r[kForm == kBefore ? 8 : kN];
+      load_row<XT, kVec>(reinterpret_cast<const XT*>(a.x) + off, g.t, g.tpr, a.D, on, v);
+      if constexpr (kForm != kBefore) load_row<YT, kVec>(reinterpret_cast<const YT*>(a.r) + off, g.t, g.tpr, a.D, on, r);
+      float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float2 sx = normalise<kVec>(g, a, v);
+      st.x = sx.x;
+      st.y = sx.y;
+      if constexpr (kForm != kBefore) {
+#pragma unroll
+        for (int u = 0; u < kN; u += 8) {
+          float s[8], t[8], gt[8], rs[8];
+          param8<kVec>(par[kPostScale], g.t, g.tpr, a.D, u, a.scale_bias, a.scale_bias, s);
+          param8<kVec>(par[kPostShift], g.t, g.tpr, a.D, u, 0.f, 0.f, t);
+          param8<kVec>(par[kGate], g.t, g.tpr, a.D, u, 0.f, 1.f, gt);
+          param8<kVec>(par[kResScale], g.t, g.tpr, a.D, u, 0.f, a.res_scale, rs);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[u + k] = fmaf(gt[k], fmaf(v[u + k], s[k], t[k]), rs[k] * r[u + k]);
+        }
+        store_row<YT, kVec>(reinterpret_cast<YT*>(a.y) + off, g.t, g.tpr, a.D, on, v);
+        if constexpr (kForm == kBetween) {
+          const float2 sy = normalise<kVec>(g, a, v);
+          st.z = sy.x;
+          st.w = sy.y;
+        }
+      }
+      if constexpr (kForm != kAfter) {
+#pragma unroll
+        for (int u = 0; u < kN; u += 8) {
+          float s[8], t[8];
+          param8<kVec>(par[kPreScale], g.t, g.tpr, a.D, u, a.pre_scale_bias, a.pre_scale_bias, s);
+          param8<kVec>(par[kPreShift], g.t, g.tpr, a.D, u, 0.f, 0.f, t);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[u + k] = fmaf(v[u + k], s[k], t[k]);
+        }
+        using ZT = typename std::conditional<kForm == kBefore, YT, XT>::type;
+        store_row<ZT, kVec>(reinterpret_cast<ZT*>(a.z) + off, g.t, g.tpr, a.D, on, v);
+      }
+      if (a.stats && on && g.t == 0) a.stats[row] = st;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Backward: 8 elements per thread, tpr = 1 .. 512 threads per row.
+// ------------------------------------------------------------------------------------------
+template <int kForm> constexpr int kSums = kForm == kBefore ? 2 : kForm == kAfter ? 4 : 6;
+constexpr int kBwdMaxThreads = 512;
+constexpr int kCombine = 1024;  // widest row that shares a block with another
+
+template <typename XT, typename YT, int kForm, bool kVec>
+__global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const NormArgs a) {
+  constexpr int kS = kSums<kForm>;
+  constexpr int kPost = 0, kPre = kForm == kBefore ? 0 : 4;  // first sum of each norm
+  using ZT = typename std::conditional<kForm == kBefore, YT, XT>::type;
+  __shared__ float buf[4 * kBwdMaxThreads / 32];
+  __shared__ float comb[kS * kCombine];
+  Group g;
+  g.tpr = a.tpr;
+  g.id = threadIdx.x / a.tpr;
+  g.t = threadIdx.x - g.id * a.tpr;
+  g.buf = buf + 4 * (g.id * a.tpr >> 5);
+  g.par = 0;
+  const int groups = blockDim.x / a.tpr, D = a.D;
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
+    const float* par[kParams];
+#pragma unroll
+    for (int i = 0; i < kParams; ++i) par[i] = a.par[i] ? a.par[i] + b * a.par_stride[i] : nullptr;
+    float acc[kS][8];
+#pragma unroll
+    for (int i = 0; i < kS; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[i][k] = 0.f;
+    for (int64_t row0 = (int64_t)blockIdx.x * groups; row0 < a.L; row0 += (int64_t)gridDim.x * groups) {
+      const bool on = row0 + g.id < a.L;
+      const int64_t row = (int64_t)b * a.L + row0 + g.id, off = row * D;
+      const float4 st = on ? __ldg(a.stats + row) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float n[8];  // x, then the normalised row
+      load_row<XT, kVec>(reinterpret_cast<const XT*>(a.x) + off, g.t, g.tpr, D, on, n);
+      float r[8], d[8], z[8];
+      if constexpr (kForm != kBefore) {
+        load_row<YT, kVec>(reinterpret_cast<const YT*>(a.r) + off, g.t, g.tpr, D, on, r);
+        load_row<YT, kVec>(reinterpret_cast<const YT*>(a.dy) + off, g.t, g.tpr, D, on && a.dy, d);
+      }
+      if constexpr (kForm != kAfter) load_row<ZT, kVec>(reinterpret_cast<const ZT*>(a.dz) + off, g.t, g.tpr, D, on && a.dz, z);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) n[k] = col_of<kVec>(g.t, g.tpr, k) < D ? (n[k] - st.x) * st.y : 0.f;
+      float dn[8];
+      if constexpr (kForm == kBefore) {
+        float s2[8];
+        param8<kVec>(par[kPreScale], g.t, g.tpr, D, 0, a.pre_scale_bias, a.pre_scale_bias, s2);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          acc[kPre][k] = fmaf(z[k], n[k], acc[kPre][k]);
+          acc[kPre + 1][k] += z[k];
+          dn[k] = z[k] * s2[k];
+        }
+      } else {
+        float s[8], gt[8], rs[8], p[8];
+        param8<kVec>(par[kPostScale], g.t, g.tpr, D, 0, a.scale_bias, a.scale_bias, s);
+        param8<kVec>(par[kPostShift], g.t, g.tpr, D, 0, 0.f, 0.f, p);
+        param8<kVec>(par[kGate], g.t, g.tpr, D, 0, 0.f, 1.f, gt);
+        param8<kVec>(par[kResScale], g.t, g.tpr, D, 0, 0.f, a.res_scale, rs);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] = fmaf(n[k], s[k], p[k]);
+        if constexpr (kForm == kBetween) {
+          float s2[8], m[8], sum[2] = {0.f, 0.f};
+          param8<kVec>(par[kPreScale], g.t, g.tpr, D, 0, a.pre_scale_bias, a.pre_scale_bias, s2);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            m[k] = (fmaf(gt[k], p[k], rs[k] * r[k]) - st.z) * st.w;
+            acc[kPre][k] = fmaf(z[k], m[k], acc[kPre][k]);
+            acc[kPre + 1][k] += z[k];
+            z[k] *= s2[k];  // dm
+            if (col_of<kVec>(g.t, g.tpr, k) >= D) z[k] = 0.f;
+            sum[0] += z[k];
+            sum[1] = fmaf(z[k], m[k], sum[1]);
+          }
+          group_sum<2>(g, sum);
+          const float c0 = a.rms ? 0.f : sum[0] * a.inv_d, c1 = sum[1] * a.inv_d;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) d[k] = fmaf(st.w, z[k] - c0 - m[k] * c1, d[k]);
+        }
+        float dr[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          acc[kPost + kGate][k] = fmaf(d[k], p[k], acc[kPost + kGate][k]);
+          acc[kPost + kResScale][k] = fmaf(d[k], r[k], acc[kPost + kResScale][k]);
+          dr[k] = rs[k] * d[k];
+          const float dp = gt[k] * d[k];
+          acc[kPost + kPostScale][k] = fmaf(dp, n[k], acc[kPost + kPostScale][k]);
+          acc[kPost + kPostShift][k] += dp;
+          dn[k] = dp * s[k];
+        }
+        if (a.dr) store_row<YT, kVec>(reinterpret_cast<YT*>(a.dr) + off, g.t, g.tpr, D, on, dr);
+      }
+      if (a.dx) {
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (col_of<kVec>(g.t, g.tpr, k) >= D) dn[k] = 0.f;
+          sum[0] += dn[k];
+          sum[1] = fmaf(dn[k], n[k], sum[1]);
+        }
+        group_sum<2>(g, sum);
+        const float c0 = a.rms ? 0.f : sum[0] * a.inv_d, c1 = sum[1] * a.inv_d;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dn[k] = st.y * (dn[k] - c0 - n[k] * c1);
+        store_row<XT, kVec>(reinterpret_cast<XT*>(a.dx) + off, g.t, g.tpr, D, on, dn);
+      }
+    }
+    // This block's column sums of batch element b: over its row groups in turn, then to the workspace.
+    float* ws = a.ws + ((int64_t)b * gridDim.x + blockIdx.x) * kS * D;
+    if (groups == 1) {
+#pragma unroll
+      for (int i = 0; i < kS; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int c = col_of<kVec>(g.t, g.tpr, k);
+          if (c < D) ws[(int64_t)i * D + c] = acc[i][k];
+        }
+    } else {
+      for (int q = 0; q < groups; ++q) {
+        __syncthreads();
+        if (g.id == q) {
+#pragma unroll
+          for (int i = 0; i < kS; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int c = col_of<kVec>(g.t, g.tpr, k);
+              if (c < D) comb[i * D + c] = q == 0 ? acc[i][k] : comb[i * D + c] + acc[i][k];
+            }
+        }
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < kS * D; e += blockDim.x) ws[e] = comb[e];
+    }
+  }
+}
+
+// Column sums over blocks (and batch elements, for a shared parameter), in double.
+struct SumArgs {
+  const float* ws;
+  float* out[kParams];
+  int per_batch[kParams];
+  int first;  // parameter of sum 0
+  int sums, blocks, B, D;
+};
+constexpr int kSumRows = 8;
+
+__global__ void __launch_bounds__(32 * kSumRows) block_norm_sum_kernel(const SumArgs a) {
+  const int i = blockIdx.z, c = blockIdx.x * 32 + threadIdx.x;
+  float* out = a.out[a.first + i];
+  if (!out) return;
+  const bool own = a.per_batch[a.first + i];
+  for (int b = blockIdx.y; b < (own ? a.B : 1); b += gridDim.y) {
+    const int64_t lo = own ? (int64_t)b * a.blocks : 0, hi = own ? lo + a.blocks : (int64_t)a.B * a.blocks;
+    double s = 0.0;
+    if (c < a.D)
+      for (int64_t e = lo + threadIdx.y; e < hi; e += kSumRows) s += (double)a.ws[(e * a.sums + i) * a.D + c];
+    __shared__ double part[kSumRows][32];
+    __syncthreads();
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < a.D) {
+      for (int y = 1; y < kSumRows; ++y) s += part[y][threadIdx.x];
+      out[(int64_t)b * a.D + c] = (float)s;
+    }
+  }
+}
+
+int pow2_at_least(int v) {
+  int p = 1;
+  while (p < v) p *= 2;
+  return p;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+bool any_per_batch(const int64_t* strides) {
+  for (int i = 0; i < kParams; ++i)
+    if (strides[i]) return true;
+  return false;
+}
+
+struct BwdShape {
+  int tpr, threads;
+  int64_t B, L, blocks;  // batch elements and rows as the kernel sees them, blocks per batch element
+};
+
+BwdShape bwd_shape(const int64_t* strides, int64_t B, int64_t L, int64_t D) {
+  BwdShape s;
+  s.tpr = pow2_at_least((int)ceil_div(D, 8));
+  s.threads = s.tpr > 256 ? 512 : 256;
+  const bool split = any_per_batch(strides);
+  s.B = split ? B : 1;
+  s.L = split ? L : B * L;
+  const int64_t resident = (int64_t)num_sms() * (512 / s.threads);
+  const int64_t most = ceil_div(s.L, s.threads / s.tpr);
+  s.blocks = resident / (s.B > 0 ? s.B : 1);
+  if (s.blocks > most) s.blocks = most;
+  if (s.blocks < 1) s.blocks = 1;
+  return s;
+}
+
+int sums_of(int form) { return form == kBefore ? 2 : form == kAfter ? 4 : 6; }
+
+template <typename XT, typename YT, int kForm>
+int launch_fwd(NormArgs& a, bool vec, cudaStream_t s) {
+  const bool wide = a.D > 512;
+  a.tpr = pow2_at_least((int)ceil_div(a.D, wide ? 32 : 16));
+  const int groups = kFwdThreads / a.tpr;
+  auto kern = vec ? (wide ? block_norm_kernel<XT, YT, kForm, true, 4> : block_norm_kernel<XT, YT, kForm, true, 2>)
+                  : (wide ? block_norm_kernel<XT, YT, kForm, false, 4> : block_norm_kernel<XT, YT, kForm, false, 2>);
+  int64_t gx = (int64_t)num_sms() * 16 / a.B;
+  const int64_t most = ceil_div(a.L, groups);
+  gx = gx > most ? most : gx;
+  kern<<<dim3((unsigned)(gx < 1 ? 1 : gx), (unsigned)(a.B < 65535 ? a.B : 65535)), kFwdThreads, 0, s>>>(a);
+  return check_launch("block_norm_kernel");
+}
+
+template <typename XT, typename YT, int kForm>
+int launch_bwd(const NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
+  auto kern = vec ? block_norm_bwd_kernel<XT, YT, kForm, true> : block_norm_bwd_kernel<XT, YT, kForm, false>;
+  kern<<<dim3((unsigned)sh.blocks, (unsigned)(sh.B < 65535 ? sh.B : 65535)), sh.threads, 0, s>>>(a);
+  return check_launch("block_norm_bwd_kernel");
+}
+
+int check_args(int form, int norm, const void* x, int x_dtype, const void* r, int y_dtype, const float* const* params,
+               const int64_t* strides, int64_t B, int64_t L, int64_t D) {
+  FA_REQUIRE(form >= kBefore && form <= kBetween, FA_ERR_INVALID, "form must be FA_NORM_BEFORE, _AFTER or _BETWEEN");
+  FA_REQUIRE(norm == FA_NORM_LAYER || norm == FA_NORM_RMS, FA_ERR_INVALID, "norm must be FA_NORM_LAYER or FA_NORM_RMS");
+  FA_REQUIRE((x_dtype == FA_F32 || x_dtype == FA_BF16) && (y_dtype == FA_F32 || y_dtype == FA_BF16), FA_ERR_INVALID,
+             "dtype must be FA_F32 or FA_BF16");
+  FA_REQUIRE(B >= 0 && L >= 0 && D >= 1 && B < ((int64_t)1 << 31), FA_ERR_INVALID, "invalid shape");
+  FA_REQUIRE(D <= kMaxDim, FA_ERR_UNSUPPORTED, "block norms support D <= 4096");
+  FA_REQUIRE(L == 0 || B <= (((int64_t)1 << 60) / kMaxDim) / L, FA_ERR_INVALID, "shape too large");
+  FA_REQUIRE(params && strides, FA_ERR_INVALID, "null parameter array");
+  FA_REQUIRE(B * L == 0 || (x && (form == kBefore || r)), FA_ERR_INVALID, "null tensor pointer");
+  for (int i = 0; i < kParams; ++i)
+    FA_REQUIRE(strides[i] == 0 || (strides[i] == D && params[i]), FA_ERR_INVALID,
+               "a parameter's batch stride must be 0 or D");
+  return FA_OK;
+}
+
+void fill(NormArgs& a, int norm, const void* x, const void* r, const float* const* params, const int64_t* strides,
+          float scale_bias, float pre_scale_bias, float res_scale, float eps, int64_t B, int64_t L, int64_t D) {
+  a.x = x; a.r = r;
+  const bool split = any_per_batch(strides);
+  for (int i = 0; i < kParams; ++i) {
+    a.par[i] = params[i];
+    a.par_stride[i] = strides[i];
+  }
+  a.scale_bias = scale_bias; a.pre_scale_bias = pre_scale_bias; a.res_scale = res_scale; a.eps = eps;
+  a.inv_d = 1.f / (float)D;
+  a.rms = norm == FA_NORM_RMS; a.D = (int)D;
+  a.B = split ? (int)B : 1;
+  a.L = split ? L : B * L;
+}
+
+bool params_aligned(const float* const* params) {
+  for (int i = 0; i < kParams; ++i)
+    if (!aligned16(params[i])) return false;
+  return true;
+}
+
+#define FA_NORM_DISPATCH(LAUNCH, ...)                                                                             \
+  if (x_dtype == FA_F32 && y_dtype == FA_F32) return LAUNCH(float, float, __VA_ARGS__);                             \
+  if (x_dtype == FA_F32) return LAUNCH(float, __nv_bfloat16, __VA_ARGS__);                                          \
+  if (y_dtype == FA_F32) return LAUNCH(__nv_bfloat16, float, __VA_ARGS__);                                          \
+  return LAUNCH(__nv_bfloat16, __nv_bfloat16, __VA_ARGS__)
+
+template <typename XT, typename YT>
+int fwd_form(int form, NormArgs& a, bool vec, cudaStream_t s) {
+  if (form == kBefore) return launch_fwd<XT, YT, kBefore>(a, vec, s);
+  if (form == kAfter) return launch_fwd<XT, YT, kAfter>(a, vec, s);
+  return launch_fwd<XT, YT, kBetween>(a, vec, s);
+}
+template <typename XT, typename YT>
+int bwd_form(int form, const NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
+  if (form == kBefore) return launch_bwd<XT, YT, kBefore>(a, sh, vec, s);
+  if (form == kAfter) return launch_bwd<XT, YT, kAfter>(a, sh, vec, s);
+  return launch_bwd<XT, YT, kBetween>(a, sh, vec, s);
+}
+#define FA_FWD(XT, YT, ...) fwd_form<XT, YT>(__VA_ARGS__)
+#define FA_BWD(XT, YT, ...) bwd_form<XT, YT>(__VA_ARGS__)
+
+int dispatch_fwd(int x_dtype, int y_dtype, int form, NormArgs& a, bool vec, cudaStream_t s) {
+  FA_NORM_DISPATCH(FA_FWD, form, a, vec, s);
+}
+int dispatch_bwd(int x_dtype, int y_dtype, int form, const NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
+  FA_NORM_DISPATCH(FA_BWD, form, a, sh, vec, s);
+}
+
+}  // namespace
+}  // namespace fa
+
+using namespace fa;
+
+extern "C" int fa_block_norm(int form, int norm, const void* x, int x_dtype, const void* residual, int y_dtype,
+                             const float* const params[6], const int64_t param_strides[6], float scale_bias,
+                             float pre_scale_bias, float residual_scale, float eps, void* y, void* z, float* stats,
+                             int64_t B, int64_t L, int64_t D, void* stream) {
+  const int rc = check_args(form, norm, x, x_dtype, residual, y_dtype, params, param_strides, B, L, D);
+  if (rc != FA_OK || B * L == 0) return rc;
+  FA_REQUIRE((form == kBefore || y) && (form == kAfter || z), FA_ERR_INVALID, "null output pointer");
+  FA_REQUIRE(aligned16(stats), FA_ERR_INVALID, "stats must be 16-byte aligned");
+  NormArgs a{};
+  fill(a, norm, x, residual, params, param_strides, scale_bias, pre_scale_bias, residual_scale, eps, B, L, D);
+  a.y = y; a.z = z; a.stats = reinterpret_cast<float4*>(stats);
+  const bool vec = D % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(y) && aligned16(z) &&
+                   params_aligned(params);
+  return dispatch_fwd(x_dtype, y_dtype, form, a, vec, (cudaStream_t)stream);
+}
+
+extern "C" int64_t fa_block_norm_workspace(int form, const int64_t param_strides[6], int64_t B, int64_t L, int64_t D) {
+  if (form < kBefore || form > kBetween || !param_strides || B < 0 || L < 0 || D < 1 || D > kMaxDim ||
+      B >= ((int64_t)1 << 31) || (L > 0 && B > (((int64_t)1 << 60) / kMaxDim) / L))
+    return set_error(FA_ERR_INVALID, "invalid block norm shape");
+  const BwdShape s = bwd_shape(param_strides, B, L, D);
+  return s.B * s.blocks * sums_of(form) * D * 4;
+}
+
+extern "C" int fa_block_norm_backward(int form, int norm, const void* x, int x_dtype, const void* residual,
+                                      int y_dtype, const float* const params[6], const int64_t param_strides[6],
+                                      float scale_bias, float pre_scale_bias, float residual_scale, float eps,
+                                      const void* dy, const void* dz, const float* stats, void* dx, void* dresidual,
+                                      float* const dparams[6], int64_t B, int64_t L, int64_t D, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  const int rc = check_args(form, norm, x, x_dtype, residual, y_dtype, params, param_strides, B, L, D);
+  if (rc != FA_OK) return rc;
+  FA_REQUIRE(dparams, FA_ERR_INVALID, "null gradient array");
+  FA_REQUIRE(B * L == 0 || (stats && aligned16(stats)), FA_ERR_INVALID, "stats must be given, 16-byte aligned");
+  const int64_t need = fa_block_norm_workspace(form, param_strides, B, L, D);
+  FA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), FA_ERR_INVALID, "workspace too small");
+  cudaStream_t s = (cudaStream_t)stream;
+  const BwdShape sh = bwd_shape(param_strides, B, L, D);
+  if (B == 0) {
+    // No batch element: per-batch gradients are empty, shared ones are zero.
+    for (int i = 0; i < kParams; ++i)
+      if (dparams[i] && param_strides[i] == 0) FA_CUDA(cudaMemsetAsync(dparams[i], 0, (size_t)D * 4, s));
+    return FA_OK;
+  }
+  NormArgs a{};
+  fill(a, norm, x, residual, params, param_strides, scale_bias, pre_scale_bias, residual_scale, eps, B, L, D);
+  a.dy = dy; a.dz = dz; a.dx = dx; a.dr = dresidual;
+  a.stats = const_cast<float4*>(reinterpret_cast<const float4*>(stats));
+  a.ws = reinterpret_cast<float*>(workspace);
+  a.tpr = sh.tpr;
+  const bool vec = D % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(dy) && aligned16(dz) &&
+                   aligned16(dx) && aligned16(dresidual) && params_aligned(params);
+  const int rc2 = dispatch_bwd(x_dtype, y_dtype, form, a, sh, vec, s);
+  if (rc2 != FA_OK) return rc2;
+  SumArgs m{};
+  m.ws = a.ws;
+  m.first = form == kBefore ? kPreScale : kPostScale;
+  m.sums = sums_of(form); m.blocks = (int)sh.blocks; m.B = (int)sh.B; m.D = (int)D;
+  bool any = false, own = false;
+  for (int i = 0; i < kParams; ++i) {
+    m.out[i] = i >= m.first && i < m.first + m.sums ? dparams[i] : nullptr;
+    m.per_batch[i] = param_strides[i] != 0;
+    any = any || m.out[i];
+    own = own || (m.out[i] && m.per_batch[i]);
+  }
+  if (!any) return FA_OK;
+  const unsigned gy = own ? (unsigned)(sh.B < 65535 ? sh.B : 65535) : 1u;
+  block_norm_sum_kernel<<<dim3((unsigned)ceil_div(D, 32), gy, (unsigned)m.sums), dim3(32, kSumRows), 0, s>>>(m);
+  return check_launch("block_norm_sum_kernel");
+}

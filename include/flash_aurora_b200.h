@@ -313,6 +313,38 @@ int fa_window_attention_rel_bias_backward(int precision, int64_t Bwin, int64_t H
                                           void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * The norms before and after a residual block, fused with the block's gate and residual scale, and
+ * their gradients (no counterpart in the reference, whose AdaLN is the post-norm alone, forward only).
+ * N is the layer norm or the RMS norm over D, without affine, in fp32:
+ *   FA_NORM_BEFORE   z = N(x) (pre_scale_bias + pre_scale) + pre_shift
+ *   FA_NORM_AFTER    y = residual_scale * residual + gate * (N(x) (scale_bias + scale) + shift)
+ *   FA_NORM_BETWEEN  y as FA_NORM_AFTER, and z = N(y) (pre_scale_bias + pre_scale) + pre_shift
+ * x, residual, y, z: (B, L, D) contiguous, 1 <= D <= 4096. y_dtype is the dtype of residual and y, or of
+ * z for FA_NORM_BEFORE; z of FA_NORM_BETWEEN has x's dtype. params: {scale, shift, gate, residual
+ * scale, pre scale, pre shift}, fp32, each null, (D) with stride 0 or (B, D) with stride D; a null scale or
+ * shift counts as zeros, a null gate as ones, and the float residual_scale stands in for a null one.
+ * stats (nullable, (B, L, 4) fp32, 16-byte aligned): row statistics that the backward call reads.
+ *
+ * Backward: dy / dz are the gradients of y / z (null: zero), dx / dresidual and the entries of dparams
+ * (fp32, shaped as their parameters) are written where not null. Sums run in a fixed order.
+ * workspace: at least fa_block_norm_workspace(...) bytes (negative: a status), used until the call's
+ * work on the stream is done.
+ */
+enum { FA_NORM_BEFORE = 0, FA_NORM_AFTER = 1, FA_NORM_BETWEEN = 2 };
+enum { FA_NORM_LAYER = 0, FA_NORM_RMS = 1 };
+int fa_block_norm(int form, int norm, const void* x, int x_dtype, const void* residual, int y_dtype,
+                  const float* const params[6], const int64_t param_strides[6], float scale_bias,
+                  float pre_scale_bias, float residual_scale, float eps, void* y, void* z, float* stats,
+                  int64_t B, int64_t L, int64_t D, void* stream);
+int64_t fa_block_norm_workspace(int form, const int64_t param_strides[6], int64_t B, int64_t L, int64_t D);
+int fa_block_norm_backward(int form, int norm, const void* x, int x_dtype, const void* residual, int y_dtype,
+                           const float* const params[6], const int64_t param_strides[6], float scale_bias,
+                           float pre_scale_bias, float residual_scale, float eps, const void* dy,
+                           const void* dz, const float* stats, void* dx, void* dresidual,
+                           float* const dparams[6], int64_t B, int64_t L, int64_t D, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/*
  * Perceiver decoder LayerNorm (+ residual): out = LayerNorm(x) * weight + bias (+ residual) over
  * the last dimension D of `rows` contiguous rows, in fp32, rounded once to x's dtype. Replaces
  * layernorm_affine_forward / layernorm_affine_add_residual_forward (ops/triton_perceiver_ln.py:25-47,
