@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) rel_bias_bwd_kernel(const Params p) 
       for (int j = 0; j < p.N; ++j) {
         const float e = exp2f(logit_log2<kMask>(p, h, w, i, j, dot64(sQ[i], sK[j])) - st.x - st.y);
         const float ds = e * (dot64(sG[i], sV[j]) - delta);
-        slot[i * p.N + j] = first ? ds : slot[i * p.N + j] + ds;
+        if (p.slots) slot[i * p.N + j] = first ? ds : slot[i * p.N + j] + ds;
         for (int d = 0; d < 64; ++d) acc[d] = fmaf(ds, sK[j][d], acc[d]);
       }
       sDelta[i] = delta;
@@ -273,11 +273,10 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
   p.stats = reinterpret_cast<float2*>(stats);
   cudaStream_t s = (cudaStream_t)stream;
   const int grid = grid_of(p.num_tiles);
-  if (precision == FA_ATTN_BF16) {
-    if (mask_u8) return launch_fwd<__nv_bfloat16, kMaskU8>(p, grid, s);
-    if (group_ids) return launch_fwd<__nv_bfloat16, kGroups>(p, grid, s);
-    return launch_fwd<__nv_bfloat16, kNoMask>(p, grid, s);
-  }
+  p.status = attn::status_ptr();
+  FA_REQUIRE(p.status, FA_ERR_CUDA, "cannot resolve the attention status word");
+  if (precision == FA_ATTN_BF16)
+    return run_bf16_forward(p, mask_u8 ? kMaskU8 : group_ids ? kGroups : kNoMask, grid, s);
   if (mask_u8) return launch_fwd<float, kMaskU8>(p, grid, s);
   if (group_ids) return launch_fwd<float, kGroups>(p, grid, s);
   return launch_fwd<float, kNoMask>(p, grid, s);
@@ -311,11 +310,11 @@ extern "C" int fa_window_attention_rel_bias_backward(
     p.table = table; p.table_bf16 = table_dtype == FA_BF16; p.index = index;
     p.mask = mask_u8 ? mask_u8 : group_ids;
     p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats));
-    p.slots = reinterpret_cast<float*>(workspace);
+    p.slots = dtable ? reinterpret_cast<float*>(workspace) : nullptr;
+    p.status = attn::status_ptr();
+    FA_REQUIRE(p.status, FA_ERR_CUDA, "cannot resolve the attention status word");
     if (precision == FA_ATTN_BF16) {
-      rc = mask_u8 ? launch_bwd<__nv_bfloat16, kMaskU8>(p, grid, s)
-                   : group_ids ? launch_bwd<__nv_bfloat16, kGroups>(p, grid, s)
-                               : launch_bwd<__nv_bfloat16, kNoMask>(p, grid, s);
+      rc = run_bf16_backward(p, mask_u8 ? kMaskU8 : group_ids ? kGroups : kNoMask, grid, s);
     } else {
       rc = mask_u8 ? launch_bwd<float, kMaskU8>(p, grid, s)
                    : group_ids ? launch_bwd<float, kGroups>(p, grid, s)

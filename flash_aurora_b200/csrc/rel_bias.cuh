@@ -48,5 +48,9 @@ __device__ __forceinline__ float bias_log2(const Params& p, int h, int i, int j)
   return isinf(x) && !isinf(b) ? copysignf(3.4028234e38f, b) : x;
 }
 
+// The bf16 kernels (rel_bias_tc.cu); mask_kind: attn::kNoMask, kGroups or kMaskU8.
+int run_bf16_forward(const Params& p, int mask_kind, int grid, cudaStream_t s);
+int run_bf16_backward(const Params& p, int mask_kind, int grid, cudaStream_t s);
+
 }  // namespace relb
 }  // namespace fa
