@@ -24,6 +24,42 @@ using attn::kMaskU8;
 using attn::kMaxN;
 using attn::kNoMask;
 
+// The bias of (query i, key j) in the log2 domain; -inf for keys past N, 0 for query rows past N.
+// A finite entry stays finite (the clamp), so that a row of the lowest values is still a row.
+__device__ __forceinline__ float bias_log2(const void* table, int bf16, const int32_t* index, int H, int N, int h, int i,
+                                           int j) {
+  if (j >= N) return -INFINITY;
+  if (i >= N) return 0.f;
+  const int64_t e = (int64_t)__ldg(index + i * N + j) * H + h;
+  const float b = bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(table)[e])
+                       : __ldg(reinterpret_cast<const float*>(table) + e);
+  const float x = b * kLog2e;
+  return isinf(x) && !isinf(b) ? copysignf(3.4028234e38f, b) : x;
+}
+
+// Every head's bias in fragment order (see bias_rows), one float4 per thread. The gathers hit L1
+// here; in the attention kernels, whose shared memory leaves no L1, they cost a block 30 us a head.
+constexpr int kExpandThreads = 192;
+__global__ void __launch_bounds__(kExpandThreads)
+expand_bias_kernel(const void* table, int bf16, const int32_t* index, int H, int N, float4* out) {
+  const int e = blockIdx.x * kExpandThreads + threadIdx.x;
+  const int lane = e & 31, j = (e >> 5) % 18, blk = (e >> 5) / 18;
+  const int i = 16 * blk + (lane >> 2), k = 8 * j + 2 * (lane & 3);
+  for (int h = blockIdx.y; h < H; h += gridDim.y) {
+    out[(int64_t)h * kBiasVecs + e] = make_float4(bias_log2(table, bf16, index, H, N, h, i, k),
+                                                  bias_log2(table, bf16, index, H, N, h, i, k + 1),
+                                                  bias_log2(table, bf16, index, H, N, h, i + 8, k),
+                                                  bias_log2(table, bf16, index, H, N, h, i + 8, k + 1));
+  }
+}
+static_assert(kBiasVecs % kExpandThreads == 0, "whole blocks");
+
+__device__ __forceinline__ float bias_at(const Params& p, int h, int i, int j) {
+  const int lane = ((i & 7) << 2) | ((j & 7) >> 1);
+  const float* f = reinterpret_cast<const float*>(bias_rows(p, h, i & ~15, lane) + (j >> 3) * 32);
+  return __ldg(f + ((i & 8) >> 2) + (j & 1));
+}
+
 constexpr int kThreads = 160;  // one thread per query row, then one per key row
 
 template <typename T>
@@ -41,7 +77,7 @@ __device__ __forceinline__ float dot64(const float* a, const float* b) {
 
 template <int kMask>
 __device__ __forceinline__ float logit_log2(const Params& p, int h, int w, int i, int j, float s) {
-  float x = fmaf(s, p.scale_log2, bias_log2(p, h, i, j));
+  float x = fmaf(s, p.scale_log2, bias_at(p, h, i, j));
   const int64_t mw = w % p.nW;
   if (kMask == kGroups && __ldg(p.mask + mw * p.N + i) != __ldg(p.mask + mw * p.N + j)) x += kMaskedLog2;
   if (kMask == kMaskU8 && __ldg(p.mask + (mw * p.N + i) * p.N + j)) x += kMaskedLog2;
@@ -202,8 +238,7 @@ int grid_of(int64_t tiles) { return (int)(tiles < num_sms() ? tiles : num_sms())
 
 // Checks shared by both directions; strides are {window, head, token} triples.
 int check_args(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, const void* const* ptrs, int n_ptrs,
-               const int64_t* strides, const void* table, int table_dtype, const int32_t* index, bool u8, bool ids,
-               int64_t nW) {
+               const int64_t* strides, const float* bias, bool u8, bool ids, int64_t nW) {
   FA_REQUIRE(precision == FA_ATTN_BF16 || precision == FA_ATTN_FP32_3XTF32, FA_ERR_INVALID,
              "precision must be FA_ATTN_BF16 or FA_ATTN_FP32_3XTF32");
   FA_REQUIRE(strides, FA_ERR_INVALID, "null stride pointer");
@@ -215,9 +250,8 @@ int check_args(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, co
   FA_REQUIRE(nW < ((int64_t)1 << 31), FA_ERR_INVALID, "too many mask windows");
   FA_REQUIRE(Bwin < ((int64_t)1 << 31) && H < ((int64_t)1 << 31) && Bwin * H < ((int64_t)1 << 31), FA_ERR_INVALID,
              "too many (window, head) tiles");
-  FA_REQUIRE(table_dtype == FA_F32 || table_dtype == FA_BF16, FA_ERR_INVALID, "table dtype must be FA_F32 or FA_BF16");
-  FA_REQUIRE(table && index, FA_ERR_INVALID, "null bias table or index");
   if (Bwin == 0) return FA_OK;
+  FA_REQUIRE(bias && aligned16(bias), FA_ERR_INVALID, "the bias buffer must be given, 16-byte aligned");
   const int64_t es = precision == FA_ATTN_FP32_3XTF32 ? 4 : 2;
   for (int i = 0; i < n_ptrs; ++i) {
     FA_REQUIRE(ptrs[i], FA_ERR_INVALID, "null tensor pointer");
@@ -240,38 +274,36 @@ void copy3(int64_t* dst, const int64_t* src) {
 using namespace fa;
 using namespace fa::relb;
 
-extern "C" int64_t fa_window_attention_rel_bias_workspace(int precision, int64_t Bwin, int64_t H, int64_t N,
-                                                          int backward) {
-  if (precision != FA_ATTN_BF16 && precision != FA_ATTN_FP32_3XTF32)
-    return set_error(FA_ERR_INVALID, "precision must be FA_ATTN_BF16 or FA_ATTN_FP32_3XTF32");
+extern "C" int64_t fa_window_attention_rel_bias_workspace(int64_t Bwin, int64_t H, int64_t N) {
   if (Bwin < 0 || H < 1 || N < 1 || N > kMaxN || Bwin >= ((int64_t)1 << 31) || H >= ((int64_t)1 << 31) ||
       Bwin * H >= ((int64_t)1 << 31))
     return set_error(FA_ERR_INVALID, "invalid attention shape");
-  return backward ? (grid_of(Bwin * H) + H) * N * N * 4 : 0;
+  return (grid_of(Bwin * H) + H) * N * N * 4;
 }
 
 extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh,
                                             const void* q, const void* k, const void* v, void* out,
                                             const int64_t strides[12], const void* table, int table_dtype,
                                             const int32_t* index, const uint8_t* mask_u8, const uint8_t* group_ids,
-                                            int64_t nW, float scale, float* stats, void* workspace,
-                                            int64_t workspace_bytes, void* stream) {
+                                            int64_t nW, float scale, float* bias, float* stats, void* stream) {
   const void* ptrs[4] = {q, k, v, out};
-  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 4, strides, table, table_dtype, index, mask_u8 != nullptr,
-                      group_ids != nullptr, nW);
+  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 4, strides, bias, mask_u8 != nullptr, group_ids != nullptr, nW);
+  FA_REQUIRE(rc != FA_OK || (table && index && (table_dtype == FA_F32 || table_dtype == FA_BF16)), FA_ERR_INVALID,
+             "null bias table or index, or table dtype not FA_F32 or FA_BF16");
   if (rc != FA_OK || Bwin == 0) return rc;
-  const int64_t need = fa_window_attention_rel_bias_workspace(precision, Bwin, H, N, 0);
-  FA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), FA_ERR_INVALID, "workspace too small");
   Params p{};
   p.Bwin = (int)Bwin; p.H = (int)H; p.N = (int)N; p.nW = (int)(nW > 0 ? nW : 1);
   p.num_tiles = (int)(Bwin * H);
   p.scale = scale; p.scale_log2 = scale * kLog2e;
   p.q = q; p.k = k; p.v = v; p.out = out;
   copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
-  p.table = table; p.table_bf16 = table_dtype == FA_BF16; p.index = index;
+  p.bias = reinterpret_cast<const float4*>(bias);
   p.mask = mask_u8 ? mask_u8 : group_ids;
   p.stats = reinterpret_cast<float2*>(stats);
   cudaStream_t s = (cudaStream_t)stream;
+  expand_bias_kernel<<<dim3(kBiasVecs / kExpandThreads, (unsigned)(H < 65535 ? H : 65535)), kExpandThreads, 0, s>>>(
+      table, table_dtype == FA_BF16, index, p.H, p.N, reinterpret_cast<float4*>(bias));
+  if ((rc = check_launch("expand_bias_kernel")) != FA_OK) return rc;
   const int grid = grid_of(p.num_tiles);
   p.status = attn::status_ptr();
   FA_REQUIRE(p.status, FA_ERR_CUDA, "cannot resolve the attention status word");
@@ -284,19 +316,20 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
 
 extern "C" int fa_window_attention_rel_bias_backward(
     int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, const void* q, const void* k, const void* v,
-    const void* dout, void* dq, void* dk, void* dv, const int64_t strides[21], const void* table, int table_dtype,
-    const int32_t* index, const uint8_t* mask_u8, const uint8_t* group_ids, int64_t nW, float scale,
-    const float* stats, const int32_t* order, const int32_t* offsets, int64_t num_buckets, void* dtable,
-    void* workspace, int64_t workspace_bytes, void* stream) {
+    const void* dout, void* dq, void* dk, void* dv, const int64_t strides[21], const uint8_t* mask_u8,
+    const uint8_t* group_ids, int64_t nW, float scale, const float* bias, const float* stats, const int32_t* order,
+    const int32_t* offsets, int64_t num_buckets, void* dtable, int dtable_dtype, void* workspace,
+    int64_t workspace_bytes, void* stream) {
   const void* ptrs[7] = {q, k, v, dout, dq, dk, dv};
-  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 7, strides, table, table_dtype, index, mask_u8 != nullptr,
-                      group_ids != nullptr, nW);
+  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 7, strides, bias, mask_u8 != nullptr, group_ids != nullptr, nW);
   if (rc != FA_OK) return rc;
   FA_REQUIRE(stats || Bwin == 0, FA_ERR_INVALID, "null row statistics");
+  FA_REQUIRE(!dtable || dtable_dtype == FA_F32 || dtable_dtype == FA_BF16, FA_ERR_INVALID,
+             "table dtype must be FA_F32 or FA_BF16");
   FA_REQUIRE(!dtable || (order && offsets && num_buckets >= 1 && num_buckets < ((int64_t)1 << 31) && H <= 65535),
              FA_ERR_INVALID, "a bias gradient needs the bucket lists (and at most 65535 heads)");
   cudaStream_t s = (cudaStream_t)stream;
-  const int64_t need = fa_window_attention_rel_bias_workspace(precision, Bwin, H, N, 1);
+  const int64_t need = fa_window_attention_rel_bias_workspace(Bwin, H, N);
   FA_REQUIRE(Bwin == 0 || (workspace && workspace_bytes >= need), FA_ERR_INVALID, "workspace too small");
   const int grid = grid_of(Bwin * H);
   if (Bwin > 0) {
@@ -307,7 +340,7 @@ extern "C" int fa_window_attention_rel_bias_backward(
     p.q = q; p.k = k; p.v = v; p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
     copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
     copy3(p.sdq, strides + 12); copy3(p.sdk, strides + 15); copy3(p.sdv, strides + 18);
-    p.table = table; p.table_bf16 = table_dtype == FA_BF16; p.index = index;
+    p.bias = reinterpret_cast<const float4*>(bias);
     p.mask = mask_u8 ? mask_u8 : group_ids;
     p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats));
     p.slots = dtable ? reinterpret_cast<float*>(workspace) : nullptr;
@@ -324,7 +357,7 @@ extern "C" int fa_window_attention_rel_bias_backward(
   }
   if (!dtable) return FA_OK;
   bias_grad_kernel<<<dim3((unsigned)num_buckets, (unsigned)H), kReduceThreads, 0, s>>>(
-      reinterpret_cast<const float*>(workspace), order, offsets, dtable, table_dtype == FA_BF16, (int)H, (int)(N * N),
+      reinterpret_cast<const float*>(workspace), order, offsets, dtable, dtable_dtype == FA_BF16, (int)H, (int)(N * N),
       (int)Bwin, (int)(Bwin * H), grid);
   return check_launch("bias_grad_kernel");
 }

@@ -20,9 +20,7 @@ struct Params {
   void *out, *dq, *dk, *dv;
   int64_t sq[3], sk[3], sv[3], so[3];  // element strides of window, head, token; so: out or dout
   int64_t sdq[3], sdk[3], sdv[3];
-  const void* table;         // (num_buckets, H)
-  int table_bf16;
-  const int32_t* index;      // (N, N) bucket of each (query, key)
+  const float4* bias;        // the bias in fragment order, see expand_bias_kernel in rel_bias.cu
   const uint8_t* mask;       // (nW, N, N) bytes or (nW, N) region ids, by MaskKind
   float2* stats;             // (Bwin, H, N): row maximum and log2 of the row sum, log2 domain
   float* slots;              // backward: (gridDim.x + H - 1) partial bias gradients (N, N)
@@ -36,16 +34,13 @@ __device__ __forceinline__ int tile_end(int num_tiles) {
   return (int)(((int64_t)(blockIdx.x + 1) * num_tiles) / gridDim.x);
 }
 
-// The bias of (query i, key j) in the log2 domain; -inf for keys past N, 0 for query rows past N.
-// A finite entry stays finite (the clamp), so that a row of the lowest values is still a row.
-__device__ __forceinline__ float bias_log2(const Params& p, int h, int i, int j) {
-  if (j >= p.N) return -INFINITY;
-  if (i >= p.N) return 0.f;
-  const int64_t e = (int64_t)__ldg(p.index + i * p.N + j) * p.H + h;
-  const float b = p.table_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.table)[e])
-                               : __ldg(reinterpret_cast<const float*>(p.table) + e);
-  const float x = b * kLog2e;
-  return isinf(x) && !isinf(b) ? copysignf(3.4028234e38f, b) : x;
+// The fragment order of a head's bias: the 144 x 144 pairs in 9 blocks of 16 rows, each as 18 blocks of 8
+// keys, each as one float4 per lane: rows t1 and t1 + 8 (x, y and z, w), keys 2 t0 and 2 t0 + 1, with
+// t0 = lane % 4 and t1 = lane / 4. It is the accumulator layout of both kinds of tensor-core kernel here,
+// so a warp reads its rows with coalesced 16-byte loads.
+constexpr int kBiasVecs = 9 * 18 * 32;  // float4 per head
+__device__ __forceinline__ const float4* bias_rows(const Params& p, int h, int row0, int lane) {
+  return p.bias + ((int64_t)h * 9 + (row0 >> 4)) * (18 * 32) + lane;
 }
 
 // The bf16 kernels (rel_bias_tc.cu); mask_kind: attn::kNoMask, kGroups or kMaskU8.

@@ -83,29 +83,22 @@ __device__ __forceinline__ void store_p(uint32_t sP, const Lane& l, int j, uint3
   }
 }
 
-// The bias of this thread's 72 (row, key) pairs: b[4j + {0,1}] row ra, keys 8j + 2 t0 + {0,1};
-// b[4j + {2,3}] row rb. Warp 3 keeps them in shared memory instead.
-__device__ __forceinline__ float4 bias4(const Params& p, int h, const Lane& l, int j) {
-  const int key = 8 * j + 2 * l.t0;
-  return make_float4(bias_log2(p, h, l.ra, key), bias_log2(p, h, l.ra, key + 1), bias_log2(p, h, l.rb, key),
-                     bias_log2(p, h, l.rb, key + 1));
-}
-
+// The bias of this thread's 72 (row, key) pairs, one float4 per 8-key block (see bias_rows). Warp 3
+// keeps them in shared memory.
 template <bool kRem>
 struct Bias {
   float4 b[kRem ? 1 : 18];
   uint32_t smem;
-  __device__ __forceinline__ void fetch(const Params& p, int h, const Lane& l) {
-    if constexpr (kRem) {
-#pragma unroll 3
-      for (int j = 0; j < 18; ++j) {
-        const float4 v = bias4(p, h, l, j);
+  __device__ __forceinline__ void fetch(const Params& p, int h, const Lane& l, int lane) {
+    const float4* src = bias_rows(p, h, l.ra - l.t1, lane);
+#pragma unroll
+    for (int j = 0; j < 18; ++j) {
+      const float4 v = __ldg(src + j * 32);
+      if constexpr (kRem)
         st_shared_v4(smem + j * 512, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z),
                      __float_as_uint(v.w));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 18; ++j) b[j] = bias4(p, h, l, j);
+      else
+        b[j] = v;
     }
   }
   __device__ __forceinline__ float4 get(int j) const {
@@ -209,8 +202,8 @@ __device__ __forceinline__ void stage_rows(uint32_t stg, const Lane& l, const ui
 
 // ------------------------------------------------------------------------------------------
 // Forward.
-//   warps 0, 2  TMA producers: Q and K (warp 0), V and the region ids (warp 2), 3-slot rings; the
-//               output of a tile is staged in its V slot and stored by warp 2 before the slot's reuse;
+//   warps 0, 2  TMA producers: Q, K and the region ids (warp 0), V (warp 2), 3-slot rings; the output
+//               of a tile is staged in its V slot and stored by warp 2 before the slot's reuse;
 //   warp 1      TMEM owner and UMMA issuer:  S = Q K^T (M=128 and M=64), O = P V (M=128 and M=64);
 //   warps 3-11  x = S scale + bias (+ mask), softmax in the log2 domain, P to shared memory in bf16,
 //               then the previous tile's output rows.
@@ -223,9 +216,13 @@ constexpr int kStageBytes = 3 * kTileBytes;
 constexpr int kOffP = kStages * kStageBytes;
 constexpr int kOffRem = kOffP + kPBytes;
 constexpr int kOffIds = kOffRem + kRemBytes;
-constexpr int kOffBars = kOffIds + kStages * kIdBytes;
+// Region ids have a ring of their own: slot i % kIdSlots is rewritten for tile i + kIdSlots once the S
+// product of tile i + kIdSlots - 3 is done, which follows every softmax warp's load of S of tile
+// i + kIdSlots - 4 >= i + 1, so its work on tile i.
+constexpr int kIdSlots = 5;
+constexpr int kOffBars = kOffIds + kIdSlots * kIdBytes;
 enum { kFullQK = 0, kEmptyQK = 3, kFullV = 6, kStaged = 9, kSFull = 12, kSFree, kPFull, kPEmpty, kOFull = 16,
-       kOFree = 18, kDone = 20, kNumBars };
+       kOFree = 18, kDone = 20, kIds = 21, kNumBars = kIds + kIdSlots };
 constexpr int kSmem = kOffBars + kNumBars * 8 + 16 + 1024;
 static_assert(kSmem <= 227 * 1024, "shared memory budget");
 constexpr uint32_t kColS = 0, kColS2 = 160, kColO0 = 320, kColO1 = 384, kColO2 = 448;
@@ -274,16 +271,16 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin;
     if (h != cur_h) {
       cur_h = h;
-      bias.fetch(p, h, l);
+      bias.fetch(p, h, l, lane);
     }
     TileMask<kMask> mask;
     if constexpr (kMask == kGroups) {
-      if (!warp_wait(c.bar(kFullV + i % kStages), (uint32_t)((i / kStages) & 1), c.abort, p.status, 102)) {
+      if (!warp_wait(c.bar(kIds + i % kIdSlots), (uint32_t)((i / kIdSlots) & 1), c.abort, p.status, 102)) {
         ok = false;
         break;
       }
     }
-    mask.begin(p, l, w, c.smem + kOffIds + (i % kStages) * kIdBytes);
+    mask.begin(p, l, w, c.smem + kOffIds + (i % kIdSlots) * kIdBytes);
     if (!warp_wait(c.bar(kSFull), (uint32_t)(i & 1), c.abort, p.status, 103)) { ok = false; break; }
     tc_fence_after();
     uint32_t v[72];
@@ -300,19 +297,34 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bar(kSFree));
-    float mxa = -INFINITY, mxb = -INFINITY;
+    // The mask has a loop of its own behind one branch: inside this loop its 18 branches keep the
+    // compiler from interleaving the blocks, which doubled the kernel's time even where none is taken.
 #pragma unroll
     for (int j = 0; j < 18; ++j) {
       const float4 b = bias.get(j);
-      float2 xa = __ffma2_rn(f2(v[4 * j], v[4 * j + 1]), c2, make_float2(b.x, b.y));
-      float2 xb = __ffma2_rn(f2(v[4 * j + 2], v[4 * j + 3]), c2, make_float2(b.z, b.w));
-      if (kMask != kNoMask && mask.on) mask.apply(p, l, j, xa, xb);
+      const float2 xa = __ffma2_rn(f2(v[4 * j], v[4 * j + 1]), c2, make_float2(b.x, b.y));
+      const float2 xb = __ffma2_rn(f2(v[4 * j + 2], v[4 * j + 3]), c2, make_float2(b.z, b.w));
       v[4 * j] = __float_as_uint(xa.x);
       v[4 * j + 1] = __float_as_uint(xa.y);
       v[4 * j + 2] = __float_as_uint(xb.x);
       v[4 * j + 3] = __float_as_uint(xb.y);
-      mxa = fmax3(mxa, xa.x, xa.y);
-      mxb = fmax3(mxb, xb.x, xb.y);
+    }
+    if (kMask != kNoMask && mask.on) {
+#pragma unroll
+      for (int j = 0; j < 18; ++j) {
+        float2 xa = f2(v[4 * j], v[4 * j + 1]), xb = f2(v[4 * j + 2], v[4 * j + 3]);
+        mask.apply(p, l, j, xa, xb);
+        v[4 * j] = __float_as_uint(xa.x);
+        v[4 * j + 1] = __float_as_uint(xa.y);
+        v[4 * j + 2] = __float_as_uint(xb.x);
+        v[4 * j + 3] = __float_as_uint(xb.y);
+      }
+    }
+    float mxa = -INFINITY, mxb = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 18; ++j) {
+      mxa = fmax3(mxa, __uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]));
+      mxb = fmax3(mxb, __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
     }
     mxa = fmaxf(mxa, __shfl_xor_sync(0xffffffffu, mxa, 1));
     mxa = fmaxf(mxa, __shfl_xor_sync(0xffffffffu, mxa, 2));
@@ -390,6 +402,7 @@ rel_bias_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
       mbar_init(c.bar(kOFree + b), 9);
     }
     mbar_init(c.bar(kDone), 1);
+    for (int b = 0; b < kIdSlots; ++b) mbar_init(c.bar(kIds + b), 1);
     fence_mbarrier_init();
   }
   if (warp == 1) {
@@ -413,17 +426,36 @@ rel_bias_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
       if (lane == 0) {
         tma_prefetch_desc(&tmq);
         tma_prefetch_desc(&tmk);
-        int last_par[kStages] = {-1, -1, -1};
-        for (int i = 0; i < n; ++i) {
-          const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i % kStages;
-          const uint32_t ph = (uint32_t)((i / kStages) & 1);
-          if (!mbar_wait(c.bar(kEmptyQK + s), ph ^ 1u, c.abort, p.status, 105, kTimeoutNs)) break;
+      }
+      int last_par[kStages] = {-1, -1, -1};
+      uint32_t id[5], next_id[5];
+      if constexpr (kMask == kGroups) {
+        if (n > 0) load_ids(p, c.t_begin % p.Bwin, lane, next_id);
+      }
+      for (int i = 0; i < n; ++i) {
+        const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i % kStages;
+        const uint32_t ph = (uint32_t)((i / kStages) & 1);
+        if constexpr (kMask == kGroups) {
+#pragma unroll
+          for (int m = 0; m < 5; ++m) id[m] = next_id[m];
+          if (i + 1 < n) load_ids(p, (t + 1) % p.Bwin, lane, next_id);  // one tile ahead
+        }
+        int ok = 1;
+        if (lane == 0) ok = mbar_wait(c.bar(kEmptyQK + s), ph ^ 1u, c.abort, p.status, 105, kTimeoutNs);
+        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        if (lane == 0) {
           const uint32_t dst = c.sbase + s * kStageBytes;
           mbar_arrive_expect_tx(c.bar(kFullQK + s), kQKBytes);
           tma_load_4d(dst, &tmq, c.bar(kFullQK + s), 0, 0, h, w);
           tma_load_4d(dst + kTileBytes, &tmk, c.bar(kFullQK + s), 0, 0, h, w);
           last_par[s] = (int)ph;
         }
+        if constexpr (kMask == kGroups) {
+          store_ids(smem + kOffIds + (i % kIdSlots) * kIdBytes, lane, id);
+          if (lane == 0) mbar_arrive(c.bar(kIds + i % kIdSlots));
+        }
+      }
+      if (lane == 0) {
         // Never leave with copies in flight (bounded, also after an abort).
         int no_abort = 0;
         for (int s = 0; s < kStages; ++s)
@@ -439,8 +471,6 @@ rel_bias_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
       };
       for (int i = 0; i < n; ++i) {
         const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i % kStages;
-        uint32_t id[5];
-        if constexpr (kMask == kGroups) load_ids(p, w, lane, id);
         int ok = 1;
         if (lane == 0 && i >= kStages) {
           // The slot still holds the output of tile i - 3: store it and wait until it has been read.
@@ -451,7 +481,6 @@ rel_bias_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
           }
         }
         if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        if constexpr (kMask == kGroups) store_ids(smem + kOffIds + s * kIdBytes, lane, id);
         if (lane == 0) {
           mbar_arrive_expect_tx(c.bar(kFullV + s), kTileBytes);
           tma_load_4d(c.sbase + s * kStageBytes + kQKBytes, &tmv, c.bar(kFullV + s), 0, 0, h, w);
@@ -665,6 +694,52 @@ __device__ __forceinline__ void stage_rem(uint32_t taddr, uint32_t stg, int quar
 }
 
 template <bool kRem, int kMask>
+__device__ __forceinline__ void pass1(const Params& p, const Lane& l, const TileMask<kMask>& mask, const Bias<kRem>& bias,
+                                      uint32_t tS, uint32_t tP, uint32_t sP, float2 sta, float2 stb, float2& da2,
+                                      float2& db2) {
+  // Pass 1, 16 keys (two 8-key blocks) at a time, the next loads in flight.
+  const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+  const float2 ma2 = make_float2(-sta.x, -sta.x), mb2 = make_float2(-stb.x, -stb.x);
+  const float2 na2 = make_float2(-sta.y, -sta.y), nb2 = make_float2(-stb.y, -stb.y);
+  uint32_t sv[8], gv[8];
+  tmem_ld_16x256b_r8(tS, sv);
+  tmem_ld_16x256b_r8(tP, gv);
+#pragma unroll
+  for (int q = 0; q < 9; ++q) {
+    tmem_wait_ld();
+    uint32_t cs[8], cg[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      cs[e] = sv[e];
+      cg[e] = gv[e];
+    }
+    if (q < 8) {
+      tmem_ld_16x256b_r8(tS + 16 * (q + 1), sv);
+      tmem_ld_16x256b_r8(tP + 16 * (q + 1), gv);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const int j = 2 * q + (e >> 2);
+      const float4 b = bias.get(j);
+      float2 xa = __ffma2_rn(f2(cs[e], cs[e + 1]), c2, make_float2(b.x, b.y));
+      float2 xb = __ffma2_rn(f2(cs[e + 2], cs[e + 3]), c2, make_float2(b.z, b.w));
+      if (kMask != kNoMask) mask.apply(p, l, j, xa, xb);
+      xa = __fadd2_rn(__fadd2_rn(xa, ma2), na2);
+      xb = __fadd2_rn(__fadd2_rn(xb, mb2), nb2);
+      const float2 ea = make_float2(ex2(xa.x), ex2(xa.y)), eb = make_float2(ex2(xb.x), ex2(xb.y));
+      da2 = __ffma2_rn(ea, f2(cg[e], cg[e + 1]), da2);
+      db2 = __ffma2_rn(eb, f2(cg[e + 2], cg[e + 3]), db2);
+      store_p(sP, l, j, pack_bf16x2(ea.x, ea.y), pack_bf16x2(eb.x, eb.y));
+      cs[e] = __float_as_uint(ea.x);
+      cs[e + 1] = __float_as_uint(ea.y);
+      cs[e + 2] = __float_as_uint(eb.x);
+      cs[e + 3] = __float_as_uint(eb.y);
+    }
+    tmem_st_16x256b_r8(tS + 16 * q, cs);
+  }
+}
+
+template <bool kRem, int kMask>
 __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int warp, int lane) {
   const Lane l = make_lane(warp, lane);
   const uint32_t tS = c.tmem + l.addr + (kRem ? kColS2 : kColS);
@@ -675,7 +750,6 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
   Grad<kRem> grad;
   grad.smem = c.sbase + kOffRemAcc + lane * 16;
   int cur_h = -1;
-  const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
   for (int i = 0; i < c.n_local; ++i) {
     const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i & 1;
     const uint32_t par = (uint32_t)(i & 1);
@@ -684,14 +758,12 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
       if (cur_h >= 0) grad.flush(p, cur_h, l);
       cur_h = h;
       grad.clear();
-      bias.fetch(p, h, l);
+      bias.fetch(p, h, l, lane);
     }
     // Row statistics; +inf past N makes the rows' P zero.
     const float2* st = p.stats + ((int64_t)w * p.H + h) * p.N;
     const float2 pad = make_float2(INFINITY, 0.f);
     const float2 sta = l.ra < p.N ? __ldg(st + l.ra) : pad, stb = l.rb < p.N ? __ldg(st + l.rb) : pad;
-    const float2 ma2 = make_float2(-sta.x, -sta.x), mb2 = make_float2(-stb.x, -stb.x);
-    const float2 na2 = make_float2(-sta.y, -sta.y), nb2 = make_float2(-stb.y, -stb.y);
     TileMask<kMask> mask;
     if (!warp_wait(c.bar(kSFull), par, c.abort, p.status, 121)) return;
     if constexpr (kMask == kGroups) {  // the ids came with the tile's loads, long complete
@@ -699,44 +771,12 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     }
     mask.begin(p, l, w, c.smem + kOffIds + s * kIdBytes);
     tc_fence_after();
-    // Pass 1, 16 keys (two 8-key blocks) at a time, the next loads in flight.
     float2 da2 = make_float2(0.f, 0.f), db2 = make_float2(0.f, 0.f);
-    uint32_t sv[8], gv[8];
-    tmem_ld_16x256b_r8(tS, sv);
-    tmem_ld_16x256b_r8(tP, gv);
-#pragma unroll
-    for (int q = 0; q < 9; ++q) {
-      tmem_wait_ld();
-      uint32_t cs[8], cg[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        cs[e] = sv[e];
-        cg[e] = gv[e];
-      }
-      if (q < 8) {
-        tmem_ld_16x256b_r8(tS + 16 * (q + 1), sv);
-        tmem_ld_16x256b_r8(tP + 16 * (q + 1), gv);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const int j = 2 * q + (e >> 2);
-        const float4 b = bias.get(j);
-        float2 xa = __ffma2_rn(f2(cs[e], cs[e + 1]), c2, make_float2(b.x, b.y));
-        float2 xb = __ffma2_rn(f2(cs[e + 2], cs[e + 3]), c2, make_float2(b.z, b.w));
-        if (kMask != kNoMask && mask.on) mask.apply(p, l, j, xa, xb);
-        xa = __fadd2_rn(__fadd2_rn(xa, ma2), na2);
-        xb = __fadd2_rn(__fadd2_rn(xb, mb2), nb2);
-        const float2 ea = make_float2(ex2(xa.x), ex2(xa.y)), eb = make_float2(ex2(xb.x), ex2(xb.y));
-        da2 = __ffma2_rn(ea, f2(cg[e], cg[e + 1]), da2);
-        db2 = __ffma2_rn(eb, f2(cg[e + 2], cg[e + 3]), db2);
-        store_p(sP, l, j, pack_bf16x2(ea.x, ea.y), pack_bf16x2(eb.x, eb.y));
-        cs[e] = __float_as_uint(ea.x);
-        cs[e + 1] = __float_as_uint(ea.y);
-        cs[e + 2] = __float_as_uint(eb.x);
-        cs[e + 3] = __float_as_uint(eb.y);
-      }
-      tmem_st_16x256b_r8(tS + 16 * q, cs);
-    }
+    // One branch for the tile, not one per block: see the forward kernel.
+    if (kMask != kNoMask && mask.on)
+      pass1<kRem, kMask>(p, l, mask, bias, tS, tP, sP, sta, stb, da2, db2);
+    else
+      pass1<kRem, kNoMask>(p, l, TileMask<kNoMask>(), bias, tS, tP, sP, sta, stb, da2, db2);
     tmem_wait_st();
     fence_proxy_async_shared();
     tc_fence_before();
@@ -748,6 +788,7 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     db += __shfl_xor_sync(0xffffffffu, db, 1);
     db += __shfl_xor_sync(0xffffffffu, db, 2);
     const float2 ea2 = make_float2(-da, -da), eb2 = make_float2(-db, -db);
+    uint32_t sv[8], gv[8];
     tmem_ld_16x256b_r8(tS, sv);
     tmem_ld_16x256b_r8(tP, gv);
     if (!warp_wait(c.bar(kDvFull), par, c.abort, p.status, 123)) {

@@ -127,13 +127,6 @@ def _precision(dtype: torch.dtype) -> int:
     return _lib.FA_ATTN_BF16 if dtype == torch.bfloat16 else _lib.FA_ATTN_FP32_3XTF32
 
 
-def _workspace(prec: int, Bwin: int, H: int, N: int, backward: int, device) -> Optional[torch.Tensor]:
-    n = _lib.load().fa_window_attention_rel_bias_workspace(prec, Bwin, H, N, backward)
-    if n < 0:
-        _lib.check(int(n), "window_attn_rel_bias")
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
-
-
 def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
@@ -156,37 +149,39 @@ class _Call:
                 self.nW, self.scale)
 
 
-def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool) -> Optional[torch.Tensor]:
-    """Launch the forward kernel into ``out``; returns the row statistics when asked for."""
+def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool):
+    """Launch the forward kernels into ``out``; returns the expanded bias, and the row statistics when asked for."""
     Bwin, H, N, Dh = q.shape
     dev = q.device
     with torch.cuda.device(dev):
         stats = torch.empty(Bwin, H, N, 2, device=dev, dtype=torch.float32) if want_stats else None
-        prec = _precision(q.dtype)
-        ws = _workspace(prec, Bwin, H, N, 0, dev)
+        bias = torch.empty(H, _lib.FA_REL_BIAS_FLOATS, device=dev, dtype=torch.float32)
         rc = _lib.load().fa_window_attention_rel_bias(
-            prec, Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(q, k, v, out),
-            table.data_ptr(), _lib.dtype_code(table.dtype), call.buckets.index.data_ptr(), *call.masks(mask),
-            _ptr(stats), _ptr(ws), ws.numel() if ws is not None else 0, _lib.stream_ptr(dev))
+            _precision(q.dtype), Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+            _strides(q, k, v, out), table.data_ptr(), _lib.dtype_code(table.dtype), call.buckets.index.data_ptr(),
+            *call.masks(mask), bias.data_ptr(), _ptr(stats), _lib.stream_ptr(dev))
         _lib.check(rc, "window_attn_rel_bias")
-    return stats
+    return bias, stats
 
 
-def _backward(q, k, v, dout, dq, dk, dv, table, mask, call: _Call, stats, want_table: bool) -> Optional[torch.Tensor]:
-    """Launch the backward kernels into ``dq``, ``dk``, ``dv``; returns the table's gradient when asked for."""
+def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, bias, stats, table_dtype) -> Optional[torch.Tensor]:
+    """Launch the backward kernels into ``dq``, ``dk``, ``dv``; returns the table's gradient, in ``table_dtype``
+    (None: not asked for)."""
     Bwin, H, N, Dh = q.shape
     dev = q.device
     b = call.buckets
     with torch.cuda.device(dev):
-        dtable = torch.empty_like(table, memory_format=torch.contiguous_format) if want_table else None
-        prec = _precision(q.dtype)
-        ws = _workspace(prec, Bwin, H, N, 1, dev)
-        rc = _lib.load().fa_window_attention_rel_bias_backward(
-            prec, Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr(), _strides(q, k, v, dout, dq, dk, dv), table.data_ptr(),
-            _lib.dtype_code(table.dtype), b.index.data_ptr(), *call.masks(mask), stats.data_ptr(), b.order.data_ptr(),
-            b.offsets.data_ptr(), b.num_buckets, _ptr(dtable), _ptr(ws), ws.numel() if ws is not None else 0,
-            _lib.stream_ptr(dev))
+        lib = _lib.load()
+        dtable = None if table_dtype is None else torch.empty(b.num_buckets, H, device=dev, dtype=table_dtype)
+        n = lib.fa_window_attention_rel_bias_workspace(Bwin, H, N)
+        if n < 0:
+            _lib.check(int(n), "window_attn_rel_bias backward")
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        rc = lib.fa_window_attention_rel_bias_backward(
+            _precision(q.dtype), Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), _strides(q, k, v, dout, dq, dk, dv), *call.masks(mask), bias.data_ptr(),
+            stats.data_ptr(), b.order.data_ptr(), b.offsets.data_ptr(), b.num_buckets, _ptr(dtable),
+            _lib.dtype_code(table_dtype or torch.float32), ws.data_ptr(), n, _lib.stream_ptr(dev))
         _lib.check(rc, "window_attn_rel_bias backward")
     return dtable
 
@@ -202,37 +197,37 @@ class _Attn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, mask, call):
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        stats = _forward(q, k, v, out, table, mask, call, True)
-        ctx.save_for_backward(q, k, v, table, mask, stats)
-        ctx.call = call
+        ctx.save_for_backward(q, k, v, mask, *_forward(q, k, v, out, table, mask, call, True))
+        ctx.call, ctx.table_dtype = call, table.dtype
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, mask, stats = ctx.saved_tensors
+        q, k, v, mask, bias, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         dq, dk, dv = (torch.empty(q.shape, device=q.device, dtype=q.dtype) for _ in range(3))
-        dtable = _backward(q, k, v, _strided(dout), dq, dk, dv, table, mask, ctx.call, stats, need[3])
+        dtable = _backward(q, k, v, _strided(dout), dq, dk, dv, mask, ctx.call, bias, stats,
+                           ctx.table_dtype if need[3] else None)
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None
 
 
 class _AttnPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, table, mask, call, H, bnc):
-        out, stats = _packed_forward(qkv, table, mask, call, H, bnc, True)
-        ctx.save_for_backward(qkv, table, mask, stats)
-        ctx.call, ctx.H, ctx.bnc = call, H, bnc
+        out, saved = _packed_forward(qkv, table, mask, call, H, bnc, True)
+        ctx.save_for_backward(qkv, mask, *saved)
+        ctx.call, ctx.table_dtype, ctx.H, ctx.bnc = call, table.dtype, H, bnc
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, table, mask, stats = ctx.saved_tensors
+        qkv, mask, bias, stats = ctx.saved_tensors
         dqkv = torch.empty_like(qkv)
         dout = _strided(_same_heads(dout.contiguous() if ctx.bnc else dout, ctx.bnc, ctx.H))
-        dtable = _backward(*_heads_of(qkv, ctx.H), dout, *_heads_of(dqkv, ctx.H), table, mask, ctx.call, stats,
-                           ctx.needs_input_grad[1])
+        dtable = _backward(*_heads_of(qkv, ctx.H), dout, *_heads_of(dqkv, ctx.H), mask, ctx.call, bias, stats,
+                           ctx.table_dtype if ctx.needs_input_grad[1] else None)
         return dqkv if ctx.needs_input_grad[0] else None, dtable, None, None, None, None
 
 

@@ -101,9 +101,9 @@ def test_abi_refusals_without_a_gpu():
     p = ctypes.c_void_p(1 << 20)
     st = (ctypes.c_int64 * 21)(*([64] * 21))
 
-    def fwd(prec=0, B=4, H=2, N=16, D=64, q=p, table=p, tdt=0, index=p, u8=None, ids=None, nW=0, strides=st):
+    def fwd(prec=0, B=4, H=2, N=16, D=64, q=p, table=p, tdt=0, index=p, u8=None, ids=None, nW=0, strides=st, bias=p):
         return lib.fa_window_attention_rel_bias(prec, B, H, N, D, q, p, p, p, strides, table, tdt, index, u8, ids, nW,
-                                                0.125, None, None, 0, None)
+                                                0.125, bias, None, None)
 
     assert fwd(prec=3) == _lib.FA_ERR_INVALID
     assert fwd(D=32) == _lib.FA_ERR_UNSUPPORTED and b"head_dim" in lib.fa_last_error()
@@ -118,16 +118,19 @@ def test_abi_refusals_without_a_gpu():
     assert fwd(B=1 << 30, H=4) == _lib.FA_ERR_INVALID and b"tiles" in lib.fa_last_error()
     bad = (ctypes.c_int64 * 21)(*([60] * 21))
     assert fwd(strides=bad) == _lib.FA_ERR_INVALID and b"16 bytes" in lib.fa_last_error()
+    assert fwd(bias=None) == _lib.FA_ERR_INVALID and b"bias buffer" in lib.fa_last_error()
     assert fwd(B=0, q=None) == _lib.FA_OK
 
-    def bwd(stats=p, order=p, nb=5, ws=p, nbytes=1 << 40):
-        return lib.fa_window_attention_rel_bias_backward(0, 4, 2, 16, 64, p, p, p, p, p, p, p, st, p, 0, p, None, None,
-                                                         0, 0.125, stats, order, p, nb, p, ws, nbytes, None)
+    def bwd(stats=p, order=p, nb=5, ws=p, nbytes=1 << 40, tdt=0, bias=p):
+        return lib.fa_window_attention_rel_bias_backward(0, 4, 2, 16, 64, p, p, p, p, p, p, p, st, None, None, 0, 0.125,
+                                                         bias, stats, order, p, nb, p, tdt, ws, nbytes, None)
 
+    assert bwd(bias=None) == _lib.FA_ERR_INVALID and b"bias buffer" in lib.fa_last_error()
+    assert bwd(tdt=2) == _lib.FA_ERR_INVALID and b"table dtype" in lib.fa_last_error()
     assert bwd(stats=None) == _lib.FA_ERR_INVALID and b"statistics" in lib.fa_last_error()
     assert bwd(order=None) == _lib.FA_ERR_INVALID and b"bucket lists" in lib.fa_last_error()
     assert bwd(nb=0) == _lib.FA_ERR_INVALID
     assert bwd(ws=None) == _lib.FA_ERR_INVALID and b"workspace" in lib.fa_last_error()
     assert bwd(nbytes=16) == _lib.FA_ERR_INVALID and b"workspace" in lib.fa_last_error()
-    assert lib.fa_window_attention_rel_bias_workspace(0, 4, 2, 145, 1) == _lib.FA_ERR_INVALID
-    assert lib.fa_window_attention_rel_bias_workspace(0, 4, 2, 16, 1) >= (4 * 2 + 1) * 16 * 16 * 4
+    assert lib.fa_window_attention_rel_bias_workspace(4, 2, 145) == _lib.FA_ERR_INVALID
+    assert lib.fa_window_attention_rel_bias_workspace(4, 2, 16) >= (4 * 2 + 1) * 16 * 16 * 4
