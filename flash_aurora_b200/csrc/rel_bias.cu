@@ -12,6 +12,8 @@
 // gives the same bits.
 #include <cuda_bf16.h>
 
+#include <cmath>
+
 #include "rel_bias.cuh"
 
 namespace fa {
@@ -238,13 +240,15 @@ int grid_of(int64_t tiles) { return (int)(tiles < num_sms() ? tiles : num_sms())
 
 // Checks shared by both directions; strides are {window, head, token} triples.
 int check_args(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, const void* const* ptrs, int n_ptrs,
-               const int64_t* strides, const float* bias, bool u8, bool ids, int64_t nW) {
+               const int64_t* strides, const float* bias, bool u8, bool ids, int64_t nW, float scale) {
   FA_REQUIRE(precision == FA_ATTN_BF16 || precision == FA_ATTN_FP32_3XTF32, FA_ERR_INVALID,
              "precision must be FA_ATTN_BF16 or FA_ATTN_FP32_3XTF32");
   FA_REQUIRE(strides, FA_ERR_INVALID, "null stride pointer");
   FA_REQUIRE(Bwin >= 0 && H >= 1 && N >= 1, FA_ERR_INVALID, "invalid attention shape");
   FA_REQUIRE(Dh == 64, FA_ERR_UNSUPPORTED, "window attention supports head_dim 64");
   FA_REQUIRE(N <= kMaxN, FA_ERR_UNSUPPORTED, "window attention supports N <= 144 tokens");
+  FA_REQUIRE(fabsf(scale) >= 1e-30f && fabsf(scale) <= 1e30f, FA_ERR_INVALID,
+             "scale must be finite and at least 1e-30 in magnitude");
   FA_REQUIRE(!(u8 && ids), FA_ERR_INVALID, "pass at most one of mask_u8 / group_ids");
   FA_REQUIRE(!(u8 || ids) || nW >= 1, FA_ERR_INVALID, "nW must be >= 1 with a mask");
   FA_REQUIRE(nW < ((int64_t)1 << 31), FA_ERR_INVALID, "too many mask windows");
@@ -261,6 +265,23 @@ int check_args(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, co
                  "strides must be positive multiples of 16 bytes");
   }
   return FA_OK;
+}
+
+// Two bf16 numbers whose product is -100 / scale to 16 bits or better: the first is the significand
+// in [1, 2) that leaves the quotient nearest to a bf16 number (exact for the default scale of 1 / 8).
+void split_mask_value(float scale, uint32_t* a_bits, uint32_t* b_bits) {
+  const double want = -100.0 / (double)scale;
+  double best = -1.0;
+  for (int m = 0; m < 128; ++m) {
+    const double a = 1.0 + m / 128.0;
+    const __nv_bfloat16 b = __float2bfloat16((float)(want / a));
+    const double off = fabs(a * (double)__bfloat162float(b) - want);
+    if (best < 0.0 || off < best) {
+      best = off;
+      *a_bits = __nv_bfloat16_raw(__float2bfloat16((float)a)).x;
+      *b_bits = __nv_bfloat16_raw(b).x;
+    }
+  }
 }
 
 void copy3(int64_t* dst, const int64_t* src) {
@@ -287,7 +308,8 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
                                             const int32_t* index, const uint8_t* mask_u8, const uint8_t* group_ids,
                                             int64_t nW, float scale, float* bias, float* stats, void* stream) {
   const void* ptrs[4] = {q, k, v, out};
-  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 4, strides, bias, mask_u8 != nullptr, group_ids != nullptr, nW);
+  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 4, strides, bias, mask_u8 != nullptr, group_ids != nullptr, nW,
+                      scale);
   FA_REQUIRE(rc != FA_OK || (table && index && (table_dtype == FA_F32 || table_dtype == FA_BF16)), FA_ERR_INVALID,
              "null bias table or index, or table dtype not FA_F32 or FA_BF16");
   if (rc != FA_OK || Bwin == 0) return rc;
@@ -299,6 +321,7 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
   copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
   p.bias = reinterpret_cast<const float4*>(bias);
   p.mask = mask_u8 ? mask_u8 : group_ids;
+  if (group_ids) split_mask_value(scale, &p.mask_a, &p.mask_b);
   p.stats = reinterpret_cast<float2*>(stats);
   cudaStream_t s = (cudaStream_t)stream;
   expand_bias_kernel<<<dim3(kBiasVecs / kExpandThreads, (unsigned)(H < 65535 ? H : 65535)), kExpandThreads, 0, s>>>(
@@ -321,7 +344,8 @@ extern "C" int fa_window_attention_rel_bias_backward(
     const int32_t* offsets, int64_t num_buckets, void* dtable, int dtable_dtype, void* workspace,
     int64_t workspace_bytes, void* stream) {
   const void* ptrs[7] = {q, k, v, dout, dq, dk, dv};
-  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 7, strides, bias, mask_u8 != nullptr, group_ids != nullptr, nW);
+  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 7, strides, bias, mask_u8 != nullptr, group_ids != nullptr, nW,
+                      scale);
   if (rc != FA_OK) return rc;
   FA_REQUIRE(stats || Bwin == 0, FA_ERR_INVALID, "null row statistics");
   FA_REQUIRE(!dtable || dtable_dtype == FA_F32 || dtable_dtype == FA_BF16, FA_ERR_INVALID,
@@ -342,6 +366,7 @@ extern "C" int fa_window_attention_rel_bias_backward(
     copy3(p.sdq, strides + 12); copy3(p.sdk, strides + 15); copy3(p.sdv, strides + 18);
     p.bias = reinterpret_cast<const float4*>(bias);
     p.mask = mask_u8 ? mask_u8 : group_ids;
+  if (group_ids) split_mask_value(scale, &p.mask_a, &p.mask_b);
     p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats));
     p.slots = dtable ? reinterpret_cast<float*>(workspace) : nullptr;
     p.status = attn::status_ptr();

@@ -22,6 +22,7 @@ struct Params {
   int64_t sdq[3], sdk[3], sdv[3];
   const float4* bias;        // the bias in fragment order, see expand_bias_kernel in rel_bias.cu
   const uint8_t* mask;       // (nW, N, N) bytes or (nW, N) region ids, by MaskKind
+  uint32_t mask_a, mask_b;   // bf16 bits: mask_a * mask_b = -100 / scale (region masks, bf16 kernels)
   float2* stats;             // (Bwin, H, N): row maximum and log2 of the row sum, log2 domain
   float* slots;              // backward: (gridDim.x + H - 1) partial bias gradients (N, N)
   int* status;

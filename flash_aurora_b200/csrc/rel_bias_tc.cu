@@ -2,13 +2,25 @@
 // accumulators in TMEM), forward and backward. The formulas are in rel_bias.cu.
 //
 // Both kernels are persistent, one CTA per SM over a contiguous range of (head, window) tiles in
-// head-major order, so that a head's bias is fetched from the table once per CTA and head and then
-// stays on chip in fp32: 72 registers of each softmax warp thread. A window has 144 query rows and an
-// M = 128 UMMA covers 128; rows 128..143 go through an M = 64 UMMA over rows 80..143 (the tile at an
-// 80-row offset), whose last 16 rows are kept. Warps 4..11 own 16 query rows each of 0..127, warp 3 owns
-// rows 128..143; a row's 144 keys sit in four threads of one warp (16x256b TMEM shape), so row
-// maxima and sums take two shuffles. Registers are moved from warps 0..3 to 4..11 (setmaxnreg); warp
-// 3, which is in the smaller group, keeps its 9 KB of bias in shared memory.
+// head-major order, so that a head's bias is fetched once per CTA and head and then stays on chip in
+// fp32, in registers of the softmax warps. A window has 144 query rows and an M = 128 UMMA covers 128;
+// rows 128..143 go through an M = 64 UMMA over rows 88..151 (the tile at an 88-row offset; what lies
+// past the tile only reaches accumulator rows that nobody reads), which puts rows 128..135 into the third
+// and rows 136..143 into the fourth TMEM quarter. Warps 4..11 own 16 query rows each of 0..127, warps 2
+// and 3 eight rows each of 128..143, so that no SM sub-partition has three full softmax warps. A row's
+// 144 keys sit in four threads of one warp (16x256b TMEM shape): row maxima and sums take two shuffles.
+// Registers are moved from warps 0..3 to 4..11 (setmaxnreg).
+//
+// Region-id masks go through the tensor cores: with the ids of a window ranked, one K = 16 step adds
+//   sum_r onehot(rank of query)[r] * (-c (1 - onehot(rank of key)[r])),  c = 100 / scale,
+// exactly 0 to the raw logit of a pair of one region and -c to the others; a window of R regions
+// takes ceil(R / 16) steps (none for R = 1), whatever its ids are. c is a product of two bf16 numbers.
+// The per-logit alternative (compare and add in the softmax warps) cost 110 us of 350 on half-masked
+// windows of 144 tokens. Byte masks are applied per logit.
+//
+// UMMAs are issued by one elected lane of a converged warp from precomputed descriptors: with a lane-0
+// branch and descriptors built in place an UMMA took 75 cycles to issue whatever its shape, against
+// 51 (128 x 64 x 16), 26 (64 x 16 x 16) and 75 (128 x 144 x 16) this way.
 //
 // P (and dS) are rounded to bf16 as tensor-core operands, the one rounding besides the outputs';
 // logits, softmax statistics, dS in the bias gradient, and all accumulators are fp32.
@@ -37,12 +49,11 @@ constexpr int kThreads = 384;
 constexpr uint32_t kRegsLaunch = 168;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kPChunk = kTileBytes;     // 64 keys x 144 rows of bf16, 128-byte swizzle
-constexpr int kRow32 = kMaxN * 32;      // 16 keys x 144 rows of bf16, 32-byte swizzle
+constexpr int kRow32 = kMaxN * 32;      // 16 columns x 144 rows of bf16, 32-byte swizzle
 constexpr int kPBytes = 2 * kPChunk + kRow32;
-constexpr int kIdBytes = 160;           // a tile's region ids and, at byte 144, whether they differ
-constexpr int kRemBytes = 18 * 32 * 16; // one float4 per lane and 8-key block: warp 3's bias
-constexpr uint32_t kRowOff80 = 80 * 128;
-constexpr uint32_t kRowOff80_32 = 80 * 32;
+constexpr int kMaskOpBytes = 2 * kRow32;  // A (queries) and B (keys) of one mask step
+constexpr int kRemRow = 88;             // first row of the M = 64 block
+constexpr uint32_t kRemOff = kRemRow * 128, kRemOff32 = kRemRow * 32;
 constexpr uint32_t kLaneHalf = 16u << 16;  // second lane half of an M = 64 accumulator
 
 constexpr uint32_t kIdescS = make_idesc(1, 128, kMaxN, false, false);
@@ -50,163 +61,196 @@ constexpr uint32_t kIdescS2 = make_idesc(1, 64, kMaxN, false, false);
 constexpr uint32_t kIdescO = make_idesc(1, 128, 64, false, true);
 constexpr uint32_t kIdescO2 = make_idesc(1, 64, 64, false, true);
 
-__device__ __forceinline__ uint32_t sw32_offset(int r, int e) {
-  return (uint32_t)(r * 32 + ((((e >> 3) ^ (r >> 2)) & 1) << 4) + (e & 7) * 2);
-}
+// A descriptor whose operand starts `bytes` further on (the start field counts 16-byte units).
+__device__ __forceinline__ uint64_t at(uint64_t desc, uint32_t bytes) { return desc + (uint64_t)(bytes >> 4); }
 
-// Row pair (ra, rb) and key quad position of one thread of a softmax warp.
-struct Lane {
-  int t0, t1, ra, rb;
-  uint32_t addr;  // TMEM lane offset of the warp's 16 rows
-};
-
-__device__ __forceinline__ Lane make_lane(int warp, int lane) {
-  Lane l;
-  l.t0 = lane & 3;
-  l.t1 = lane >> 2;
-  const int rbase = warp == 3 ? 128 : 32 * (warp & 3) + 16 * ((warp - 4) >> 2);
-  l.ra = rbase + l.t1;
-  l.rb = l.ra + 8;
-  l.addr = warp == 3 ? (96u << 16) : ((uint32_t)rbase << 16);  // rows 48..63 of an M = 64 block
-  return l;
-}
-
-// bf16 pairs of 8-key block j (0..17), rows ra and rb, into the P operand tile.
-__device__ __forceinline__ void store_p(uint32_t sP, const Lane& l, int j, uint32_t a, uint32_t b) {
-  if (j < 16) {
-    const uint32_t off = sP + (j >> 3) * kPChunk + (uint32_t)(4 * l.t0);
-    st_shared_u32(off + l.ra * 128 + (((j & 7) ^ (l.ra & 7)) << 4), a);
-    st_shared_u32(off + l.rb * 128 + (((j & 7) ^ (l.rb & 7)) << 4), b);
-  } else {
-    st_shared_u32(sP + 2 * kPChunk + sw32_offset(l.ra, (j & 1) * 8 + 2 * l.t0), a);
-    st_shared_u32(sP + 2 * kPChunk + sw32_offset(l.rb, (j & 1) * 8 + 2 * l.t0), b);
-  }
-}
-
-// The bias of this thread's 72 (row, key) pairs, one float4 per 8-key block (see bias_rows). Warp 3
-// keeps them in shared memory.
-template <bool kRem>
-struct Bias {
-  float4 b[kRem ? 1 : 18];
-  uint32_t smem;
-  __device__ __forceinline__ void fetch(const Params& p, int h, const Lane& l, int lane) {
-    const float4* src = bias_rows(p, h, l.ra - l.t1, lane);
-#pragma unroll
-    for (int j = 0; j < 18; ++j) {
-      const float4 v = __ldg(src + j * 32);
-      if constexpr (kRem)
-        st_shared_v4(smem + j * 512, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z),
-                     __float_as_uint(v.w));
-      else
-        b[j] = v;
-    }
-  }
-  __device__ __forceinline__ float4 get(int j) const {
-    if constexpr (kRem) {
-      uint32_t x, y, z, w;
-      ld_shared_v4(smem + j * 512, x, y, z, w);
-      return make_float4(__uint_as_float(x), __uint_as_float(y), __uint_as_float(z), __uint_as_float(w));
-    } else {
-      return b[j];
-    }
-  }
-};
-
-// Mask of one tile as the softmax warps apply it.
-template <int kMask>
-struct TileMask {
-  bool on;
-  uint32_t ta, tb;      // region ids of rows ra, rb
-  const uint8_t* ids;   // shared memory
-  const uint8_t *ma, *mb;  // byte-mask rows (global), null past N
-  __device__ __forceinline__ void begin(const Params& p, const Lane& l, int w, const uint8_t* tile_ids) {
-    if constexpr (kMask == kGroups) {
-      on = tile_ids[kMaxN] != 0;
-      ids = tile_ids;
-      ta = tile_ids[l.ra];
-      tb = tile_ids[l.rb];
-    } else if constexpr (kMask == kMaskU8) {
-      on = true;
-      const uint8_t* base = p.mask + (int64_t)(w % p.nW) * p.N * p.N;
-      ma = l.ra < p.N ? base + l.ra * p.N : nullptr;
-      mb = l.rb < p.N ? base + l.rb * p.N : nullptr;
-    } else {
-      on = false;
-    }
-  }
-  // Adds -100 (log2 domain) to the masked logits of 8-key block j.
-  __device__ __forceinline__ void apply(const Params& p, const Lane& l, int j, float2& xa, float2& xb) const {
-    const int key = 8 * j + 2 * l.t0;
-    if constexpr (kMask == kGroups) {
-      const uint32_t kk = *reinterpret_cast<const unsigned short*>(ids + key);
-      const uint32_t k0 = kk & 0xffu, k1 = kk >> 8;
-      xa.x += k0 != ta ? kMaskedLog2 : 0.f;
-      xa.y += k1 != ta ? kMaskedLog2 : 0.f;
-      xb.x += k0 != tb ? kMaskedLog2 : 0.f;
-      xb.y += k1 != tb ? kMaskedLog2 : 0.f;
-    } else if constexpr (kMask == kMaskU8) {
-      if (key < p.N) {
-        if (ma && __ldg(ma + key)) xa.x += kMaskedLog2;
-        if (mb && __ldg(mb + key)) xb.x += kMaskedLog2;
-      }
-      if (key + 1 < p.N) {
-        if (ma && __ldg(ma + key + 1)) xa.y += kMaskedLog2;
-        if (mb && __ldg(mb + key + 1)) xb.y += kMaskedLog2;
-      }
-    }
-  }
-};
-
-// Region ids of a window's tokens lane + 32 m, and the store of a tile's ids with their "differ" flag.
-__device__ __forceinline__ void load_ids(const Params& p, int w, int lane, uint32_t (&id)[5]) {
-  const uint8_t* g = p.mask + (int64_t)(w % p.nW) * p.N;
-  const uint32_t first = __ldg(g);
-#pragma unroll
-  for (int m = 0; m < 5; ++m) id[m] = lane + 32 * m < p.N ? (uint32_t)__ldg(g + lane + 32 * m) : first;
-}
-__device__ __forceinline__ void store_ids(uint8_t* dst, int lane, const uint32_t (&id)[5]) {
-  const uint32_t first = __shfl_sync(0xffffffffu, id[0], 0);
-  bool differ = false;
-#pragma unroll
-  for (int m = 0; m < 5; ++m) {
-    differ = differ || id[m] != first;
-    if (lane + 32 * m < kMaxN) dst[lane + 32 * m] = (uint8_t)id[m];
-  }
-  differ = __any_sync(0xffffffffu, differ);
-  if (lane == 0) dst[kMaxN] = differ ? 1 : 0;
-  __syncwarp();
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(e));
+  return e != 0;
 }
 
 // A whole warp's bounded wait: every lane gets the same answer, so that the warp stays together.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, int* status, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, code, kTimeoutNs));
 }
+__device__ __forceinline__ bool warp_test(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_test_wait(bar, parity));
+}
 
 __device__ __forceinline__ float2 f2(uint32_t a, uint32_t b) {
   return make_float2(__uint_as_float(a), __uint_as_float(b));
 }
 
-// Rows ra, rb of a 64-wide accumulator block (32 registers, 16x256b), scaled, to a staged bf16 tile.
-__device__ __forceinline__ void stage_rows(uint32_t stg, const Lane& l, const uint32_t (&o)[32], float sa, float sb) {
-  const float2 a2 = make_float2(sa, sa), b2 = make_float2(sb, sb);
-#pragma unroll
-  for (int jd = 0; jd < 8; ++jd) {
-    const float2 ya = __fmul2_rn(f2(o[4 * jd], o[4 * jd + 1]), a2);
-    const float2 yb = __fmul2_rn(f2(o[4 * jd + 2], o[4 * jd + 3]), b2);
-    st_shared_u32(stg + (uint32_t)l.ra * 128u + (uint32_t)(((jd ^ (l.ra & 7)) & 7) << 4) + 4u * l.t0,
-                  pack_bf16x2(ya.x, ya.y));
-    st_shared_u32(stg + (uint32_t)l.rb * 128u + (uint32_t)(((jd ^ (l.rb & 7)) & 7) << 4) + 4u * l.t0,
-                  pack_bf16x2(yb.x, yb.y));
+// ------------------------------------------------------------------------------------------
+// Rows and keys of one thread of a softmax warp. Warps 4..11: rows ra and rb = ra + 8. Warps 2 and 3
+// (kRem): one row, which is the rb of warp 2's TMEM lanes and the ra of warp 3's. A thread holds keys
+// 8j + 2 t0 and 8j + 2 t0 + 1 of each of its rows, j = 0..17.
+// ------------------------------------------------------------------------------------------
+template <bool kRem>
+struct Lane {
+  static constexpr int kRows = kRem ? 1 : 2;
+  int t0, t1, row[kRows];
+  bool hi;        // kRem: the row is in the rb registers
+  uint32_t addr;  // TMEM lane offset of the warp's 16 lanes
+  __device__ __forceinline__ Lane(int warp, int lane) {
+    t0 = lane & 3;
+    t1 = lane >> 2;
+    if constexpr (kRem) {
+      hi = warp == 2;
+      row[0] = (hi ? 128 : 136) + t1;
+      addr = (uint32_t)(32 * warp) << 16;
+    } else {
+      hi = false;
+      const int base = 32 * (warp & 3) + 16 * ((warp - 4) >> 2);
+      row[0] = base + t1;
+      row[1] = base + 8 + t1;
+      addr = (uint32_t)base << 16;
+    }
   }
-}
+  // The pair of row r in the four accumulator registers of an 8-key block.
+  __device__ __forceinline__ float2 pick(const uint32_t* v, int r) const {
+    if constexpr (kRem) return hi ? f2(v[2], v[3]) : f2(v[0], v[1]);
+    else return f2(v[2 * r], v[2 * r + 1]);
+  }
+  // Row r is row[0] + 8 r and row[0] % 8 = t1, so that the swizzle terms of both rows are equal.
+  // Two bf16 of row r, 8-key block j, into a P-shaped operand tile.
+  __device__ __forceinline__ void store_p(uint32_t sP, int j, int r, uint32_t v) const {
+    if (j < 16)
+      st_shared_u32(sP + row[0] * 128 + 4 * t0 + (((j & 7) ^ t1) << 4) + (j >> 3) * kPChunk + r * 1024, v);
+    else
+      st_shared_u32(sP + row[0] * 32 + 4 * t0 + ((((j & 1) ^ (t1 >> 2)) & 1) << 4) + 2 * kPChunk + r * 256, v);
+  }
+  // Row r of a 64-wide accumulator block (32 registers, 16x256b), scaled, to a staged bf16 tile.
+  __device__ __forceinline__ void stage(uint32_t stg, const uint32_t (&o)[32], int r, float scale) const {
+    const float2 s2 = make_float2(scale, scale);
+#pragma unroll
+    for (int jd = 0; jd < 8; ++jd) {
+      const float2 y = __fmul2_rn(pick(&o[4 * jd], r), s2);
+      st_shared_u32(stg + row[0] * 128 + 4 * t0 + ((jd ^ t1) << 4) + r * 1024, pack_bf16x2(y.x, y.y));
+    }
+  }
+};
+
+// The bias of this thread's pairs (see bias_rows).
+template <bool kRem>
+struct Bias {
+  float2 b[18][Lane<kRem>::kRows];
+  __device__ __forceinline__ void fetch(const Params& p, int h, const Lane<kRem>& l, int lane) {
+    const float4* src = bias_rows(p, h, l.row[0], lane);
+#pragma unroll
+    for (int j = 0; j < 18; ++j) {
+      if constexpr (kRem) {
+        b[j][0] = __ldg(reinterpret_cast<const float2*>(src + j * 32) + (l.row[0] >= 136 ? 1 : 0));
+      } else {
+        const float4 v = __ldg(src + j * 32);
+        b[j][0] = make_float2(v.x, v.y);
+        b[j][1] = make_float2(v.z, v.w);
+      }
+    }
+  }
+};
+
+// A byte mask's row of this thread (global memory), null past N.
+template <bool kRem>
+struct ByteMask {
+  const uint8_t* m[Lane<kRem>::kRows];
+  __device__ __forceinline__ void begin(const Params& p, const Lane<kRem>& l, int w) {
+    const uint8_t* base = p.mask + (int64_t)(w % p.nW) * p.N * p.N;
+#pragma unroll
+    for (int r = 0; r < l.kRows; ++r) m[r] = l.row[r] < p.N ? base + l.row[r] * p.N : nullptr;
+  }
+  // Adds -100 (log2 domain) to the masked logits of 8-key block j.
+  __device__ __forceinline__ void apply(const Params& p, const Lane<kRem>& l, int j, int r, float2& x) const {
+    const int key = 8 * j + 2 * l.t0;
+    if (m[r] && key < p.N && __ldg(m[r] + key)) x.x += kMaskedLog2;
+    if (m[r] && key + 1 < p.N && __ldg(m[r] + key + 1)) x.y += kMaskedLog2;
+  }
+};
+
+// ------------------------------------------------------------------------------------------
+// Region masks: a window's ids, ranked, by one warp; lane holds tokens lane + 32 m.
+// ------------------------------------------------------------------------------------------
+struct Regions {
+  uint32_t id[5];
+  uint32_t present[8];  // bit i of word k: id 32 k + i occurs
+  int steps;            // mask K-steps: 0 for one region
+  __device__ __forceinline__ void load(const Params& p, int w, int lane) {
+    const uint8_t* g = p.mask + (int64_t)(w % p.nW) * p.N;
+#pragma unroll
+    for (int m = 0; m < 5; ++m) id[m] = lane + 32 * m < p.N ? (uint32_t)__ldg(g + lane + 32 * m) : 256u;
+  }
+  __device__ __forceinline__ void classify() {
+    const uint32_t first = __shfl_sync(0xffffffffu, id[0], 0);
+    bool differ = false;
+#pragma unroll
+    for (int m = 0; m < 5; ++m) differ = differ || (id[m] != first && id[m] < 256u);
+    steps = 0;
+    if (!__any_sync(0xffffffffu, differ)) return;
+    int distinct = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int m = 0; m < 5; ++m) bits |= (id[m] >> 5) == (uint32_t)k ? 1u << (id[m] & 31) : 0u;
+      present[k] = __reduce_or_sync(0xffffffffu, bits);
+      distinct += __popc(present[k]);
+    }
+    steps = (distinct + 15) >> 4;
+  }
+  __device__ __forceinline__ int rank(uint32_t v) const {
+    int r = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t below = (v >> 5) > (uint32_t)k ? 0xffffffffu : (v >> 5) == (uint32_t)k ? (1u << (v & 31)) - 1u : 0u;
+      r += __popc(present[k] & below);
+    }
+    return r;
+  }
+  // The A and B operands of step `st` (32-byte swizzle rows of 16 bf16) at shared address `op`.
+  __device__ __noinline__ void build(uint32_t op, int st, int lane, uint32_t a_bits, uint32_t b_bits) const {
+    const uint32_t fill = b_bits | (b_bits << 16);
+#pragma unroll 1
+    for (int m = 0; m < 5; ++m) {
+      const int r = lane + 32 * m;
+      if (r >= kMaxN) break;
+      const uint32_t v = m == 0 ? id[0] : m == 1 ? id[1] : m == 2 ? id[2] : m == 3 ? id[3] : id[4];
+      const int slot = v < 256u ? rank(v) - 16 * st : -1;
+      const bool in = slot >= 0 && slot < 16;
+      const uint32_t sel = 0xffffu << (16 * (slot & 1)), a = a_bits << (16 * (slot & 1));
+      uint32_t wa[8], wb[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool hot = in && (slot >> 1) == e;
+        wa[e] = hot ? a : 0u;
+        wb[e] = v >= 256u ? 0u : hot ? fill & ~sel : fill;
+      }
+      const uint32_t row = op + (uint32_t)r * 32u, swz = (uint32_t)((r >> 2) & 1) << 4;
+      st_shared_v4(row + swz, wa[0], wa[1], wa[2], wa[3]);
+      st_shared_v4(row + (swz ^ 16u), wa[4], wa[5], wa[6], wa[7]);
+      st_shared_v4(row + kRow32 + swz, wb[0], wb[1], wb[2], wb[3]);
+      st_shared_v4(row + kRow32 + (swz ^ 16u), wb[4], wb[5], wb[6], wb[7]);
+    }
+    fence_proxy_async_shared();
+    __syncwarp();
+  }
+};
+
+struct Ctx {
+  uint32_t sbase, bar0, tmem;
+  volatile int* abort;
+  volatile int* steps;  // mask steps of a tile, by slot
+  int t_begin, n_local;
+  __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8u * (uint32_t)i; }
+};
 
 // ------------------------------------------------------------------------------------------
 // Forward.
-//   warps 0, 2  TMA producers: Q, K and the region ids (warp 0), V (warp 2), 3-slot rings; the output
-//               of a tile is staged in its V slot and stored by warp 2 before the slot's reuse;
+//   warp 0      TMA producer: Q and K, V, 3-slot rings, and the mask operands; the output of a tile is
+//               staged in its V slot and stored before the slot's reuse;
 //   warp 1      TMEM owner and UMMA issuer:  S = Q K^T (M=128 and M=64), O = P V (M=128 and M=64);
-//   warps 3-11  x = S scale + bias (+ mask), softmax in the log2 domain, P to shared memory in bf16,
-//               then the previous tile's output rows.
+//   warps 2-11  x = S scale + bias, softmax in the log2 domain, P to shared memory in bf16, then the
+//               previous tile's output rows.
 // ------------------------------------------------------------------------------------------
 namespace fwd {
 
@@ -214,51 +258,40 @@ constexpr int kStages = 3;
 constexpr int kQKBytes = 2 * kTileBytes;
 constexpr int kStageBytes = 3 * kTileBytes;
 constexpr int kOffP = kStages * kStageBytes;
-constexpr int kOffRem = kOffP + kPBytes;
-constexpr int kOffIds = kOffRem + kRemBytes;
-// Region ids have a ring of their own: slot i % kIdSlots is rewritten for tile i + kIdSlots once the S
-// product of tile i + kIdSlots - 3 is done, which follows every softmax warp's load of S of tile
-// i + kIdSlots - 4 >= i + 1, so its work on tile i.
-constexpr int kIdSlots = 5;
-constexpr int kOffBars = kOffIds + kIdSlots * kIdBytes;
+constexpr int kOffMask = kOffP + kPBytes;  // two mask steps in flight
+constexpr int kOffBars = kOffMask + 2 * kMaskOpBytes;
+constexpr int kInfoSlots = 4;  // tile i + 4 is classified after S of tile i + 1 is done, which follows tile i's
 enum { kFullQK = 0, kEmptyQK = 3, kFullV = 6, kStaged = 9, kSFull = 12, kSFree, kPFull, kPEmpty, kOFull = 16,
-       kOFree = 18, kDone = 20, kIds = 21, kNumBars = kIds + kIdSlots };
-constexpr int kSmem = kOffBars + kNumBars * 8 + 16 + 1024;
+       kOFree = 18, kDone = 20, kMaskFull = 21, kMaskEmpty = 23, kInfo = 25, kNumBars = kInfo + kInfoSlots };
+constexpr int kSmem = kOffBars + kNumBars * 8 + 64 + 1024;
 static_assert(kSmem <= 227 * 1024, "shared memory budget");
 constexpr uint32_t kColS = 0, kColS2 = 160, kColO0 = 320, kColO1 = 384, kColO2 = 448;
 constexpr uint32_t kRegsSmall = 120, kRegsMain = 192;
 static_assert(4 * kRegsSmall + 8 * kRegsMain <= 12 * kRegsLaunch, "register split");
-
-struct Ctx {
-  uint32_t sbase, bar0, tmem;
-  uint8_t* smem;
-  volatile int* abort;
-  int t_begin, n_local;
-  __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8u * (uint32_t)i; }
-};
+constexpr int kSoftmaxWarps = 10;
 
 template <bool kRem, int kMask>
 __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int warp, int lane) {
-  const Lane l = make_lane(warp, lane);
-  const uint32_t s_col = kRem ? kColS2 : kColS;
+  const Lane<kRem> l(warp, lane);
+  constexpr int R = Lane<kRem>::kRows;
+  const uint32_t tS = c.tmem + l.addr + (kRem ? kColS2 : kColS);
   const uint32_t sP = c.sbase + kOffP;
   Bias<kRem> bias;
-  bias.smem = c.sbase + kOffRem + lane * 16;
   int cur_h = -1, prev = -1;
-  float la_prev = 1.f, lb_prev = 1.f;
+  float l_prev[R];
 
-  auto epilogue = [&](int j, float la, float lb) -> bool {
+  auto epilogue = [&](int j) -> bool {
     const int ob = j & 1;
     if (!warp_wait(c.bar(kOFull + ob), (uint32_t)((j >> 1) & 1), c.abort, p.status, 101)) return false;
     tc_fence_after();
     uint32_t o[32];
-    const uint32_t col = kRem ? kColO2 + (ob ? kLaneHalf : 0u) : (ob ? kColO1 : kColO0);
-    tmem_ld_16x256b_r32(c.tmem + l.addr + col, o);
+    tmem_ld_16x256b_r32(c.tmem + l.addr + (kRem ? kColO2 + (ob ? kLaneHalf : 0u) : (ob ? kColO1 : kColO0)), o);
     tmem_wait_ld();
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bar(kOFree + ob));
-    stage_rows(c.sbase + (j % kStages) * kStageBytes + kQKBytes, l, o, 1.f / la, 1.f / lb);
+#pragma unroll
+    for (int r = 0; r < R; ++r) l.stage(c.sbase + (j % kStages) * kStageBytes + kQKBytes, o, r, 1.f / l_prev[r]);
     fence_proxy_async_shared();
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bar(kStaged + j % kStages));
@@ -273,98 +306,279 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
       cur_h = h;
       bias.fetch(p, h, l, lane);
     }
-    TileMask<kMask> mask;
-    if constexpr (kMask == kGroups) {
-      if (!warp_wait(c.bar(kIds + i % kIdSlots), (uint32_t)((i / kIdSlots) & 1), c.abort, p.status, 102)) {
-        ok = false;
-        break;
-      }
-    }
-    mask.begin(p, l, w, c.smem + kOffIds + (i % kIdSlots) * kIdBytes);
-    if (!warp_wait(c.bar(kSFull), (uint32_t)(i & 1), c.abort, p.status, 103)) { ok = false; break; }
+    if (!warp_wait(c.bar(kSFull), (uint32_t)(i & 1), c.abort, p.status, 102)) { ok = false; break; }
     tc_fence_after();
-    uint32_t v[72];
-    {
+    float2 x[18][R];
+    if constexpr (kRem) {
+#pragma unroll
+      for (int q = 0; q < 9; q += 3) {
+        uint32_t a[3][8];
+#pragma unroll
+        for (int e = 0; e < 3; ++e) tmem_ld_16x256b_r8(tS + 16 * (q + e), a[e]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 6; ++e) x[2 * q + e][0] = l.pick(&a[e >> 1][4 * (e & 1)], 0);
+      }
+    } else {
       uint32_t a[64], b[8];
-      tmem_ld_16x256b_r64(c.tmem + l.addr + s_col, a);
-      tmem_ld_16x256b_r8(c.tmem + l.addr + s_col + 128, b);
+      tmem_ld_16x256b_r64(tS, a);
+      tmem_ld_16x256b_r8(tS + 128, b);
       tmem_wait_ld();
 #pragma unroll
-      for (int k = 0; k < 64; ++k) v[k] = a[k];
+      for (int j = 0; j < 18; ++j)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[64 + k] = b[k];
+        for (int r = 0; r < R; ++r) x[j][r] = j < 16 ? l.pick(&a[4 * (j & 15)], r) : l.pick(&b[4 * (j & 1)], r);
     }
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bar(kSFree));
-    // The mask has a loop of its own behind one branch: inside this loop its 18 branches keep the
-    // compiler from interleaving the blocks, which doubled the kernel's time even where none is taken.
 #pragma unroll
-    for (int j = 0; j < 18; ++j) {
-      const float4 b = bias.get(j);
-      const float2 xa = __ffma2_rn(f2(v[4 * j], v[4 * j + 1]), c2, make_float2(b.x, b.y));
-      const float2 xb = __ffma2_rn(f2(v[4 * j + 2], v[4 * j + 3]), c2, make_float2(b.z, b.w));
-      v[4 * j] = __float_as_uint(xa.x);
-      v[4 * j + 1] = __float_as_uint(xa.y);
-      v[4 * j + 2] = __float_as_uint(xb.x);
-      v[4 * j + 3] = __float_as_uint(xb.y);
+    for (int j = 0; j < 18; ++j)
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[j][r] = __ffma2_rn(x[j][r], c2, bias.b[j][r]);
+    if constexpr (kMask == kMaskU8) {
+      ByteMask<kRem> mask;
+      mask.begin(p, l, w);
+#pragma unroll
+      for (int j = 0; j < 18; ++j)
+#pragma unroll
+        for (int r = 0; r < R; ++r) mask.apply(p, l, j, r, x[j][r]);
     }
-    if (kMask != kNoMask && mask.on) {
+    float mx[R], sum[R];
+    uint32_t pk[18][R];
 #pragma unroll
-      for (int j = 0; j < 18; ++j) {
-        float2 xa = f2(v[4 * j], v[4 * j + 1]), xb = f2(v[4 * j + 2], v[4 * j + 3]);
-        mask.apply(p, l, j, xa, xb);
-        v[4 * j] = __float_as_uint(xa.x);
-        v[4 * j + 1] = __float_as_uint(xa.y);
-        v[4 * j + 2] = __float_as_uint(xb.x);
-        v[4 * j + 3] = __float_as_uint(xb.y);
+    for (int r = 0; r < R; ++r) {
+      mx[r] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 18; ++j) mx[r] = fmax3(mx[r], x[j][r].x, x[j][r].y);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+#pragma unroll
+    for (int r = 0; r < R; ++r) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+    float2 s2[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) s2[r] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 18; ++j)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float2 y = __fadd2_rn(x[j][r], make_float2(-mx[r], -mx[r]));
+        const float2 e = make_float2(ex2(y.x), ex2(y.y));
+        s2[r] = __fadd2_rn(s2[r], e);
+        pk[j][r] = pack_bf16x2(e.x, e.y);
       }
-    }
-    float mxa = -INFINITY, mxb = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 18; ++j) {
-      mxa = fmax3(mxa, __uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]));
-      mxb = fmax3(mxb, __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
-    }
-    mxa = fmaxf(mxa, __shfl_xor_sync(0xffffffffu, mxa, 1));
-    mxa = fmaxf(mxa, __shfl_xor_sync(0xffffffffu, mxa, 2));
-    mxb = fmaxf(mxb, __shfl_xor_sync(0xffffffffu, mxb, 1));
-    mxb = fmaxf(mxb, __shfl_xor_sync(0xffffffffu, mxb, 2));
-    const float2 ma2 = make_float2(-mxa, -mxa), mb2 = make_float2(-mxb, -mxb);
-    float2 la2 = make_float2(0.f, 0.f), lb2 = make_float2(0.f, 0.f);
-    uint32_t pa[18], pb[18];
+    for (int r = 0; r < R; ++r) sum[r] = s2[r].x + s2[r].y;
 #pragma unroll
-    for (int j = 0; j < 18; ++j) {
-      const float2 ya = __fadd2_rn(f2(v[4 * j], v[4 * j + 1]), ma2);
-      const float2 yb = __fadd2_rn(f2(v[4 * j + 2], v[4 * j + 3]), mb2);
-      const float2 ea = make_float2(ex2(ya.x), ex2(ya.y)), eb = make_float2(ex2(yb.x), ex2(yb.y));
-      la2 = __fadd2_rn(la2, ea);
-      lb2 = __fadd2_rn(lb2, eb);
-      pa[j] = pack_bf16x2(ea.x, ea.y);
-      pb[j] = pack_bf16x2(eb.x, eb.y);
-    }
-    float la = la2.x + la2.y, lb = lb2.x + lb2.y;
-    la += __shfl_xor_sync(0xffffffffu, la, 1);
-    la += __shfl_xor_sync(0xffffffffu, la, 2);
-    lb += __shfl_xor_sync(0xffffffffu, lb, 1);
-    lb += __shfl_xor_sync(0xffffffffu, lb, 2);
-    if (!warp_wait(c.bar(kPEmpty), (uint32_t)((i & 1) ^ 1), c.abort, p.status, 104)) { ok = false; break; }
+    for (int r = 0; r < R; ++r) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
 #pragma unroll
-    for (int j = 0; j < 18; ++j) store_p(sP, l, j, pa[j], pb[j]);
+    for (int r = 0; r < R; ++r) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    if (!warp_wait(c.bar(kPEmpty), (uint32_t)((i & 1) ^ 1), c.abort, p.status, 103)) { ok = false; break; }
+#pragma unroll
+    for (int j = 0; j < 18; ++j)
+#pragma unroll
+      for (int r = 0; r < R; ++r) l.store_p(sP, j, r, pk[j][r]);
     fence_proxy_async_shared();
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bar(kPFull));
     if (p.stats && l.t0 == 0) {
       float2* st = p.stats + ((int64_t)w * p.H + h) * p.N;
-      if (l.ra < p.N) st[l.ra] = make_float2(mxa, log2f(la));
-      if (l.rb < p.N) st[l.rb] = make_float2(mxb, log2f(lb));
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (l.row[r] < p.N) st[l.row[r]] = make_float2(mx[r], log2f(sum[r]));
     }
-    if (prev >= 0 && !epilogue(prev, la_prev, lb_prev)) { ok = false; break; }
+    if (prev >= 0 && !epilogue(prev)) { ok = false; break; }
     prev = i;
-    la_prev = la;
-    lb_prev = lb;
+#pragma unroll
+    for (int r = 0; r < R; ++r) l_prev[r] = sum[r];
   }
-  if (ok && prev >= 0) epilogue(prev, la_prev, lb_prev);
+  if (ok && prev >= 0) epilogue(prev);
+}
+
+template <int kMask>
+__device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane, const CUtensorMap* tmq,
+                                         const CUtensorMap* tmk, const CUtensorMap* tmv, const CUtensorMap* tmo) {
+  const int n = c.n_local;
+  if (lane == 0) {
+    tma_prefetch_desc(tmq);
+    tma_prefetch_desc(tmk);
+    tma_prefetch_desc(tmv);
+  }
+  auto store_out = [&](int j) {
+    const int t = c.t_begin + j, h = t / p.Bwin;
+    tma_store_4d(tmo, c.sbase + (j % kStages) * kStageBytes + kQKBytes, 0, 0, h, t - h * p.Bwin);
+    bulk_commit_group();
+  };
+  int qk_issued = 0, v_issued = 0, jobs = 0;
+  Regions now, next;
+  if constexpr (kMask == kGroups) {
+    if (n > 0) next.load(p, c.t_begin % p.Bwin, lane);
+  }
+  // Step i loads Q and K of tile i, then V of tile i - 1, whose slot is freed about as late.
+  for (int i = 0; i <= n; ++i) {
+    int ok = 1;
+    if (i < n) {
+      const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i % kStages;
+      if constexpr (kMask == kGroups) {
+        now = next;
+        if (i + 1 < n) next.load(p, (t + 1) % p.Bwin, lane);  // one tile ahead
+      }
+      if (lane == 0) {
+        ok = mbar_wait(c.bar(kEmptyQK + s), (uint32_t)(((i / kStages) & 1) ^ 1), c.abort, p.status, 105, kTimeoutNs);
+        if (ok) {
+          const uint32_t dst = c.sbase + s * kStageBytes;
+          mbar_arrive_expect_tx(c.bar(kFullQK + s), kQKBytes);
+          tma_load_4d(dst, tmq, c.bar(kFullQK + s), 0, 0, h, w);
+          tma_load_4d(dst + kTileBytes, tmk, c.bar(kFullQK + s), 0, 0, h, w);
+          ++qk_issued;
+        }
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if constexpr (kMask == kGroups) {
+        now.classify();
+        if (lane == 0) {
+          c.steps[i % kInfoSlots] = now.steps;
+          mbar_arrive(c.bar(kInfo + i % kInfoSlots));
+        }
+        for (int st = 0; st < now.steps; ++st, ++jobs) {
+          const int b = jobs & 1;
+          if (!warp_wait(c.bar(kMaskEmpty + b), (uint32_t)(((jobs >> 1) & 1) ^ 1), c.abort, p.status, 104)) { ok = 0; break; }
+          now.build(c.sbase + kOffMask + b * kMaskOpBytes, st, lane, p.mask_a, p.mask_b);
+          if (lane == 0) mbar_arrive(c.bar(kMaskFull + b));
+        }
+        if (!ok) break;
+      }
+    }
+    if (i > 0) {
+      if (lane == 0) {
+        const int j = i - 1, t = c.t_begin + j, h = t / p.Bwin, s = j % kStages;
+        if (j >= kStages) {
+          // The slot still holds the output of tile j - 3: store it and wait until it has been read.
+          ok = mbar_wait(c.bar(kStaged + s), (uint32_t)(((j - kStages) / kStages) & 1), c.abort, p.status, 107, kTimeoutNs);
+          if (ok) {
+            store_out(j - kStages);
+            bulk_wait_group_read0();
+          }
+        }
+        if (ok) {
+          mbar_arrive_expect_tx(c.bar(kFullV + s), kTileBytes);
+          tma_load_4d(c.sbase + s * kStageBytes + kQKBytes, tmv, c.bar(kFullV + s), 0, 0, h, t - h * p.Bwin);
+          ++v_issued;
+        }
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+    }
+  }
+  if (lane == 0) {
+    // Never leave with copies in flight (bounded, also after an abort).
+    int no_abort = 0;
+    for (int j = qk_issued > kStages ? qk_issued - kStages : 0; j < qk_issued; ++j)
+      mbar_wait(c.bar(kFullQK + j % kStages), (uint32_t)((j / kStages) & 1), &no_abort, p.status, 106, kTimeoutNs);
+    for (int j = v_issued > kStages ? v_issued - kStages : 0; j < v_issued; ++j)
+      mbar_wait(c.bar(kFullV + j % kStages), (uint32_t)((j / kStages) & 1), &no_abort, p.status, 108, kTimeoutNs);
+    for (int j = n > kStages ? n - kStages : 0; j < n; ++j) {
+      if (!mbar_wait(c.bar(kStaged + j % kStages), (uint32_t)((j / kStages) & 1), c.abort, p.status, 109, kTimeoutNs))
+        break;
+      store_out(j);
+    }
+    bulk_wait_group0();
+  }
+}
+
+// S and PV in whatever order their inputs become ready.
+template <int kMask>
+__device__ __forceinline__ void issuer(const Params& p, const Ctx& c) {
+  const int n = c.n_local;
+  const bool leader = elect_one();
+  const uint64_t dQ = desc_sw128(c.sbase, 16, 1024), dV = desc_sw128(c.sbase + kQKBytes, kTileBytes, 1024);
+  const uint64_t dP = desc_sw128(c.sbase + kOffP, 16, 1024), dP32 = desc_sw32(c.sbase + kOffP + 2 * kPChunk, 256);
+  const uint64_t dM = desc_sw32(c.sbase + kOffMask, 256);
+  int ns = 0, npv = 0, jobs = 0;
+  uint64_t t_last = cycles();
+  uint32_t idle = 0;
+  bool ok = true;
+  while (ok && npv < n) {
+    bool progressed = false;
+    if (ns < n) {
+      const int s = ns % kStages;
+      bool ready = warp_test(c.bar(kFullQK + s), (uint32_t)((ns / kStages) & 1)) &&
+                   warp_test(c.bar(kSFree), (uint32_t)((ns & 1) ^ 1));
+      if constexpr (kMask == kGroups)
+        ready = ready && warp_test(c.bar(kInfo + ns % kInfoSlots), (uint32_t)((ns / kInfoSlots) & 1));
+      if (ready) {
+        tc_fence_after();
+        const uint64_t q = at(dQ, s * kStageBytes), k = at(q, kTileBytes);
+        if (leader) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            umma_f16(c.tmem + kColS, at(q, e * 32), at(k, e * 32), kIdescS, e > 0 ? 1u : 0u);
+            umma_f16(c.tmem + kColS2, at(q, kRemOff + e * 32), at(k, e * 32), kIdescS2, e > 0 ? 1u : 0u);
+          }
+        }
+        if constexpr (kMask == kGroups) {
+          for (int st = c.steps[ns % kInfoSlots]; st > 0; --st, ++jobs) {
+            const int b = jobs & 1;
+            ok = warp_wait(c.bar(kMaskFull + b), (uint32_t)((jobs >> 1) & 1), c.abort, p.status, 112);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+              const uint64_t a = at(dM, b * kMaskOpBytes), bb = at(a, kRow32);
+              umma_f16(c.tmem + kColS, a, bb, kIdescS, 1u);
+              umma_f16(c.tmem + kColS2, at(a, kRemOff32), bb, kIdescS2, 1u);
+              umma_commit(c.bar(kMaskEmpty + b));
+            }
+          }
+          if (!ok) break;
+        }
+        if (leader) {
+          umma_commit(c.bar(kSFull));
+          umma_commit(c.bar(kEmptyQK + s));
+        }
+        ++ns;
+        progressed = true;
+      }
+    }
+    if (npv < ns) {
+      const int s = npv % kStages, ob = npv & 1;
+      if (warp_test(c.bar(kPFull), (uint32_t)(npv & 1)) && warp_test(c.bar(kFullV + s), (uint32_t)((npv / kStages) & 1)) &&
+          warp_test(c.bar(kOFree + ob), (uint32_t)(((npv >> 1) & 1) ^ 1))) {
+        tc_fence_after();
+        if (leader) {
+          const uint64_t v = at(dV, s * kStageBytes);
+          const uint32_t o = c.tmem + (ob ? kColO1 : kColO0), o2 = c.tmem + kColO2 + (ob ? kLaneHalf : 0u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t off = (e >> 2) * kPChunk + (e & 3) * 32;
+            umma_f16(o, at(dP, off), at(v, e * 2048), kIdescO, e > 0 ? 1u : 0u);
+            umma_f16(o2, at(dP, off + kRemOff), at(v, e * 2048), kIdescO2, e > 0 ? 1u : 0u);
+          }
+          umma_f16(o, dP32, at(v, 8 * 2048), kIdescO, 1u);  // keys 128..143
+          umma_f16(o2, at(dP32, kRemOff32), at(v, 8 * 2048), kIdescO2, 1u);
+          umma_commit(c.bar(kOFull + ob));
+          umma_commit(c.bar(kPEmpty));
+        }
+        ++npv;
+        progressed = true;
+      }
+    }
+    if (progressed) {
+      idle = 0;
+      t_last = cycles();
+    } else if ((++idle & 63u) == 0) {
+      bool stop = *c.abort != 0;
+      if (cycles() - t_last > ns_to_cycles(kTimeoutNs)) {
+        atomicCAS(p.status, 0, 110);
+        *c.abort = 1;
+        stop = true;
+      }
+      if (__any_sync(0xffffffffu, stop)) break;
+    }
+  }
+  if (leader) umma_commit(c.bar(kDone));
+  int no_abort = 0;
+  mbar_wait(c.bar(kDone), 0, &no_abort, p.status, 111, kTimeoutNs);
+  __syncwarp();
 }
 
 template <int kMask>
@@ -375,197 +589,40 @@ rel_bias_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kNumBars);
-  __shared__ int abort_flag;
+  int* words = reinterpret_cast<int*>(bars + kNumBars);  // abort flag, TMEM address, mask steps
   Ctx c;
-  c.smem = smem;
   c.sbase = smem_u32(smem);
   c.bar0 = smem_u32(bars);
-  c.abort = &abort_flag;
+  c.abort = words;
+  c.steps = words + 4;
   c.t_begin = tile_begin(p.num_tiles);
   c.n_local = tile_end(p.num_tiles) - c.t_begin;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(c.bar(kFullQK + s), 1);
-      mbar_init(c.bar(kEmptyQK + s), 1);
-      mbar_init(c.bar(kFullV + s), 1);
-      mbar_init(c.bar(kStaged + s), 9);
+    *words = 0;
+    for (int b = 0; b < kNumBars; ++b) {
+      const bool all = (b >= kStaged && b < kStaged + kStages) || b == kSFree || b == kPFull || b == kOFree || b == kOFree + 1;
+      mbar_init(c.bar(b), all ? kSoftmaxWarps : 1);
     }
-    mbar_init(c.bar(kSFull), 1);
-    mbar_init(c.bar(kSFree), 9);
-    mbar_init(c.bar(kPFull), 9);
-    mbar_init(c.bar(kPEmpty), 1);
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(c.bar(kOFull + b), 1);
-      mbar_init(c.bar(kOFree + b), 9);
-    }
-    mbar_init(c.bar(kDone), 1);
-    for (int b = 0; b < kIdSlots; ++b) mbar_init(c.bar(kIds + b), 1);
     fence_mbarrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_holder), kTmemCols);
+    tmem_alloc(smem_u32(words + 1), kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  c.tmem = *tmem_holder;
-  const int n = c.n_local;
+  c.tmem = (uint32_t)*reinterpret_cast<volatile int*>(words + 1);
 
   if (warp >= 4) {
     warpgroup_reg_alloc<kRegsMain>();
     softmax_warps<false, kMask>(p, c, warp, lane);
   } else {
     warpgroup_reg_dealloc<kRegsSmall>();
-    if (warp == 3) {
-      softmax_warps<true, kMask>(p, c, warp, lane);
-    } else if (warp == 0) {
-      if (lane == 0) {
-        tma_prefetch_desc(&tmq);
-        tma_prefetch_desc(&tmk);
-      }
-      int last_par[kStages] = {-1, -1, -1};
-      uint32_t id[5], next_id[5];
-      if constexpr (kMask == kGroups) {
-        if (n > 0) load_ids(p, c.t_begin % p.Bwin, lane, next_id);
-      }
-      for (int i = 0; i < n; ++i) {
-        const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i % kStages;
-        const uint32_t ph = (uint32_t)((i / kStages) & 1);
-        if constexpr (kMask == kGroups) {
-#pragma unroll
-          for (int m = 0; m < 5; ++m) id[m] = next_id[m];
-          if (i + 1 < n) load_ids(p, (t + 1) % p.Bwin, lane, next_id);  // one tile ahead
-        }
-        int ok = 1;
-        if (lane == 0) ok = mbar_wait(c.bar(kEmptyQK + s), ph ^ 1u, c.abort, p.status, 105, kTimeoutNs);
-        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        if (lane == 0) {
-          const uint32_t dst = c.sbase + s * kStageBytes;
-          mbar_arrive_expect_tx(c.bar(kFullQK + s), kQKBytes);
-          tma_load_4d(dst, &tmq, c.bar(kFullQK + s), 0, 0, h, w);
-          tma_load_4d(dst + kTileBytes, &tmk, c.bar(kFullQK + s), 0, 0, h, w);
-          last_par[s] = (int)ph;
-        }
-        if constexpr (kMask == kGroups) {
-          store_ids(smem + kOffIds + (i % kIdSlots) * kIdBytes, lane, id);
-          if (lane == 0) mbar_arrive(c.bar(kIds + i % kIdSlots));
-        }
-      }
-      if (lane == 0) {
-        // Never leave with copies in flight (bounded, also after an abort).
-        int no_abort = 0;
-        for (int s = 0; s < kStages; ++s)
-          if (last_par[s] >= 0) mbar_wait(c.bar(kFullQK + s), (uint32_t)last_par[s], &no_abort, p.status, 106, kTimeoutNs);
-      }
-    } else if (warp == 2) {
-      if (lane == 0) tma_prefetch_desc(&tmv);
-      int last_par[kStages] = {-1, -1, -1};
-      auto store_out = [&](int j) {
-        const int t = c.t_begin + j, h = t / p.Bwin;
-        tma_store_4d(&tmo, c.sbase + (j % kStages) * kStageBytes + kQKBytes, 0, 0, h, t - h * p.Bwin);
-        bulk_commit_group();
-      };
-      for (int i = 0; i < n; ++i) {
-        const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i % kStages;
-        int ok = 1;
-        if (lane == 0 && i >= kStages) {
-          // The slot still holds the output of tile i - 3: store it and wait until it has been read.
-          ok = mbar_wait(c.bar(kStaged + s), (uint32_t)(((i - kStages) / kStages) & 1), c.abort, p.status, 107, kTimeoutNs);
-          if (ok) {
-            store_out(i - kStages);
-            bulk_wait_group_read0();
-          }
-        }
-        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(c.bar(kFullV + s), kTileBytes);
-          tma_load_4d(c.sbase + s * kStageBytes + kQKBytes, &tmv, c.bar(kFullV + s), 0, 0, h, w);
-          last_par[s] = (i / kStages) & 1;
-        }
-      }
-      if (lane == 0) {
-        int no_abort = 0;
-        for (int s = 0; s < kStages; ++s)
-          if (last_par[s] >= 0) mbar_wait(c.bar(kFullV + s), (uint32_t)last_par[s], &no_abort, p.status, 108, kTimeoutNs);
-        for (int j = n > kStages ? n - kStages : 0; j < n; ++j) {
-          if (!mbar_wait(c.bar(kStaged + j % kStages), (uint32_t)((j / kStages) & 1), c.abort, p.status, 109, kTimeoutNs))
-            break;
-          store_out(j);
-        }
-        bulk_wait_group0();
-      }
-    } else if (lane == 0) {
-      // UMMA issuer: S and PV in whatever order their inputs become ready (non-blocking tests).
-      int ns = 0, npv = 0;
-      uint64_t t_last = cycles();
-      uint32_t idle = 0;
-      const uint32_t sP = c.sbase + kOffP;
-      while (npv < n) {
-        bool progressed = false;
-        if (ns < n) {
-          const int s = ns % kStages;
-          if (mbar_test_wait(c.bar(kFullQK + s), (uint32_t)((ns / kStages) & 1)) &&
-              mbar_test_wait(c.bar(kSFree), (uint32_t)((ns & 1) ^ 1))) {
-            tc_fence_after();
-            const uint32_t sQ = c.sbase + s * kStageBytes, sK = sQ + kTileBytes;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint64_t b = desc_sw128(sK + k * 32, 16, 1024);
-              umma_f16(c.tmem + kColS, desc_sw128(sQ + k * 32, 16, 1024), b, kIdescS, k > 0 ? 1u : 0u);
-              umma_f16(c.tmem + kColS2, desc_sw128(sQ + kRowOff80 + k * 32, 16, 1024), b, kIdescS2, k > 0 ? 1u : 0u);
-            }
-            umma_commit(c.bar(kSFull));
-            umma_commit(c.bar(kEmptyQK + s));
-            ++ns;
-            progressed = true;
-          }
-        }
-        if (npv < ns) {
-          const int j = npv, s = j % kStages, ob = j & 1;
-          if (mbar_test_wait(c.bar(kPFull), (uint32_t)(j & 1)) &&
-              mbar_test_wait(c.bar(kFullV + s), (uint32_t)((j / kStages) & 1)) &&
-              mbar_test_wait(c.bar(kOFree + ob), (uint32_t)(((j >> 1) & 1) ^ 1))) {
-            tc_fence_after();
-            const uint32_t sV = c.sbase + s * kStageBytes + kQKBytes;
-            const uint32_t dO = c.tmem + (ob ? kColO1 : kColO0);
-            const uint32_t dO2 = c.tmem + kColO2 + (ob ? kLaneHalf : 0u);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t pa = sP + (k >> 2) * kPChunk + (k & 3) * 32;
-              const uint64_t b = desc_sw128(sV + k * 2048, kTileBytes, 1024);
-              umma_f16(dO, desc_sw128(pa, 16, 1024), b, kIdescO, k > 0 ? 1u : 0u);
-              umma_f16(dO2, desc_sw128(pa + kRowOff80, 16, 1024), b, kIdescO2, k > 0 ? 1u : 0u);
-            }
-            const uint32_t pa = sP + 2 * kPChunk;  // keys 128..143
-            const uint64_t b = desc_sw128(sV + 8 * 2048, kTileBytes, 1024);
-            umma_f16(dO, desc_sw32(pa, 256), b, kIdescO, 1u);
-            umma_f16(dO2, desc_sw32(pa + kRowOff80_32, 256), b, kIdescO2, 1u);
-            umma_commit(c.bar(kOFull + ob));
-            umma_commit(c.bar(kPEmpty));
-            ++npv;
-            progressed = true;
-          }
-        }
-        if (progressed) {
-          idle = 0;
-          t_last = cycles();
-        } else if ((++idle & 63u) == 0) {
-          if (*c.abort) break;
-          if (cycles() - t_last > ns_to_cycles(kTimeoutNs)) {
-            atomicCAS(p.status, 0, 110);
-            *c.abort = 1;
-            break;
-          }
-        }
-      }
-      umma_commit(c.bar(kDone));
-      int no_abort = 0;
-      mbar_wait(c.bar(kDone), 0, &no_abort, p.status, 111, kTimeoutNs);
-    }
+    if (warp >= 2) softmax_warps<true, kMask>(p, c, warp, lane);
+    else if (warp == 1) issuer<kMask>(p, c);
+    else producer<kMask>(p, c, lane, &tmq, &tmk, &tmv, &tmo);
   }
   tc_fence_before();
   __syncthreads();
@@ -579,113 +636,57 @@ rel_bias_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
 
 // ------------------------------------------------------------------------------------------
 // Backward. Per tile:
-//   S = Q K^T, dP = dO V^T                     M=128 (rows 0..127) and M=64 (rows 80..143), N=144
+//   S = Q K^T, dP = dO V^T                     M=128 (rows 0..127) and M=64 (rows 88..151), N=144
 //   pass 1   P = exp2(x - max - log2 sum) from the forward's row statistics; delta = sum_k P dP; P
 //            replaces S in TMEM (fp32) and goes to shared memory in bf16
 //   dV = P^T dO                                runs while pass 2 computes
-//   pass 2   dS = P (dP - delta), added to the head's bias gradient (fp32, 72 registers of each
-//            thread), to shared memory in bf16 over P once dV is done
-//   dK = dS^T Q, dQ = dS K
+//   pass 2   dS = P (dP - delta), added to the head's bias gradient (fp32, in registers: 72 of each
+//            thread of warps 4..11), and to shared memory in bf16
+//   dQ = dS K, dK = dS^T Q                     dV and dQ are drained meanwhile; then S and dP of the next tile,
+//                                              while dK is drained
 // dV, dK, dQ of keys / rows 0..127 are M=128 UMMAs (P and dS are read MN-major for dV and dK); those
-// of 128..143 are computed transposed, (64 head dims) x (16 rows), as M=64, N=16 UMMAs, which costs
-// a quarter of an M=64, N=64 block.
-// TMEM columns: S / P 0..143, dP 144..287 (then dK 144..207 and dQ 208..271), the M=64 blocks of S
-// and dP in the two lane halves of 288..431 (then dQ's transposed remainder 416..431), dV 432..495,
-// the transposed remainders of dV and dK in the lane halves of 496..511.
-// Outputs are staged in the tile's own slots (dV over V, dK over K, dQ over Q) and stored by warp 0
-// before it loads the tile after next into them. Two input slots (147 KB) and one P / dS tile leave
-// no room for a second tile in flight: the chain of a tile is serial, its loads are not.
+// of 128..143 are computed transposed, (64 head dims) x (16 rows), as M=64, N=16 UMMAs, at half
+// the cost of an M=64, N=64 block.
+// TMEM columns: S / P 0..143, dP 144..287, the M=64 blocks of S and dP in the two lane halves of 288..431,
+// and over them, once pass 2 has read them, dQ 288..351, dK 352..415 and dQ's transposed remainder
+// 416..431; dV 432..495; the transposed remainders of dV and dK in the lane halves of 496..511.
+// Outputs are staged in the tile's own slots (dV over V, dK over K, dQ over dO, which dV was the last to
+// read) and stored by warp 0 before it loads the tile after next into them. Two input slots, P and dS fill shared memory (230 KB);
+// the mask operands of a tile are built in the P buffer, which is free between dV of the tile before and
+// the tile's own pass 1.
 // ------------------------------------------------------------------------------------------
 namespace bwd {
 
 constexpr int kStages = 2;
 constexpr int kOffQ = 0, kOffK = kTileBytes, kOffV = 2 * kTileBytes, kOffG = 3 * kTileBytes;
 constexpr int kStageBytes = 4 * kTileBytes;
-constexpr int kOffP = kStages * kStageBytes;
-constexpr int kOffRem = kOffP + kPBytes;          // warp 3's bias
-constexpr int kOffRemAcc = kOffRem + kRemBytes;   // warp 3's bias gradient
-constexpr int kOffIds = kOffRemAcc + kRemBytes;
-constexpr int kOffBars = kOffIds + kStages * kIdBytes;
-enum { kFull = 0, kStaged = 2, kSFull = 4, kPFull, kDvFull, kDsFull, kDkFull, kTFree, kDone, kNumBars };
-constexpr int kSmem = kOffBars + kNumBars * 8 + 16 + 1024;
+constexpr int kOffP = kStages * kStageBytes, kOffDs = (kOffP + kPBytes + 1023) / 1024 * 1024;
+constexpr int kOffBars = kOffDs + kPBytes;
+constexpr int kMaskSlots = 4;  // mask steps built at once in the P buffer
+static_assert(kMaskSlots * kMaskOpBytes <= kPBytes, "mask operands fit the P buffer");
+enum { kFull = 0, kStaged = 2, kSMain = 4, kSRem, kPFull, kDvFull, kDsFull, kDqFull, kDkFull, kTFree, kInfo, kMaskMore,
+       kMaskEmpty, kDone, kNumBars };
+constexpr int kSmem = kOffBars + kNumBars * 8 + 64 + 1024;
 static_assert(kSmem <= 227 * 1024, "shared memory budget");
 constexpr uint32_t kColS = 0, kColP = 144, kColS2 = 288, kColDv = 432, kColRem = 496;
-constexpr uint32_t kColDk = kColP, kColDq = kColP + 64, kColDq2 = kColS2 + 128;
-constexpr uint32_t kRegsSmall = 104, kRegsMain = 200;
+constexpr uint32_t kColDq = kColS2, kColDk = kColS2 + 64, kColDq2 = kColS2 + 128;
+constexpr uint32_t kRegsSmall = 120, kRegsMain = 192;
 static_assert(4 * kRegsSmall + 8 * kRegsMain <= 12 * kRegsLaunch, "register split");
 constexpr uint32_t kIdescT = make_idesc(1, 128, 64, true, true);    // A and B MN-major: dV, dK
 constexpr uint32_t kIdescRemT = make_idesc(1, 64, 16, true, true);  // (64 dims) x (16 keys)
 constexpr uint32_t kIdescRemQ = make_idesc(1, 64, 16, true, false); // (64 dims) x (16 queries)
 
-struct Ctx {
-  uint32_t sbase, bar0, tmem;
-  uint8_t* smem;
-  volatile int* abort;
-  int t_begin, n_local;
-  __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8u * (uint32_t)i; }
-};
-
-// The head's bias gradient of this thread's 72 pairs.
-template <bool kRem>
-struct Grad {
-  float2 a[kRem ? 1 : 36];
-  uint32_t smem;
-  __device__ __forceinline__ void clear() {
-    if constexpr (kRem) {
-      for (int j = 0; j < 18; ++j) st_shared_v4(smem + j * 512, 0u, 0u, 0u, 0u);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 36; ++j) a[j] = make_float2(0.f, 0.f);
-    }
-  }
-  __device__ __forceinline__ void add(int j, float2 ga, float2 gb) {
-    if constexpr (kRem) {
-      uint32_t x, y, z, w;
-      ld_shared_v4(smem + j * 512, x, y, z, w);
-      const float2 sa = __fadd2_rn(f2(x, y), ga), sb = __fadd2_rn(f2(z, w), gb);
-      st_shared_v4(smem + j * 512, __float_as_uint(sa.x), __float_as_uint(sa.y), __float_as_uint(sb.x),
-                   __float_as_uint(sb.y));
-    } else {
-      a[2 * j] = __fadd2_rn(a[2 * j], ga);
-      a[2 * j + 1] = __fadd2_rn(a[2 * j + 1], gb);
-    }
-  }
-  __device__ __forceinline__ void flush(const Params& p, int h, const Lane& l) const {
-    if (!p.slots) return;
-    float* slot = p.slots + (int64_t)(blockIdx.x + h) * p.N * p.N;
-#pragma unroll
-    for (int j = 0; j < 18; ++j) {
-      float4 v;
-      if constexpr (kRem) {
-        uint32_t x, y, z, w;
-        ld_shared_v4(smem + j * 512, x, y, z, w);
-        v = make_float4(__uint_as_float(x), __uint_as_float(y), __uint_as_float(z), __uint_as_float(w));
-      } else {
-        v = make_float4(a[2 * j].x, a[2 * j].y, a[2 * j + 1].x, a[2 * j + 1].y);
-      }
-      const int key = 8 * j + 2 * l.t0;
-      if (l.ra < p.N) {
-        if (key < p.N) slot[l.ra * p.N + key] = v.x;
-        if (key + 1 < p.N) slot[l.ra * p.N + key + 1] = v.y;
-      }
-      if (l.rb < p.N) {
-        if (key < p.N) slot[l.rb * p.N + key] = v.z;
-        if (key + 1 < p.N) slot[l.rb * p.N + key + 1] = v.w;
-      }
-    }
-  }
-};
-
 // A transposed remainder block, (64 head dims) x (rows 128..143), of this warp's TMEM quarter: 16
 // head dims, scaled, into rows 128..143 of a staged bf16 tile.
-__device__ __forceinline__ void stage_rem(uint32_t taddr, uint32_t stg, int quarter, const Lane& l, float scale) {
+__device__ __forceinline__ void stage_rem(uint32_t taddr, uint32_t stg, int warp, int lane, float scale) {
+  const int quarter = warp & 3, t0 = lane & 3, t1 = lane >> 2;
   uint32_t r[8];
   tmem_ld_16x256b_r8(taddr + ((uint32_t)(32 * quarter) << 16), r);
   tmem_wait_ld();
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int row = 128 + 8 * (e >> 2) + 2 * l.t0 + (e & 1);
-    const int d = 16 * quarter + l.t1 + 8 * ((e >> 1) & 1);
+    const int row = 128 + 8 * (e >> 2) + 2 * t0 + (e & 1);
+    const int d = 16 * quarter + t1 + 8 * ((e >> 1) & 1);
     const __nv_bfloat16 v = __float2bfloat16_rn(__uint_as_float(r[e]) * scale);
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(stg + (uint32_t)(row * 128 + (((d >> 3) ^ (row & 7)) << 4) + (d & 7) * 2)),
                  "h"(__bfloat16_as_ushort(v))
@@ -693,166 +694,361 @@ __device__ __forceinline__ void stage_rem(uint32_t taddr, uint32_t stg, int quar
   }
 }
 
-template <bool kRem, int kMask>
-__device__ __forceinline__ void pass1(const Params& p, const Lane& l, const TileMask<kMask>& mask, const Bias<kRem>& bias,
-                                      uint32_t tS, uint32_t tP, uint32_t sP, float2 sta, float2 stb, float2& da2,
-                                      float2& db2) {
-  // Pass 1, 16 keys (two 8-key blocks) at a time, the next loads in flight.
-  const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
-  const float2 ma2 = make_float2(-sta.x, -sta.x), mb2 = make_float2(-stb.x, -stb.x);
-  const float2 na2 = make_float2(-sta.y, -sta.y), nb2 = make_float2(-stb.y, -stb.y);
-  uint32_t sv[8], gv[8];
-  tmem_ld_16x256b_r8(tS, sv);
-  tmem_ld_16x256b_r8(tP, gv);
-#pragma unroll
-  for (int q = 0; q < 9; ++q) {
+// The 16-column blocks of two accumulators in turn. Warps 4..11 keep the next block's loads in flight;
+// warps 2 and 3, with fewer registers and half the rows, do not.
+template <bool kRem>
+struct TmemBlocks {
+  uint32_t a, b;
+  uint32_t va[8], vb[8];
+  __device__ __forceinline__ TmemBlocks(uint32_t a_, uint32_t b_) : a(a_), b(b_) {
+    if constexpr (!kRem) load(0);
+  }
+  __device__ __forceinline__ void load(int q) {
+    tmem_ld_16x256b_r8(a + 16 * q, va);
+    tmem_ld_16x256b_r8(b + 16 * q, vb);
+  }
+  __device__ __forceinline__ void next(int q, uint32_t (&ca)[8], uint32_t (&cb)[8]) {
+    if constexpr (kRem) load(q);
     tmem_wait_ld();
-    uint32_t cs[8], cg[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      cs[e] = sv[e];
-      cg[e] = gv[e];
+      ca[e] = va[e];
+      cb[e] = vb[e];
     }
-    if (q < 8) {
-      tmem_ld_16x256b_r8(tS + 16 * (q + 1), sv);
-      tmem_ld_16x256b_r8(tP + 16 * (q + 1), gv);
+    if constexpr (!kRem) {
+      if (q < 8) load(q + 1);
     }
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const int j = 2 * q + (e >> 2);
-      const float4 b = bias.get(j);
-      float2 xa = __ffma2_rn(f2(cs[e], cs[e + 1]), c2, make_float2(b.x, b.y));
-      float2 xb = __ffma2_rn(f2(cs[e + 2], cs[e + 3]), c2, make_float2(b.z, b.w));
-      if (kMask != kNoMask) mask.apply(p, l, j, xa, xb);
-      xa = __fadd2_rn(__fadd2_rn(xa, ma2), na2);
-      xb = __fadd2_rn(__fadd2_rn(xb, mb2), nb2);
-      const float2 ea = make_float2(ex2(xa.x), ex2(xa.y)), eb = make_float2(ex2(xb.x), ex2(xb.y));
-      da2 = __ffma2_rn(ea, f2(cg[e], cg[e + 1]), da2);
-      db2 = __ffma2_rn(eb, f2(cg[e + 2], cg[e + 3]), db2);
-      store_p(sP, l, j, pack_bf16x2(ea.x, ea.y), pack_bf16x2(eb.x, eb.y));
-      cs[e] = __float_as_uint(ea.x);
-      cs[e + 1] = __float_as_uint(ea.y);
-      cs[e + 2] = __float_as_uint(eb.x);
-      cs[e + 3] = __float_as_uint(eb.y);
-    }
-    tmem_st_16x256b_r8(tS + 16 * q, cs);
   }
-}
+};
 
 template <bool kRem, int kMask>
 __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int warp, int lane) {
-  const Lane l = make_lane(warp, lane);
+  const Lane<kRem> l(warp, lane);
+  constexpr int R = Lane<kRem>::kRows;
   const uint32_t tS = c.tmem + l.addr + (kRem ? kColS2 : kColS);
   const uint32_t tP = c.tmem + l.addr + (kRem ? kColS2 + kLaneHalf : kColP);
-  const uint32_t sP = c.sbase + kOffP;
+  const uint32_t sP = c.sbase + kOffP, sDs = c.sbase + kOffDs;
+  const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
   Bias<kRem> bias;
-  bias.smem = c.sbase + kOffRem + lane * 16;
-  Grad<kRem> grad;
-  grad.smem = c.sbase + kOffRemAcc + lane * 16;
+  float2 grad[18][R];  // the head's bias gradient of this thread's pairs
   int cur_h = -1;
+  auto flush = [&](int h) {
+    if (!p.slots) return;
+    float* slot = p.slots + (int64_t)(blockIdx.x + h) * p.N * p.N;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (l.row[r] >= p.N) continue;
+      float* dst = slot + l.row[r] * p.N + 2 * l.t0;
+#pragma unroll
+      for (int j = 0; j < 18; ++j) {
+        if (8 * j + 2 * l.t0 < p.N) dst[8 * j] = grad[j][r].x;
+        if (8 * j + 2 * l.t0 + 1 < p.N) dst[8 * j + 1] = grad[j][r].y;
+      }
+    }
+  };
   for (int i = 0; i < c.n_local; ++i) {
     const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i & 1;
     const uint32_t par = (uint32_t)(i & 1);
     const uint32_t slot = c.sbase + s * kStageBytes;
     if (h != cur_h) {
-      if (cur_h >= 0) grad.flush(p, cur_h, l);
+      if (cur_h >= 0) flush(cur_h);
       cur_h = h;
-      grad.clear();
+#pragma unroll
+      for (int j = 0; j < 18; ++j)
+#pragma unroll
+        for (int r = 0; r < R; ++r) grad[j][r] = make_float2(0.f, 0.f);
       bias.fetch(p, h, l, lane);
     }
     // Row statistics; +inf past N makes the rows' P zero.
+    float2 mx[R], lg[R], d2[R];
     const float2* st = p.stats + ((int64_t)w * p.H + h) * p.N;
-    const float2 pad = make_float2(INFINITY, 0.f);
-    const float2 sta = l.ra < p.N ? __ldg(st + l.ra) : pad, stb = l.rb < p.N ? __ldg(st + l.rb) : pad;
-    TileMask<kMask> mask;
-    if (!warp_wait(c.bar(kSFull), par, c.abort, p.status, 121)) return;
-    if constexpr (kMask == kGroups) {  // the ids came with the tile's loads, long complete
-      if (!warp_wait(c.bar(kFull + s), (uint32_t)((i >> 1) & 1), c.abort, p.status, 122)) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float2 v = l.row[r] < p.N ? __ldg(st + l.row[r]) : make_float2(INFINITY, 0.f);
+      mx[r] = make_float2(-v.x, -v.x);
+      lg[r] = make_float2(-v.y, -v.y);
+      d2[r] = make_float2(0.f, 0.f);
     }
-    mask.begin(p, l, w, c.smem + kOffIds + s * kIdBytes);
+    ByteMask<kRem> mask;
+    if constexpr (kMask == kMaskU8) mask.begin(p, l, w);
+    if (!warp_wait(c.bar(kRem ? kSRem : kSMain), par, c.abort, p.status, 121)) return;
     tc_fence_after();
-    float2 da2 = make_float2(0.f, 0.f), db2 = make_float2(0.f, 0.f);
-    // One branch for the tile, not one per block: see the forward kernel.
-    if (kMask != kNoMask && mask.on)
-      pass1<kRem, kMask>(p, l, mask, bias, tS, tP, sP, sta, stb, da2, db2);
-    else
-      pass1<kRem, kNoMask>(p, l, TileMask<kNoMask>(), bias, tS, tP, sP, sta, stb, da2, db2);
-    tmem_wait_st();
-    fence_proxy_async_shared();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(c.bar(kPFull));
-    float da = da2.x + da2.y, db = db2.x + db2.y;
-    da += __shfl_xor_sync(0xffffffffu, da, 1);
-    da += __shfl_xor_sync(0xffffffffu, da, 2);
-    db += __shfl_xor_sync(0xffffffffu, db, 1);
-    db += __shfl_xor_sync(0xffffffffu, db, 2);
-    const float2 ea2 = make_float2(-da, -da), eb2 = make_float2(-db, -db);
-    uint32_t sv[8], gv[8];
-    tmem_ld_16x256b_r8(tS, sv);
-    tmem_ld_16x256b_r8(tP, gv);
-    if (!warp_wait(c.bar(kDvFull), par, c.abort, p.status, 123)) {
-      tmem_wait_ld();
-      return;
-    }
-    // Pass 2: dS over P in shared memory.
+    // Pass 1, 16 keys (two 8-key blocks) at a time, the next loads in flight.
+    TmemBlocks<kRem> blk(tS, tP);
 #pragma unroll
     for (int q = 0; q < 9; ++q) {
-      tmem_wait_ld();
       uint32_t cs[8], cg[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        cs[e] = sv[e];
-        cg[e] = gv[e];
-      }
-      if (q < 8) {
-        tmem_ld_16x256b_r8(tS + 16 * (q + 1), sv);
-        tmem_ld_16x256b_r8(tP + 16 * (q + 1), gv);
-      }
+      blk.next(q, cs, cg);
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {
         const int j = 2 * q + (e >> 2);
-        const float2 ga = __fmul2_rn(f2(cs[e], cs[e + 1]), __fadd2_rn(f2(cg[e], cg[e + 1]), ea2));
-        const float2 gb = __fmul2_rn(f2(cs[e + 2], cs[e + 3]), __fadd2_rn(f2(cg[e + 2], cg[e + 3]), eb2));
-        grad.add(j, ga, gb);
-        store_p(sP, l, j, pack_bf16x2(ga.x, ga.y), pack_bf16x2(gb.x, gb.y));
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float2 x = __ffma2_rn(l.pick(&cs[e], r), c2, bias.b[j][r]);
+          if constexpr (kMask == kMaskU8) mask.apply(p, l, j, r, x);
+          x = __fadd2_rn(__fadd2_rn(x, mx[r]), lg[r]);
+          const float2 pr = make_float2(ex2(x.x), ex2(x.y));
+          d2[r] = __ffma2_rn(pr, l.pick(&cg[e], r), d2[r]);
+          l.store_p(sP, j, r, pack_bf16x2(pr.x, pr.y));
+          cs[e + 2 * r] = __float_as_uint(pr.x);
+          cs[e + 2 * r + 1] = __float_as_uint(pr.y);
+          if constexpr (kRem) {  // the lanes' other row is nobody's
+            cs[e + 2] = cs[e];
+            cs[e + 3] = cs[e + 1];
+          }
+        }
+      }
+      tmem_st_16x256b_r8(tS + 16 * q, cs);
+    }
+    tmem_wait_st();
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(c.bar(kPFull));
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float d = d2[r].x + d2[r].y;
+      d += __shfl_xor_sync(0xffffffffu, d, 1);
+      d += __shfl_xor_sync(0xffffffffu, d, 2);
+      d2[r] = make_float2(-d, -d);
+    }
+    // Pass 2.
+    TmemBlocks<kRem> blk2(tS, tP);
+#pragma unroll
+    for (int q = 0; q < 9; ++q) {
+      uint32_t cs[8], cg[8];
+      blk2.next(q, cs, cg);
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const int j = 2 * q + (e >> 2);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float2 g = __fmul2_rn(l.pick(&cs[e], r), __fadd2_rn(l.pick(&cg[e], r), d2[r]));
+          grad[j][r] = __fadd2_rn(grad[j][r], g);
+          l.store_p(sDs, j, r, pack_bf16x2(g.x, g.y));
+        }
       }
     }
     fence_proxy_async_shared();
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bar(kDsFull));
-    // dV while the dK and dQ products run, then those.
-    const int quarter = warp & 3;
-    uint32_t o[32];
     if constexpr (!kRem) {
-      tc_fence_after();
-      tmem_ld_16x256b_r32(c.tmem + l.addr + kColDv, o);
-      tmem_wait_ld();
-      stage_rows(slot + kOffV, l, o, 1.f, 1.f);
-      if (warp < 8) stage_rem(c.tmem + kColRem, slot + kOffV, quarter, l, 1.f);
-    }
-    if (!warp_wait(c.bar(kDkFull), par, c.abort, p.status, 124)) return;
-    if constexpr (!kRem) {
-      tc_fence_after();
-      tmem_ld_16x256b_r32(c.tmem + l.addr + kColDk, o);
-      tmem_wait_ld();
-      stage_rows(slot + kOffK, l, o, p.scale, p.scale);
-      tmem_ld_16x256b_r32(c.tmem + l.addr + kColDq, o);
-      tmem_wait_ld();
-      stage_rows(slot + kOffQ, l, o, p.scale, p.scale);
-      if (warp < 8) stage_rem(c.tmem + kColDq2, slot + kOffQ, quarter, l, p.scale);
-      else stage_rem(c.tmem + kColRem + kLaneHalf, slot + kOffK, quarter, l, p.scale);
+      uint32_t o[32];
+      auto drain = [&](int bar, int code, uint32_t col, uint32_t stg, float scale) -> bool {
+        if (!warp_wait(c.bar(bar), par, c.abort, p.status, code)) return false;
+        tc_fence_after();
+        tmem_ld_16x256b_r32(c.tmem + l.addr + col, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int r = 0; r < R; ++r) l.stage(stg, o, r, scale);
+        return true;
+      };
+      if (!drain(kDvFull, 122, kColDv, slot + kOffV, 1.f)) return;
+      if (warp < 8) stage_rem(c.tmem + kColRem, slot + kOffV, warp, lane, 1.f);
+      if (!drain(kDqFull, 123, kColDq, slot + kOffG, p.scale)) return;
+      if (warp >= 8) stage_rem(c.tmem + kColDq2, slot + kOffG, warp, lane, p.scale);
+      if (!drain(kDkFull, 124, kColDk, slot + kOffK, p.scale)) return;
+      if (warp < 8) stage_rem(c.tmem + kColRem + kLaneHalf, slot + kOffK, warp, lane, p.scale);
       fence_proxy_async_shared();
-    }
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) {
-      mbar_arrive(c.bar(kTFree));
-      mbar_arrive(c.bar(kStaged + s));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(c.bar(kTFree));
+        mbar_arrive(c.bar(kStaged + s));
+      }
     }
   }
-  if (cur_h >= 0) grad.flush(p, cur_h, l);
+  if (cur_h >= 0) flush(cur_h);
+}
+
+template <int kMask>
+__device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane, const CUtensorMap* tmq,
+                                         const CUtensorMap* tmk, const CUtensorMap* tmv, const CUtensorMap* tmg,
+                                         const CUtensorMap* tmdq, const CUtensorMap* tmdk, const CUtensorMap* tmdv) {
+  const int n = c.n_local;
+  int issued = 0, more = 0;
+  auto load = [&](int i) {
+    const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin;
+    const uint32_t bar = c.bar(kFull + (i & 1)), slot = c.sbase + (i & 1) * kStageBytes;
+    mbar_arrive_expect_tx(bar, kStageBytes);
+    tma_load_4d(slot + kOffQ, tmq, bar, 0, 0, h, w);
+    tma_load_4d(slot + kOffK, tmk, bar, 0, 0, h, w);
+    tma_load_4d(slot + kOffG, tmg, bar, 0, 0, h, w);
+    tma_load_4d(slot + kOffV, tmv, bar, 0, 0, h, w);
+    ++issued;
+  };
+  auto store = [&](int j) {
+    const int t = c.t_begin + j, h = t / p.Bwin, w = t - h * p.Bwin;
+    const uint32_t slot = c.sbase + (j & 1) * kStageBytes;
+    tma_store_4d(tmdq, slot + kOffG, 0, 0, h, w);
+    tma_store_4d(tmdk, slot + kOffK, 0, 0, h, w);
+    tma_store_4d(tmdv, slot + kOffV, 0, 0, h, w);
+    bulk_commit_group();
+  };
+  if (lane == 0) {
+    for (int i = 0; i < kStages && i < n; ++i) load(i);
+  }
+  Regions now, next;
+  if constexpr (kMask == kGroups) {
+    if (n > 0) next.load(p, c.t_begin % p.Bwin, lane);
+  }
+  for (int i = 0; i < n; ++i) {
+    int ok = 1;
+    if constexpr (kMask == kGroups) {
+      now = next;
+      if (i + 1 < n) next.load(p, (c.t_begin + i + 1) % p.Bwin, lane);
+      now.classify();
+      // The P buffer is free once dV of the tile before is done.
+      if (i > 0 && !warp_wait(c.bar(kDvFull), (uint32_t)((i - 1) & 1), c.abort, p.status, 133)) break;
+      for (int st = 0; st < now.steps && ok; ++st) {
+        if (st > 0 && st % kMaskSlots == 0) {  // more than 64 regions: wait until the slots have been read
+          if (lane == 0) {
+            if (st == kMaskSlots) {
+              c.steps[i & 1] = now.steps;
+              mbar_arrive(c.bar(kInfo));
+            } else {
+              mbar_arrive(c.bar(kMaskMore));
+            }
+          }
+          ok = warp_wait(c.bar(kMaskEmpty), (uint32_t)(more & 1), c.abort, p.status, 134);
+          ++more;
+        }
+        if (ok) now.build(c.sbase + kOffP + (st % kMaskSlots) * kMaskOpBytes, st, lane, p.mask_a, p.mask_b);
+      }
+      if (!ok) break;
+      if (lane == 0) {
+        if (now.steps <= kMaskSlots) {
+          c.steps[i & 1] = now.steps;
+          mbar_arrive(c.bar(kInfo));
+        } else {
+          mbar_arrive(c.bar(kMaskMore));
+        }
+      }
+    }
+    if (i > 0 && i + 1 < n) {
+      // Tile i - 1's outputs leave its slot, tile i + 1's inputs enter it.
+      if (lane == 0) {
+        ok = mbar_wait(c.bar(kStaged + ((i - 1) & 1)), (uint32_t)(((i - 1) >> 1) & 1), c.abort, p.status, 125, kTimeoutNs);
+        if (ok) {
+          store(i - 1);
+          bulk_wait_group_read0();
+          load(i + 1);
+        }
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+    }
+  }
+  if (lane == 0) {
+    // Never leave with copies in flight (bounded, also after an abort).
+    int no_abort = 0;
+    for (int j = issued > kStages ? issued - kStages : 0; j < issued; ++j)
+      mbar_wait(c.bar(kFull + (j & 1)), (uint32_t)((j >> 1) & 1), &no_abort, p.status, 126, kTimeoutNs);
+    for (int j = n > kStages ? n - kStages : 0; j < n; ++j) {
+      if (!mbar_wait(c.bar(kStaged + (j & 1)), (uint32_t)((j >> 1) & 1), c.abort, p.status, 127, kTimeoutNs)) break;
+      store(j);
+    }
+    bulk_wait_group0();
+  }
+}
+
+template <int kMask>
+__device__ __forceinline__ void issuer(const Params& p, const Ctx& c) {
+  const bool leader = elect_one();
+  const uint32_t sP = c.sbase + kOffP, sDs = c.sbase + kOffDs;
+  // K-major (row) and MN-major (column) views of the input tiles, P and dS; 32-byte-swizzled parts.
+  const uint64_t row0 = desc_sw128(c.sbase, 16, 1024), col0 = desc_sw128(c.sbase, kTileBytes, 1024);
+  const uint64_t pT = desc_sw128(sP, kPChunk, 1024), p32 = desc_sw32(sP + 2 * kPChunk, 256);
+  const uint64_t dsT = desc_sw128(sDs, kPChunk, 1024), ds = desc_sw128(sDs, 16, 1024);
+  const uint64_t ds32 = desc_sw32(sDs + 2 * kPChunk, 256), mask0 = desc_sw32(sP, 256);
+  int more = 0;
+  for (int i = 0; i < c.n_local; ++i) {
+    const int s = i & 1;
+    const uint32_t par = (uint32_t)(i & 1), slot = s * kStageBytes;
+    const uint64_t qr = at(row0, slot + kOffQ), kr = at(row0, slot + kOffK), vr = at(row0, slot + kOffV),
+                   gr = at(row0, slot + kOffG);
+    const uint64_t qc = at(col0, slot + kOffQ), kc = at(col0, slot + kOffK), gc = at(col0, slot + kOffG);
+    // S and dP of rows 0..127 as soon as the inputs are there (their columns are free: pass 2 of the
+    // tile before is done); the M=64 blocks once dQ and dK have been drained. A masked tile issues
+    // both together: its mask operands are overwritten by P.
+    if (!warp_wait(c.bar(kFull + s), (uint32_t)((i >> 1) & 1), c.abort, p.status, 128)) break;
+    int steps = 0;
+    if constexpr (kMask == kGroups) {
+      if (!warp_wait(c.bar(kInfo), par, c.abort, p.status, 135)) break;
+      steps = c.steps[i & 1];
+      if (steps > 0 && !warp_wait(c.bar(kTFree), par ^ 1u, c.abort, p.status, 129)) break;
+    }
+    tc_fence_after();
+    if (leader) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) umma_f16(c.tmem + kColS, at(qr, e * 32), at(kr, e * 32), kIdescS, e > 0 ? 1u : 0u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) umma_f16(c.tmem + kColP, at(gr, e * 32), at(vr, e * 32), kIdescS, e > 0 ? 1u : 0u);
+      if (steps == 0) umma_commit(c.bar(kSMain));
+    }
+    if (steps == 0 && !warp_wait(c.bar(kTFree), par ^ 1u, c.abort, p.status, 129)) break;
+    tc_fence_after();
+    if (leader) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        umma_f16(c.tmem + kColS2, at(qr, kRemOff + e * 32), at(kr, e * 32), kIdescS2, e > 0 ? 1u : 0u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        umma_f16(c.tmem + kColS2 + kLaneHalf, at(gr, kRemOff + e * 32), at(vr, e * 32), kIdescS2, e > 0 ? 1u : 0u);
+    }
+    if constexpr (kMask == kGroups) {
+      bool ok = true;
+      for (int st = 0; st < steps; ++st) {
+        if (st > 0 && st % kMaskSlots == 0) {
+          if (leader) umma_commit(c.bar(kMaskEmpty));
+          ok = warp_wait(c.bar(kMaskMore), (uint32_t)(more & 1), c.abort, p.status, 136);
+          ++more;
+          if (!ok) break;
+          tc_fence_after();
+        }
+        if (leader) {
+          const uint64_t a = at(mask0, (st % kMaskSlots) * kMaskOpBytes), b = at(a, kRow32);
+          umma_f16(c.tmem + kColS, a, b, kIdescS, 1u);
+          umma_f16(c.tmem + kColS2, at(a, kRemOff32), b, kIdescS2, 1u);
+        }
+      }
+      if (!ok) break;
+    }
+    if (leader) {
+      if (steps > 0) umma_commit(c.bar(kSMain));
+      umma_commit(c.bar(kSRem));
+    }
+    if (!warp_wait(c.bar(kPFull), par, c.abort, p.status, 130)) break;
+    tc_fence_after();
+    if (leader) {
+#pragma unroll
+      for (int e = 0; e < 9; ++e) {  // queries 16e .. 16e + 15
+        umma_f16(c.tmem + kColDv, at(pT, e * 2048), at(gc, e * 2048), kIdescT, e > 0 ? 1u : 0u);
+        umma_f16(c.tmem + kColRem, at(gc, e * 2048), at(p32, e * 512), kIdescRemT, e > 0 ? 1u : 0u);
+      }
+      umma_commit(c.bar(kDvFull));
+    }
+    if (!warp_wait(c.bar(kDsFull), par, c.abort, p.status, 131)) break;
+    tc_fence_after();
+    if (leader) {
+#pragma unroll
+      for (int e = 0; e < 9; ++e) {  // keys 16e .. 16e + 15
+        const uint64_t a = e < 8 ? at(ds, (e >> 2) * kPChunk + (e & 3) * 32) : ds32;
+        umma_f16(c.tmem + kColDq, a, at(kc, e * 2048), kIdescO, e > 0 ? 1u : 0u);
+        umma_f16(c.tmem + kColDq2, at(kc, e * 2048), at(a, e < 8 ? 128 * 128 : 128 * 32), kIdescRemQ, e > 0 ? 1u : 0u);
+      }
+      umma_commit(c.bar(kDqFull));
+#pragma unroll
+      for (int e = 0; e < 9; ++e) {
+        umma_f16(c.tmem + kColDk, at(dsT, e * 2048), at(qc, e * 2048), kIdescT, e > 0 ? 1u : 0u);
+        umma_f16(c.tmem + kColRem + kLaneHalf, at(qc, e * 2048), at(ds32, e * 512), kIdescRemT, e > 0 ? 1u : 0u);
+      }
+      umma_commit(c.bar(kDkFull));
+    }
+  }
+  if (leader) umma_commit(c.bar(kDone));
+  int no_abort = 0;
+  mbar_wait(c.bar(kDone), 0, &no_abort, p.status, 132, kTimeoutNs);
+  __syncwarp();
 }
 
 template <int kMask>
@@ -864,143 +1060,40 @@ rel_bias_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kNumBars);
-  __shared__ int abort_flag;
+  int* words = reinterpret_cast<int*>(bars + kNumBars);  // abort flag, TMEM address, mask steps
   Ctx c;
-  c.smem = smem;
   c.sbase = smem_u32(smem);
   c.bar0 = smem_u32(bars);
-  c.abort = &abort_flag;
+  c.abort = words;
+  c.steps = words + 4;
   c.t_begin = tile_begin(p.num_tiles);
   c.n_local = tile_end(p.num_tiles) - c.t_begin;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    *words = 0;
     for (int b = 0; b < kNumBars; ++b) {
-      const bool nine = b == kStaged || b == kStaged + 1 || b == kPFull || b == kDsFull || b == kTFree;
-      mbar_init(c.bar(b), nine ? 9 : 1);
+      const bool main = b == kStaged || b == kStaged + 1 || b == kTFree, all = b == kPFull || b == kDsFull;
+      mbar_init(c.bar(b), main ? 8 : all ? 10 : 1);
     }
     fence_mbarrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_holder), kTmemCols);
+    tmem_alloc(smem_u32(words + 1), kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  c.tmem = *tmem_holder;
-  const int n = c.n_local;
+  c.tmem = (uint32_t)*reinterpret_cast<volatile int*>(words + 1);
 
   if (warp >= 4) {
     warpgroup_reg_alloc<kRegsMain>();
     softmax_warps<false, kMask>(p, c, warp, lane);
   } else {
     warpgroup_reg_dealloc<kRegsSmall>();
-    if (warp == 3) {
-      softmax_warps<true, kMask>(p, c, warp, lane);
-    } else if (warp == 0) {
-      // Loads, and the stores of finished tiles.
-      int last_par[kStages] = {-1, -1};
-      auto store_out = [&](int j) {
-        const int t = c.t_begin + j, h = t / p.Bwin, w = t - h * p.Bwin;
-        const uint32_t slot = c.sbase + (j & 1) * kStageBytes;
-        tma_store_4d(&tmdq, slot + kOffQ, 0, 0, h, w);
-        tma_store_4d(&tmdk, slot + kOffK, 0, 0, h, w);
-        tma_store_4d(&tmdv, slot + kOffV, 0, 0, h, w);
-        bulk_commit_group();
-      };
-      for (int i = 0; i < n; ++i) {
-        const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i & 1;
-        uint32_t id[5];
-        if constexpr (kMask == kGroups) load_ids(p, w, lane, id);
-        int ok = 1;
-        if (lane == 0 && i >= kStages) {
-          ok = mbar_wait(c.bar(kStaged + s), (uint32_t)(((i - kStages) >> 1) & 1), c.abort, p.status, 125, kTimeoutNs);
-          if (ok) {
-            store_out(i - kStages);
-            bulk_wait_group_read0();
-          }
-        }
-        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        if constexpr (kMask == kGroups) store_ids(smem + kOffIds + s * kIdBytes, lane, id);
-        if (lane == 0) {
-          const uint32_t bar = c.bar(kFull + s), slot = c.sbase + s * kStageBytes;
-          mbar_arrive_expect_tx(bar, kStageBytes);
-          tma_load_4d(slot + kOffQ, &tmq, bar, 0, 0, h, w);
-          tma_load_4d(slot + kOffK, &tmk, bar, 0, 0, h, w);
-          tma_load_4d(slot + kOffV, &tmv, bar, 0, 0, h, w);
-          tma_load_4d(slot + kOffG, &tmg, bar, 0, 0, h, w);
-          last_par[s] = (i >> 1) & 1;
-        }
-      }
-      if (lane == 0) {
-        // Never leave with copies in flight (bounded, also after an abort).
-        int no_abort = 0;
-        for (int s = 0; s < kStages; ++s)
-          if (last_par[s] >= 0) mbar_wait(c.bar(kFull + s), (uint32_t)last_par[s], &no_abort, p.status, 126, kTimeoutNs);
-        for (int j = n > kStages ? n - kStages : 0; j < n; ++j) {
-          if (!mbar_wait(c.bar(kStaged + (j & 1)), (uint32_t)((j >> 1) & 1), c.abort, p.status, 127, kTimeoutNs)) break;
-          store_out(j);
-        }
-        bulk_wait_group0();
-      }
-    } else if (warp == 1 && lane == 0) {
-      const uint32_t sP = c.sbase + kOffP;
-      for (int i = 0; i < n; ++i) {
-        const int s = i & 1;
-        const uint32_t par = (uint32_t)(i & 1);
-        const uint32_t slot = c.sbase + s * kStageBytes;
-        const uint32_t sQ = slot + kOffQ, sK = slot + kOffK, sV = slot + kOffV, sG = slot + kOffG;
-        if (!mbar_wait(c.bar(kFull + s), (uint32_t)((i >> 1) & 1), c.abort, p.status, 128, kTimeoutNs)) break;
-        if (!mbar_wait(c.bar(kTFree), par ^ 1u, c.abort, p.status, 129, kTimeoutNs)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint64_t b = desc_sw128(sK + k * 32, 16, 1024);
-          umma_f16(c.tmem + kColS, desc_sw128(sQ + k * 32, 16, 1024), b, kIdescS, k > 0 ? 1u : 0u);
-          umma_f16(c.tmem + kColS2, desc_sw128(sQ + kRowOff80 + k * 32, 16, 1024), b, kIdescS2, k > 0 ? 1u : 0u);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint64_t b = desc_sw128(sV + k * 32, 16, 1024);
-          umma_f16(c.tmem + kColP, desc_sw128(sG + k * 32, 16, 1024), b, kIdescS, k > 0 ? 1u : 0u);
-          umma_f16(c.tmem + kColS2 + kLaneHalf, desc_sw128(sG + kRowOff80 + k * 32, 16, 1024), b, kIdescS2,
-                   k > 0 ? 1u : 0u);
-        }
-        umma_commit(c.bar(kSFull));
-        if (!mbar_wait(c.bar(kPFull), par, c.abort, p.status, 130, kTimeoutNs)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < 9; ++k) {  // queries 16k .. 16k + 15
-          const uint64_t g = desc_sw128(sG + k * 2048, kTileBytes, 1024);
-          umma_f16(c.tmem + kColDv, desc_sw128(sP + k * 2048, kPChunk, 1024), g, kIdescT, k > 0 ? 1u : 0u);
-          umma_f16(c.tmem + kColRem, g, desc_sw32(sP + 2 * kPChunk + k * 512, 256), kIdescRemT, k > 0 ? 1u : 0u);
-        }
-        umma_commit(c.bar(kDvFull));
-        if (!mbar_wait(c.bar(kDsFull), par, c.abort, p.status, 131, kTimeoutNs)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < 9; ++k) {
-          const uint64_t q = desc_sw128(sQ + k * 2048, kTileBytes, 1024);
-          umma_f16(c.tmem + kColDk, desc_sw128(sP + k * 2048, kPChunk, 1024), q, kIdescT, k > 0 ? 1u : 0u);
-          umma_f16(c.tmem + kColRem + kLaneHalf, q, desc_sw32(sP + 2 * kPChunk + k * 512, 256), kIdescRemT,
-                   k > 0 ? 1u : 0u);
-        }
-#pragma unroll
-        for (int k = 0; k < 9; ++k) {  // keys 16k .. 16k + 15
-          const uint64_t kd = desc_sw128(sK + k * 2048, kTileBytes, 1024);
-          const uint32_t pa = k < 8 ? sP + (k >> 2) * kPChunk + (k & 3) * 32 : sP + 2 * kPChunk;
-          umma_f16(c.tmem + kColDq, k < 8 ? desc_sw128(pa, 16, 1024) : desc_sw32(pa, 256), kd, kIdescO, k > 0 ? 1u : 0u);
-          umma_f16(c.tmem + kColDq2, kd, k < 8 ? desc_sw128(pa + 128 * 128, 16, 1024) : desc_sw32(pa + 128 * 32, 256),
-                   kIdescRemQ, k > 0 ? 1u : 0u);
-        }
-        umma_commit(c.bar(kDkFull));
-      }
-      umma_commit(c.bar(kDone));
-      int no_abort = 0;
-      mbar_wait(c.bar(kDone), 0, &no_abort, p.status, 132, kTimeoutNs);
-    }
+    if (warp >= 2) softmax_warps<true, kMask>(p, c, warp, lane);
+    else if (warp == 1) issuer<kMask>(p, c);
+    else producer<kMask>(p, c, lane, &tmq, &tmk, &tmv, &tmg, &tmdq, &tmdk, &tmdv);
   }
   tc_fence_before();
   __syncthreads();
