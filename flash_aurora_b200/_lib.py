@@ -27,7 +27,6 @@ FA_STATUS_REGIONS_BROKEN, FA_STATUS_WATCHDOG_SELFTEST = 28, 90
 FA_ROWS_TOKENS, FA_ROWS_WINDOWS = 0, 1
 FA_NORM_BEFORE, FA_NORM_AFTER, FA_NORM_BETWEEN = 0, 1, 2
 FA_NORM_LAYER, FA_NORM_RMS = 0, 1
-FA_REL_BIAS_FLOATS = 20736
 
 _i64, _i32, _f32, _vp = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p
 _u32 = ctypes.c_uint
@@ -69,6 +68,7 @@ SIGNATURES = {
                                              _u32, _vp]),
     "fa_window_attention_bias_noalloc": (_i32, [_i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64p, _vp,
                                                  _i64, _f32, _vp]),
+    "fa_window_attention_rel_bias_state": (_i64, [_i64, _i64]),
     "fa_window_attention_rel_bias_workspace": (_i64, [_i64, _i64, _i64]),
     "fa_window_attention_rel_bias": (_i32, [_i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64p, _vp, _i32, _vp,
                                             _u8p, _u8p, _i64, _f32, _vp, _vp, _vp]),

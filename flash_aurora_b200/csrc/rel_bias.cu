@@ -39,22 +39,53 @@ __device__ __forceinline__ float bias_log2(const void* table, int bf16, const in
   return isinf(x) && !isinf(b) ? copysignf(3.4028234e38f, b) : x;
 }
 
-// Every head's bias in fragment order (see bias_rows), one float4 per thread. The gathers hit L1
-// here; in the attention kernels, whose shared memory leaves no L1, they cost a block 30 us a head.
+// What the attention kernels read beside their tensors: every head's bias in fragment order (see
+// bias_rows), one float4 per thread of the first blocks, and with region ids the rank of every token's id
+// among the ids of its window, one warp per window of the others. The gathers hit L1 here; in the
+// attention kernels, whose shared memory leaves no L1, they cost a block 30 us a head.
 constexpr int kExpandThreads = 192;
+constexpr int kExpandBlocks = kBiasVecs / kExpandThreads;  // per head
+static_assert(kBiasVecs % kExpandThreads == 0, "whole blocks");
+
+__device__ __forceinline__ void rank_window(const uint8_t* ids, int N, int lane, uint8_t* out) {
+  uint32_t id[5];
+  int rank[5];
+#pragma unroll
+  for (int m = 0; m < 5; ++m) {
+    id[m] = lane + 32 * m < N ? (uint32_t)__ldg(ids + lane + 32 * m) : 256u;
+    rank[m] = 0;
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 8; ++k) {  // ids 32 k .. 32 k + 31
+    uint32_t bits = 0;
+#pragma unroll
+    for (int m = 0; m < 5; ++m) bits |= (id[m] >> 5) == k ? 1u << (id[m] & 31) : 0u;
+    bits = __reduce_or_sync(0xffffffffu, bits);
+#pragma unroll
+    for (int m = 0; m < 5; ++m)
+      rank[m] += (id[m] >> 5) > k ? __popc(bits) : (id[m] >> 5) == k ? __popc(bits & ((1u << (id[m] & 31)) - 1u)) : 0;
+  }
+#pragma unroll
+  for (int m = 0; m < 5; ++m)
+    if (lane + 32 * m < kMaxN) out[lane + 32 * m] = (uint8_t)(id[m] < 256u ? rank[m] : kNoRank);
+}
+
 __global__ void __launch_bounds__(kExpandThreads)
-expand_bias_kernel(const void* table, int bf16, const int32_t* index, int H, int N, float4* out) {
-  const int e = blockIdx.x * kExpandThreads + threadIdx.x;
+expand_bias_kernel(const void* table, int bf16, const int32_t* index, int H, int N, float4* out, const uint8_t* ids,
+                   int64_t nW, uint8_t* ranks) {
+  if ((int64_t)blockIdx.x >= (int64_t)H * kExpandBlocks) {
+    const int64_t w = ((int64_t)blockIdx.x - (int64_t)H * kExpandBlocks) * (kExpandThreads / 32) + (threadIdx.x >> 5);
+    if (w < nW) rank_window(ids + w * N, N, threadIdx.x & 31, ranks + w * kMaxN);
+    return;
+  }
+  const int h = blockIdx.x / kExpandBlocks, e = (blockIdx.x % kExpandBlocks) * kExpandThreads + threadIdx.x;
   const int lane = e & 31, j = (e >> 5) % 18, blk = (e >> 5) / 18;
   const int i = 16 * blk + (lane >> 2), k = 8 * j + 2 * (lane & 3);
-  for (int h = blockIdx.y; h < H; h += gridDim.y) {
-    out[(int64_t)h * kBiasVecs + e] = make_float4(bias_log2(table, bf16, index, H, N, h, i, k),
-                                                  bias_log2(table, bf16, index, H, N, h, i, k + 1),
-                                                  bias_log2(table, bf16, index, H, N, h, i + 8, k),
-                                                  bias_log2(table, bf16, index, H, N, h, i + 8, k + 1));
-  }
+  out[(int64_t)h * kBiasVecs + e] = make_float4(bias_log2(table, bf16, index, H, N, h, i, k),
+                                                bias_log2(table, bf16, index, H, N, h, i, k + 1),
+                                                bias_log2(table, bf16, index, H, N, h, i + 8, k),
+                                                bias_log2(table, bf16, index, H, N, h, i + 8, k + 1));
 }
-static_assert(kBiasVecs % kExpandThreads == 0, "whole blocks");
 
 __device__ __forceinline__ float bias_at(const Params& p, int h, int i, int j) {
   const int lane = ((i & 7) << 2) | ((j & 7) >> 1);
@@ -240,7 +271,7 @@ int grid_of(int64_t tiles) { return (int)(tiles < num_sms() ? tiles : num_sms())
 
 // Checks shared by both directions; strides are {window, head, token} triples.
 int check_args(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, const void* const* ptrs, int n_ptrs,
-               const int64_t* strides, const float* bias, bool u8, bool ids, int64_t nW, float scale) {
+               const int64_t* strides, const void* state, bool u8, bool ids, int64_t nW, float scale) {
   FA_REQUIRE(precision == FA_ATTN_BF16 || precision == FA_ATTN_FP32_3XTF32, FA_ERR_INVALID,
              "precision must be FA_ATTN_BF16 or FA_ATTN_FP32_3XTF32");
   FA_REQUIRE(strides, FA_ERR_INVALID, "null stride pointer");
@@ -255,7 +286,7 @@ int check_args(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, co
   FA_REQUIRE(Bwin < ((int64_t)1 << 31) && H < ((int64_t)1 << 31) && Bwin * H < ((int64_t)1 << 31), FA_ERR_INVALID,
              "too many (window, head) tiles");
   if (Bwin == 0) return FA_OK;
-  FA_REQUIRE(bias && aligned16(bias), FA_ERR_INVALID, "the bias buffer must be given, 16-byte aligned");
+  FA_REQUIRE(state && aligned16(state), FA_ERR_INVALID, "the state buffer must be given, 16-byte aligned");
   const int64_t es = precision == FA_ATTN_FP32_3XTF32 ? 4 : 2;
   for (int i = 0; i < n_ptrs; ++i) {
     FA_REQUIRE(ptrs[i], FA_ERR_INVALID, "null tensor pointer");
@@ -295,6 +326,12 @@ void copy3(int64_t* dst, const int64_t* src) {
 using namespace fa;
 using namespace fa::relb;
 
+extern "C" int64_t fa_window_attention_rel_bias_state(int64_t H, int64_t nW_ids) {
+  if (H < 1 || H >= ((int64_t)1 << 31) || nW_ids < 0 || nW_ids >= ((int64_t)1 << 31))
+    return set_error(FA_ERR_INVALID, "invalid attention shape");
+  return H * kBiasVecs * 16 + nW_ids * kMaxN;
+}
+
 extern "C" int64_t fa_window_attention_rel_bias_workspace(int64_t Bwin, int64_t H, int64_t N) {
   if (Bwin < 0 || H < 1 || N < 1 || N > kMaxN || Bwin >= ((int64_t)1 << 31) || H >= ((int64_t)1 << 31) ||
       Bwin * H >= ((int64_t)1 << 31))
@@ -306,9 +343,9 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
                                             const void* q, const void* k, const void* v, void* out,
                                             const int64_t strides[12], const void* table, int table_dtype,
                                             const int32_t* index, const uint8_t* mask_u8, const uint8_t* group_ids,
-                                            int64_t nW, float scale, float* bias, float* stats, void* stream) {
+                                            int64_t nW, float scale, void* state, float* stats, void* stream) {
   const void* ptrs[4] = {q, k, v, out};
-  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 4, strides, bias, mask_u8 != nullptr, group_ids != nullptr, nW,
+  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 4, strides, state, mask_u8 != nullptr, group_ids != nullptr, nW,
                       scale);
   FA_REQUIRE(rc != FA_OK || (table && index && (table_dtype == FA_F32 || table_dtype == FA_BF16)), FA_ERR_INVALID,
              "null bias table or index, or table dtype not FA_F32 or FA_BF16");
@@ -319,13 +356,17 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
   p.scale = scale; p.scale_log2 = scale * kLog2e;
   p.q = q; p.k = k; p.v = v; p.out = out;
   copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
-  p.bias = reinterpret_cast<const float4*>(bias);
+  p.bias = reinterpret_cast<const float4*>(state);
+  p.ranks = reinterpret_cast<const uint8_t*>(p.bias + H * kBiasVecs);
   p.mask = mask_u8 ? mask_u8 : group_ids;
   if (group_ids) split_mask_value(scale, &p.mask_a, &p.mask_b);
   p.stats = reinterpret_cast<float2*>(stats);
   cudaStream_t s = (cudaStream_t)stream;
-  expand_bias_kernel<<<dim3(kBiasVecs / kExpandThreads, (unsigned)(H < 65535 ? H : 65535)), kExpandThreads, 0, s>>>(
-      table, table_dtype == FA_BF16, index, p.H, p.N, reinterpret_cast<float4*>(bias));
+  const int64_t blocks = H * kExpandBlocks + (group_ids ? (nW + kExpandThreads / 32 - 1) / (kExpandThreads / 32) : 0);
+  FA_REQUIRE(blocks < ((int64_t)1 << 31), FA_ERR_INVALID, "too many heads or mask windows");
+  expand_bias_kernel<<<(unsigned)blocks, kExpandThreads, 0, s>>>(table, table_dtype == FA_BF16, index, p.H, p.N,
+                                                                reinterpret_cast<float4*>(state), group_ids,
+                                                                group_ids ? nW : 0, const_cast<uint8_t*>(p.ranks));
   if ((rc = check_launch("expand_bias_kernel")) != FA_OK) return rc;
   const int grid = grid_of(p.num_tiles);
   p.status = attn::status_ptr();
@@ -340,11 +381,11 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
 extern "C" int fa_window_attention_rel_bias_backward(
     int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, const void* q, const void* k, const void* v,
     const void* dout, void* dq, void* dk, void* dv, const int64_t strides[21], const uint8_t* mask_u8,
-    const uint8_t* group_ids, int64_t nW, float scale, const float* bias, const float* stats, const int32_t* order,
+    const uint8_t* group_ids, int64_t nW, float scale, const void* state, const float* stats, const int32_t* order,
     const int32_t* offsets, int64_t num_buckets, void* dtable, int dtable_dtype, void* workspace,
     int64_t workspace_bytes, void* stream) {
   const void* ptrs[7] = {q, k, v, dout, dq, dk, dv};
-  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 7, strides, bias, mask_u8 != nullptr, group_ids != nullptr, nW,
+  int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 7, strides, state, mask_u8 != nullptr, group_ids != nullptr, nW,
                       scale);
   if (rc != FA_OK) return rc;
   FA_REQUIRE(stats || Bwin == 0, FA_ERR_INVALID, "null row statistics");
@@ -364,7 +405,8 @@ extern "C" int fa_window_attention_rel_bias_backward(
     p.q = q; p.k = k; p.v = v; p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
     copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
     copy3(p.sdq, strides + 12); copy3(p.sdk, strides + 15); copy3(p.sdv, strides + 18);
-    p.bias = reinterpret_cast<const float4*>(bias);
+    p.bias = reinterpret_cast<const float4*>(state);
+  p.ranks = reinterpret_cast<const uint8_t*>(p.bias + H * kBiasVecs);
     p.mask = mask_u8 ? mask_u8 : group_ids;
   if (group_ids) split_mask_value(scale, &p.mask_a, &p.mask_b);
     p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats));

@@ -9,6 +9,8 @@ namespace relb {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+constexpr int kNoRank = 255;
+
 // Tiles are (head, window) pairs in head-major order: tile t = head t / Bwin, window t % Bwin. A
 // persistent block takes a contiguous range, so it meets one head, or few, and keeps that head's
 // bias (and, backward, that head's bias gradient) across its windows.
@@ -22,6 +24,7 @@ struct Params {
   int64_t sdq[3], sdk[3], sdv[3];
   const float4* bias;        // the bias in fragment order, see expand_bias_kernel in rel_bias.cu
   const uint8_t* mask;       // (nW, N, N) bytes or (nW, N) region ids, by MaskKind
+  const uint8_t* ranks;      // with region ids: (nW, 144) rank of each token's id in its window, kNoRank past N
   uint32_t mask_a, mask_b;   // bf16 bits: mask_a * mask_b = -100 / scale (region masks, bf16 kernels)
   float2* stats;             // (Bwin, H, N): row maximum and log2 of the row sum, log2 domain
   float* slots;              // backward: (gridDim.x + H - 1) partial bias gradients (N, N)

@@ -169,75 +169,55 @@ struct ByteMask {
 };
 
 // ------------------------------------------------------------------------------------------
-// Region masks: a window's ids, ranked, by one warp; lane holds tokens lane + 32 m.
+// Region masks. The ranks of a window's ids (kMaxN bytes, kNoRank past N) come with the tile's loads;
+// one warp builds the operands, lane holds tokens lane + 32 m.
 // ------------------------------------------------------------------------------------------
 struct Regions {
-  uint32_t id[5];
-  uint32_t present[8];  // bit i of word k: id 32 k + i occurs
-  int steps;            // mask K-steps: 0 for one region
-  __device__ __forceinline__ void load(const Params& p, int w, int lane) {
-    const uint8_t* g = p.mask + (int64_t)(w % p.nW) * p.N;
+  int rank[5];
+  int steps;  // mask K-steps: 0 for one region
+  __device__ __forceinline__ void read(const uint8_t* ranks, int lane) {
+    uint32_t most = 0;
 #pragma unroll
-    for (int m = 0; m < 5; ++m) id[m] = lane + 32 * m < p.N ? (uint32_t)__ldg(g + lane + 32 * m) : 256u;
-  }
-  __device__ __forceinline__ void classify() {
-    const uint32_t first = __shfl_sync(0xffffffffu, id[0], 0);
-    bool differ = false;
-#pragma unroll
-    for (int m = 0; m < 5; ++m) differ = differ || (id[m] != first && id[m] < 256u);
-    steps = 0;
-    if (!__any_sync(0xffffffffu, differ)) return;
-    int distinct = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t bits = 0;
-#pragma unroll
-      for (int m = 0; m < 5; ++m) bits |= (id[m] >> 5) == (uint32_t)k ? 1u << (id[m] & 31) : 0u;
-      present[k] = __reduce_or_sync(0xffffffffu, bits);
-      distinct += __popc(present[k]);
-    }
-    steps = (distinct + 15) >> 4;
-  }
-  __device__ __forceinline__ int rank(uint32_t v) const {
-    int r = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t below = (v >> 5) > (uint32_t)k ? 0xffffffffu : (v >> 5) == (uint32_t)k ? (1u << (v & 31)) - 1u : 0u;
-      r += __popc(present[k] & below);
-    }
-    return r;
-  }
-  // The A and B operands of step `st` (32-byte swizzle rows of 16 bf16) at shared address `op`.
-  __device__ __noinline__ void build(uint32_t op, int st, int lane, uint32_t a_bits, uint32_t b_bits) const {
-    const uint32_t fill = b_bits | (b_bits << 16);
-#pragma unroll 1
     for (int m = 0; m < 5; ++m) {
-      const int r = lane + 32 * m;
-      if (r >= kMaxN) break;
-      const uint32_t v = m == 0 ? id[0] : m == 1 ? id[1] : m == 2 ? id[2] : m == 3 ? id[3] : id[4];
-      const int slot = v < 256u ? rank(v) - 16 * st : -1;
-      const bool in = slot >= 0 && slot < 16;
-      const uint32_t sel = 0xffffu << (16 * (slot & 1)), a = a_bits << (16 * (slot & 1));
-      uint32_t wa[8], wb[8];
+      rank[m] = lane + 32 * m < kMaxN ? (int)ranks[lane + 32 * m] : kNoRank;
+      most = max(most, rank[m] == kNoRank ? 0u : (uint32_t)rank[m]);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    steps = most > 0 ? (int)(most >> 4) + 1 : 0;
+  }
+  // The A and B operands of step `st` (rows of 16 bf16, 32-byte swizzle) at shared address `op`.
+  __device__ __forceinline__ void build(uint32_t op, int st, int lane, uint32_t a_bits, uint32_t b_bits) const {
+    const uint32_t fill = b_bits | (b_bits << 16);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool hot = in && (slot >> 1) == e;
-        wa[e] = hot ? a : 0u;
-        wb[e] = v >= 256u ? 0u : hot ? fill & ~sel : fill;
+    for (int m = 0; m < 5; ++m) {
+      if (m == 4 && lane >= kMaxN - 128) break;
+      const int r = lane + 32 * m, slot = rank[m] - 16 * st;
+      const uint32_t row = op + (uint32_t)r * 32u, f = rank[m] != kNoRank ? fill : 0u;
+      st_shared_v4(row, 0u, 0u, 0u, 0u);
+      st_shared_v4(row + 16u, 0u, 0u, 0u, 0u);
+      st_shared_v4(row + kRow32, f, f, f, f);
+      st_shared_v4(row + kRow32 + 16u, f, f, f, f);
+      if ((uint32_t)slot < 16u && rank[m] != kNoRank) {
+        const uint32_t hot = row + ((uint32_t)(((slot >> 3) ^ (r >> 2)) & 1) << 4) + (uint32_t)(slot & 7) * 2u;
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(hot), "h"((unsigned short)a_bits) : "memory");
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(hot + kRow32), "h"((unsigned short)0) : "memory");
       }
-      const uint32_t row = op + (uint32_t)r * 32u, swz = (uint32_t)((r >> 2) & 1) << 4;
-      st_shared_v4(row + swz, wa[0], wa[1], wa[2], wa[3]);
-      st_shared_v4(row + (swz ^ 16u), wa[4], wa[5], wa[6], wa[7]);
-      st_shared_v4(row + kRow32 + swz, wb[0], wb[1], wb[2], wb[3]);
-      st_shared_v4(row + kRow32 + (swz ^ 16u), wb[4], wb[5], wb[6], wb[7]);
     }
     fence_proxy_async_shared();
     __syncwarp();
   }
 };
 
+// kMaxN bytes (16-byte aligned on both sides) global -> shared, counted on an mbarrier.
+__device__ __forceinline__ void load_ranks(uint32_t dst, const Params& p, int w, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(p.ranks + (int64_t)(w % p.nW) * kMaxN), "r"((uint32_t)kMaxN), "r"(bar)
+               : "memory");
+}
+
 struct Ctx {
   uint32_t sbase, bar0, tmem;
+  uint8_t* smem;
   volatile int* abort;
   volatile int* steps;  // mask steps of a tile, by slot
   int t_begin, n_local;
@@ -259,8 +239,9 @@ constexpr int kQKBytes = 2 * kTileBytes;
 constexpr int kStageBytes = 3 * kTileBytes;
 constexpr int kOffP = kStages * kStageBytes;
 constexpr int kOffMask = kOffP + kPBytes;  // two mask steps in flight
-constexpr int kOffBars = kOffMask + 2 * kMaskOpBytes;
-constexpr int kInfoSlots = 4;  // tile i + 4 is classified after S of tile i + 1 is done, which follows tile i's
+constexpr int kOffRanks = kOffMask + 2 * kMaskOpBytes;
+constexpr int kOffBars = kOffRanks + kStages * kMaxN;
+constexpr int kInfoSlots = 4;  // tile i + 4's steps are written after S of tile i + 2 is done, which follows tile i's
 enum { kFullQK = 0, kEmptyQK = 3, kFullV = 6, kStaged = 9, kSFull = 12, kSFree, kPFull, kPEmpty, kOFull = 16,
        kOFree = 18, kDone = 20, kMaskFull = 21, kMaskEmpty = 23, kInfo = 25, kNumBars = kInfo + kInfoSlots };
 constexpr int kSmem = kOffBars + kNumBars * 8 + 64 + 1024;
@@ -411,63 +392,55 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
     bulk_commit_group();
   };
   int qk_issued = 0, v_issued = 0, jobs = 0;
-  Regions now, next;
-  if constexpr (kMask == kGroups) {
-    if (n > 0) next.load(p, c.t_begin % p.Bwin, lane);
-  }
-  // Step i loads Q and K of tile i, then V of tile i - 1, whose slot is freed about as late.
+  // Step i loads Q, K and the ranks of tile i, then V of tile i - 1, whose slot is freed about as late,
+  // and builds the mask of tile i - 1, whose ranks have landed meanwhile.
   for (int i = 0; i <= n; ++i) {
     int ok = 1;
-    if (i < n) {
+    if (lane == 0 && i < n) {
       const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i % kStages;
-      if constexpr (kMask == kGroups) {
-        now = next;
-        if (i + 1 < n) next.load(p, (t + 1) % p.Bwin, lane);  // one tile ahead
-      }
-      if (lane == 0) {
-        ok = mbar_wait(c.bar(kEmptyQK + s), (uint32_t)(((i / kStages) & 1) ^ 1), c.abort, p.status, 105, kTimeoutNs);
-        if (ok) {
-          const uint32_t dst = c.sbase + s * kStageBytes;
-          mbar_arrive_expect_tx(c.bar(kFullQK + s), kQKBytes);
-          tma_load_4d(dst, tmq, c.bar(kFullQK + s), 0, 0, h, w);
-          tma_load_4d(dst + kTileBytes, tmk, c.bar(kFullQK + s), 0, 0, h, w);
-          ++qk_issued;
-        }
-      }
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-      if constexpr (kMask == kGroups) {
-        now.classify();
-        if (lane == 0) {
-          c.steps[i % kInfoSlots] = now.steps;
-          mbar_arrive(c.bar(kInfo + i % kInfoSlots));
-        }
-        for (int st = 0; st < now.steps; ++st, ++jobs) {
-          const int b = jobs & 1;
-          if (!warp_wait(c.bar(kMaskEmpty + b), (uint32_t)(((jobs >> 1) & 1) ^ 1), c.abort, p.status, 104)) { ok = 0; break; }
-          now.build(c.sbase + kOffMask + b * kMaskOpBytes, st, lane, p.mask_a, p.mask_b);
-          if (lane == 0) mbar_arrive(c.bar(kMaskFull + b));
-        }
-        if (!ok) break;
+      ok = mbar_wait(c.bar(kEmptyQK + s), (uint32_t)(((i / kStages) & 1) ^ 1), c.abort, p.status, 105, kTimeoutNs);
+      if (ok) {
+        const uint32_t dst = c.sbase + s * kStageBytes;
+        mbar_arrive_expect_tx(c.bar(kFullQK + s), kQKBytes + (kMask == kGroups ? kMaxN : 0));
+        tma_load_4d(dst, tmq, c.bar(kFullQK + s), 0, 0, h, w);
+        tma_load_4d(dst + kTileBytes, tmk, c.bar(kFullQK + s), 0, 0, h, w);
+        if constexpr (kMask == kGroups) load_ranks(c.sbase + kOffRanks + s * kMaxN, p, w, c.bar(kFullQK + s));
+        ++qk_issued;
       }
     }
-    if (i > 0) {
-      if (lane == 0) {
-        const int j = i - 1, t = c.t_begin + j, h = t / p.Bwin, s = j % kStages;
-        if (j >= kStages) {
-          // The slot still holds the output of tile j - 3: store it and wait until it has been read.
-          ok = mbar_wait(c.bar(kStaged + s), (uint32_t)(((j - kStages) / kStages) & 1), c.abort, p.status, 107, kTimeoutNs);
-          if (ok) {
-            store_out(j - kStages);
-            bulk_wait_group_read0();
-          }
-        }
+    if (lane == 0 && ok && i > 0) {
+      const int j = i - 1, t = c.t_begin + j, h = t / p.Bwin, s = j % kStages;
+      if (j >= kStages) {
+        // The slot still holds the output of tile j - 3: store it and wait until it has been read.
+        ok = mbar_wait(c.bar(kStaged + s), (uint32_t)(((j - kStages) / kStages) & 1), c.abort, p.status, 107, kTimeoutNs);
         if (ok) {
-          mbar_arrive_expect_tx(c.bar(kFullV + s), kTileBytes);
-          tma_load_4d(c.sbase + s * kStageBytes + kQKBytes, tmv, c.bar(kFullV + s), 0, 0, h, t - h * p.Bwin);
-          ++v_issued;
+          store_out(j - kStages);
+          bulk_wait_group_read0();
         }
       }
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (ok) {
+        mbar_arrive_expect_tx(c.bar(kFullV + s), kTileBytes);
+        tma_load_4d(c.sbase + s * kStageBytes + kQKBytes, tmv, c.bar(kFullV + s), 0, 0, h, t - h * p.Bwin);
+        ++v_issued;
+      }
+    }
+    if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+    if (kMask == kGroups && i > 0) {
+      const int j = i - 1, s = j % kStages;
+      if (!warp_wait(c.bar(kFullQK + s), (uint32_t)((j / kStages) & 1), c.abort, p.status, 113)) break;
+      Regions reg;
+      reg.read(c.smem + kOffRanks + s * kMaxN, lane);
+      if (lane == 0) {
+        c.steps[j % kInfoSlots] = reg.steps;
+        mbar_arrive(c.bar(kInfo + j % kInfoSlots));
+      }
+      for (int st = 0; st < reg.steps; ++st, ++jobs) {
+        const int b = jobs & 1;
+        if (!warp_wait(c.bar(kMaskEmpty + b), (uint32_t)(((jobs >> 1) & 1) ^ 1), c.abort, p.status, 104)) { ok = 0; break; }
+        reg.build(c.sbase + kOffMask + b * kMaskOpBytes, st, lane, p.mask_a, p.mask_b);
+        if (lane == 0) mbar_arrive(c.bar(kMaskFull + b));
+      }
+      if (!ok) break;
     }
   }
   if (lane == 0) {
@@ -591,6 +564,7 @@ rel_bias_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
   int* words = reinterpret_cast<int*>(bars + kNumBars);  // abort flag, TMEM address, mask steps
   Ctx c;
+  c.smem = smem;
   c.sbase = smem_u32(smem);
   c.bar0 = smem_u32(bars);
   c.abort = words;
@@ -661,7 +635,8 @@ constexpr int kStages = 2;
 constexpr int kOffQ = 0, kOffK = kTileBytes, kOffV = 2 * kTileBytes, kOffG = 3 * kTileBytes;
 constexpr int kStageBytes = 4 * kTileBytes;
 constexpr int kOffP = kStages * kStageBytes, kOffDs = (kOffP + kPBytes + 1023) / 1024 * 1024;
-constexpr int kOffBars = kOffDs + kPBytes;
+constexpr int kOffRanks = kOffDs + kPBytes;
+constexpr int kOffBars = kOffRanks + kStages * kMaxN;
 constexpr int kMaskSlots = 4;  // mask steps built at once in the P buffer
 static_assert(kMaskSlots * kMaskOpBytes <= kPBytes, "mask operands fit the P buffer");
 enum { kFull = 0, kStaged = 2, kSMain = 4, kSRem, kPFull, kDvFull, kDsFull, kDqFull, kDkFull, kTFree, kInfo, kMaskMore,
@@ -870,11 +845,12 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
   auto load = [&](int i) {
     const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin;
     const uint32_t bar = c.bar(kFull + (i & 1)), slot = c.sbase + (i & 1) * kStageBytes;
-    mbar_arrive_expect_tx(bar, kStageBytes);
+    mbar_arrive_expect_tx(bar, kStageBytes + (kMask == kGroups ? kMaxN : 0));
     tma_load_4d(slot + kOffQ, tmq, bar, 0, 0, h, w);
     tma_load_4d(slot + kOffK, tmk, bar, 0, 0, h, w);
     tma_load_4d(slot + kOffG, tmg, bar, 0, 0, h, w);
     tma_load_4d(slot + kOffV, tmv, bar, 0, 0, h, w);
+    if constexpr (kMask == kGroups) load_ranks(c.sbase + kOffRanks + (i & 1) * kMaxN, p, w, bar);
     ++issued;
   };
   auto store = [&](int j) {
@@ -888,16 +864,12 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
   if (lane == 0) {
     for (int i = 0; i < kStages && i < n; ++i) load(i);
   }
-  Regions now, next;
-  if constexpr (kMask == kGroups) {
-    if (n > 0) next.load(p, c.t_begin % p.Bwin, lane);
-  }
   for (int i = 0; i < n; ++i) {
     int ok = 1;
     if constexpr (kMask == kGroups) {
-      now = next;
-      if (i + 1 < n) next.load(p, (c.t_begin + i + 1) % p.Bwin, lane);
-      now.classify();
+      if (!warp_wait(c.bar(kFull + (i & 1)), (uint32_t)((i >> 1) & 1), c.abort, p.status, 137)) break;
+      Regions now;
+      now.read(c.smem + kOffRanks + (i & 1) * kMaxN, lane);
       // The P buffer is free once dV of the tile before is done.
       if (i > 0 && !warp_wait(c.bar(kDvFull), (uint32_t)((i - 1) & 1), c.abort, p.status, 133)) break;
       for (int st = 0; st < now.steps && ok; ++st) {
@@ -1062,6 +1034,7 @@ rel_bias_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
   int* words = reinterpret_cast<int*>(bars + kNumBars);  // abort flag, TMEM address, mask steps
   Ctx c;
+  c.smem = smem;
   c.sbase = smem_u32(smem);
   c.bar0 = smem_u32(bars);
   c.abort = words;

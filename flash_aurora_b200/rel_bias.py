@@ -150,21 +150,26 @@ class _Call:
 
 
 def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool):
-    """Launch the forward kernels into ``out``; returns the expanded bias, and the row statistics when asked for."""
+    """Launch the forward kernels into ``out``; returns the state that the backward pass reads, and the
+    row statistics when asked for."""
     Bwin, H, N, Dh = q.shape
     dev = q.device
     with torch.cuda.device(dev):
         stats = torch.empty(Bwin, H, N, 2, device=dev, dtype=torch.float32) if want_stats else None
-        bias = torch.empty(H, _lib.FA_REL_BIAS_FLOATS, device=dev, dtype=torch.float32)
-        rc = _lib.load().fa_window_attention_rel_bias(
+        lib = _lib.load()
+        n = lib.fa_window_attention_rel_bias_state(H, call.nW if call.kind == "group_ids" else 0)
+        if n < 0:
+            _lib.check(int(n), "window_attn_rel_bias")
+        state = torch.empty(n, dtype=torch.uint8, device=dev)
+        rc = lib.fa_window_attention_rel_bias(
             _precision(q.dtype), Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
             _strides(q, k, v, out), table.data_ptr(), _lib.dtype_code(table.dtype), call.buckets.index.data_ptr(),
-            *call.masks(mask), bias.data_ptr(), _ptr(stats), _lib.stream_ptr(dev))
+            *call.masks(mask), state.data_ptr(), _ptr(stats), _lib.stream_ptr(dev))
         _lib.check(rc, "window_attn_rel_bias")
-    return bias, stats
+    return state, stats
 
 
-def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, bias, stats, table_dtype) -> Optional[torch.Tensor]:
+def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, state, stats, table_dtype) -> Optional[torch.Tensor]:
     """Launch the backward kernels into ``dq``, ``dk``, ``dv``; returns the table's gradient, in ``table_dtype``
     (None: not asked for)."""
     Bwin, H, N, Dh = q.shape
@@ -179,7 +184,7 @@ def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, bias, stats, table_d
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         rc = lib.fa_window_attention_rel_bias_backward(
             _precision(q.dtype), Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr(), _strides(q, k, v, dout, dq, dk, dv), *call.masks(mask), bias.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), _strides(q, k, v, dout, dq, dk, dv), *call.masks(mask), state.data_ptr(),
             stats.data_ptr(), b.order.data_ptr(), b.offsets.data_ptr(), b.num_buckets, _ptr(dtable),
             _lib.dtype_code(table_dtype or torch.float32), ws.data_ptr(), n, _lib.stream_ptr(dev))
         _lib.check(rc, "window_attn_rel_bias backward")
@@ -204,10 +209,10 @@ class _Attn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, mask, bias, stats = ctx.saved_tensors
+        q, k, v, mask, state, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         dq, dk, dv = (torch.empty(q.shape, device=q.device, dtype=q.dtype) for _ in range(3))
-        dtable = _backward(q, k, v, _strided(dout), dq, dk, dv, mask, ctx.call, bias, stats,
+        dtable = _backward(q, k, v, _strided(dout), dq, dk, dv, mask, ctx.call, state, stats,
                            ctx.table_dtype if need[3] else None)
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None
 
@@ -223,10 +228,10 @@ class _AttnPacked(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, mask, bias, stats = ctx.saved_tensors
+        qkv, mask, state, stats = ctx.saved_tensors
         dqkv = torch.empty_like(qkv)
         dout = _strided(_same_heads(dout.contiguous() if ctx.bnc else dout, ctx.bnc, ctx.H))
-        dtable = _backward(*_heads_of(qkv, ctx.H), dout, *_heads_of(dqkv, ctx.H), mask, ctx.call, bias, stats,
+        dtable = _backward(*_heads_of(qkv, ctx.H), dout, *_heads_of(dqkv, ctx.H), mask, ctx.call, state, stats,
                            ctx.table_dtype if ctx.needs_input_grad[1] else None)
         return dqkv if ctx.needs_input_grad[0] else None, dtable, None, None, None, None
 
@@ -260,6 +265,8 @@ def _call_args(t, N, H, table, buckets, bias, group_ids, scale_qk):
     if (mask_u8 is not None or gids is not None) and nW < 1:
         raise ValueError("a mask needs at least one window")
     scale = 1.0 / math.sqrt(_HEAD_DIM) if scale_qk is None else float(scale_qk)
+    if not 1e-30 <= abs(scale) <= 1e30:
+        raise ValueError(f"scale_qk must be finite and at least 1e-30 in magnitude, got {scale}")
     kind = "mask_u8" if mask_u8 is not None else "group_ids" if gids is not None else None
     return table.contiguous(), mask_u8 if mask_u8 is not None else gids, _Call(buckets, kind, nW, scale)
 

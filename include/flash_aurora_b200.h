@@ -286,8 +286,9 @@ int fa_window_attention_bias_noalloc(int precision, int64_t Bwin, int64_t H, int
  * head-dim stride 1, 16-byte aligned, strides multiples of 16 bytes; Dh == 64, 1 <= N <= 144.
  * table (num_buckets, H) contiguous, FA_F32 or FA_BF16; index (N, N) int32, the bucket of (query,
  * key), every value in [0, num_buckets). Masks as in fa_window_attention (region ids of any form).
- * bias (H * FA_REL_BIAS_FLOATS fp32, 16-byte aligned) receives the expanded bias, stats (nullable,
- * (Bwin, H, N, 2) fp32, 8-byte aligned) the row statistics; the backward call reads both.
+ * state (fa_window_attention_rel_bias_state(H, nW with region ids, else 0) bytes, 16-byte aligned)
+ * receives the expanded bias and mask, stats (nullable, (Bwin, H, N, 2) fp32, 8-byte aligned) the row
+ * statistics; the backward call reads both. scale must be finite, of magnitude 1e-30 to 1e30.
  *
  * The backward call takes dout with out's meaning and writes dq, dk, dv; strides are {q, k, v,
  * dout, dq, dk, dv} x {window, head, token}. dtable (nullable, (num_buckets, H), FA_F32 or FA_BF16) is
@@ -297,18 +298,18 @@ int fa_window_attention_bias_noalloc(int precision, int64_t Bwin, int64_t H, int
  * fa_window_attention_rel_bias_workspace(...) bytes (negative: a status), 16-byte aligned, used until the
  * call's work on the stream is done.
  */
-enum { FA_REL_BIAS_FLOATS = 20736 };
 int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, const void* q,
                                  const void* k, const void* v, void* out, const int64_t strides[12],
                                  const void* table, int table_dtype, const int32_t* index,
                                  const uint8_t* mask_u8, const uint8_t* group_ids, int64_t nW, float scale,
-                                 float* bias, float* stats, void* stream);
+                                 void* state, float* stats, void* stream);
+int64_t fa_window_attention_rel_bias_state(int64_t H, int64_t nW_ids);
 int64_t fa_window_attention_rel_bias_workspace(int64_t Bwin, int64_t H, int64_t N);
 int fa_window_attention_rel_bias_backward(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh,
                                           const void* q, const void* k, const void* v, const void* dout,
                                           void* dq, void* dk, void* dv, const int64_t strides[21],
                                           const uint8_t* mask_u8, const uint8_t* group_ids, int64_t nW,
-                                          float scale, const float* bias, const float* stats,
+                                          float scale, const void* state, const float* stats,
                                           const int32_t* order, const int32_t* offsets, int64_t num_buckets,
                                           void* dtable, int dtable_dtype, void* workspace,
                                           int64_t workspace_bytes, void* stream);

@@ -101,9 +101,9 @@ def test_abi_refusals_without_a_gpu():
     p = ctypes.c_void_p(1 << 20)
     st = (ctypes.c_int64 * 21)(*([64] * 21))
 
-    def fwd(prec=0, B=4, H=2, N=16, D=64, q=p, table=p, tdt=0, index=p, u8=None, ids=None, nW=0, strides=st, bias=p):
+    def fwd(prec=0, B=4, H=2, N=16, D=64, q=p, table=p, tdt=0, index=p, u8=None, ids=None, nW=0, strides=st, bias=p, scale=0.125):
         return lib.fa_window_attention_rel_bias(prec, B, H, N, D, q, p, p, p, strides, table, tdt, index, u8, ids, nW,
-                                                0.125, bias, None, None)
+                                                scale, bias, None, None)
 
     assert fwd(prec=3) == _lib.FA_ERR_INVALID
     assert fwd(D=32) == _lib.FA_ERR_UNSUPPORTED and b"head_dim" in lib.fa_last_error()
@@ -118,14 +118,18 @@ def test_abi_refusals_without_a_gpu():
     assert fwd(B=1 << 30, H=4) == _lib.FA_ERR_INVALID and b"tiles" in lib.fa_last_error()
     bad = (ctypes.c_int64 * 21)(*([60] * 21))
     assert fwd(strides=bad) == _lib.FA_ERR_INVALID and b"16 bytes" in lib.fa_last_error()
-    assert fwd(bias=None) == _lib.FA_ERR_INVALID and b"bias buffer" in lib.fa_last_error()
+    for bad_scale in (0.0, float("nan"), float("inf"), 1e-35):
+        assert fwd(scale=bad_scale) == _lib.FA_ERR_INVALID and b"scale" in lib.fa_last_error()
+    assert lib.fa_window_attention_rel_bias_state(3, 5) == 3 * 144 * 144 * 4 + 5 * 144
+    assert lib.fa_window_attention_rel_bias_state(0, 5) == _lib.FA_ERR_INVALID
+    assert fwd(bias=None) == _lib.FA_ERR_INVALID and b"state buffer" in lib.fa_last_error()
     assert fwd(B=0, q=None) == _lib.FA_OK
 
     def bwd(stats=p, order=p, nb=5, ws=p, nbytes=1 << 40, tdt=0, bias=p):
         return lib.fa_window_attention_rel_bias_backward(0, 4, 2, 16, 64, p, p, p, p, p, p, p, st, None, None, 0, 0.125,
                                                          bias, stats, order, p, nb, p, tdt, ws, nbytes, None)
 
-    assert bwd(bias=None) == _lib.FA_ERR_INVALID and b"bias buffer" in lib.fa_last_error()
+    assert bwd(bias=None) == _lib.FA_ERR_INVALID and b"state buffer" in lib.fa_last_error()
     assert bwd(tdt=2) == _lib.FA_ERR_INVALID and b"table dtype" in lib.fa_last_error()
     assert bwd(stats=None) == _lib.FA_ERR_INVALID and b"statistics" in lib.fa_last_error()
     assert bwd(order=None) == _lib.FA_ERR_INVALID and b"bucket lists" in lib.fa_last_error()
