@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) rel_bias_fwd_kernel(const Params p) 
     }
     T* orow = reinterpret_cast<T*>(p.out) + w * p.so[0] + h * p.so[1] + i * p.so[2];
     for (int d = 0; d < 64; ++d) orow[d] = from_f32<T>(o[d] / l);
-    if (p.stats) p.stats[((int64_t)w * p.H + h) * p.N + i] = make_float2(m, log2f(l));
+    if (p.stats) p.stats[((int64_t)w * p.H + h) * kMaxN + i] = make_float2(m, log2f(l));
   }
 }
 
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) rel_bias_bwd_kernel(const Params p) 
     load_rows<T>(sK, p.k, p.sk, w, h, p.N);
     load_rows<T>(sV, p.v, p.sv, w, h, p.N);
     load_rows<T>(sG, p.dout, p.so, w, h, p.N);
-    if (i < p.N) sStat[i] = p.stats[((int64_t)w * p.H + h) * p.N + i];
+    if (i < p.N) sStat[i] = p.stats[((int64_t)w * p.H + h) * kMaxN + i];
     __syncthreads();
     if (i < p.N) {
       float acc[64];
@@ -350,6 +350,7 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
   FA_REQUIRE(rc != FA_OK || (table && index && (table_dtype == FA_F32 || table_dtype == FA_BF16)), FA_ERR_INVALID,
              "null bias table or index, or table dtype not FA_F32 or FA_BF16");
   if (rc != FA_OK || Bwin == 0) return rc;
+  FA_REQUIRE(aligned16(stats), FA_ERR_INVALID, "the row statistics must be 16-byte aligned");
   Params p{};
   p.Bwin = (int)Bwin; p.H = (int)H; p.N = (int)N; p.nW = (int)(nW > 0 ? nW : 1);
   p.num_tiles = (int)(Bwin * H);
@@ -388,7 +389,8 @@ extern "C" int fa_window_attention_rel_bias_backward(
   int rc = check_args(precision, Bwin, H, N, Dh, ptrs, 7, strides, state, mask_u8 != nullptr, group_ids != nullptr, nW,
                       scale);
   if (rc != FA_OK) return rc;
-  FA_REQUIRE(stats || Bwin == 0, FA_ERR_INVALID, "null row statistics");
+  FA_REQUIRE((stats && aligned16(stats)) || Bwin == 0, FA_ERR_INVALID,
+             "the row statistics must be given, 16-byte aligned");
   FA_REQUIRE(!dtable || dtable_dtype == FA_F32 || dtable_dtype == FA_BF16, FA_ERR_INVALID,
              "table dtype must be FA_F32 or FA_BF16");
   FA_REQUIRE(!dtable || (order && offsets && num_buckets >= 1 && num_buckets < ((int64_t)1 << 31) && H <= 65535),

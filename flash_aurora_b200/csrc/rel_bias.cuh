@@ -26,7 +26,7 @@ struct Params {
   const uint8_t* mask;       // (nW, N, N) bytes or (nW, N) region ids, by MaskKind
   const uint8_t* ranks;      // with region ids: (nW, 144) rank of each token's id in its window, kNoRank past N
   uint32_t mask_a, mask_b;   // bf16 bits: mask_a * mask_b = -100 / scale (region masks, bf16 kernels)
-  float2* stats;             // (Bwin, H, N): row maximum and log2 of the row sum, log2 domain
+  float2* stats;             // (Bwin, H, 144): row maximum and log2 of the row sum, log2 domain
   float* slots;              // backward: (gridDim.x + H - 1) partial bias gradients (N, N)
   int* status;
 };

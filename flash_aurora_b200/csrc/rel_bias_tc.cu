@@ -208,11 +208,14 @@ struct Regions {
   }
 };
 
-// kMaxN bytes (16-byte aligned on both sides) global -> shared, counted on an mbarrier.
-__device__ __forceinline__ void load_ranks(uint32_t dst, const Params& p, int w, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(p.ranks + (int64_t)(w % p.nW) * kMaxN), "r"((uint32_t)kMaxN), "r"(bar)
+// `bytes` (a multiple of 16, 16-byte aligned on both sides) global -> shared, counted on an mbarrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
                : "memory");
+}
+__device__ __forceinline__ void load_ranks(uint32_t dst, const Params& p, int w, uint32_t bar) {
+  bulk_load(dst, p.ranks + (int64_t)(w % p.nW) * kMaxN, kMaxN, bar);
 }
 
 struct Ctx {
@@ -364,10 +367,9 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bar(kPFull));
     if (p.stats && l.t0 == 0) {
-      float2* st = p.stats + ((int64_t)w * p.H + h) * p.N;
+      float2* st = p.stats + ((int64_t)w * p.H + h) * kMaxN;
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (l.row[r] < p.N) st[l.row[r]] = make_float2(mx[r], log2f(sum[r]));
+      for (int r = 0; r < R; ++r) st[l.row[r]] = make_float2(mx[r], log2f(sum[r]));
     }
     if (prev >= 0 && !epilogue(prev)) { ok = false; break; }
     prev = i;
@@ -634,14 +636,18 @@ namespace bwd {
 constexpr int kStages = 2;
 constexpr int kOffQ = 0, kOffK = kTileBytes, kOffV = 2 * kTileBytes, kOffG = 3 * kTileBytes;
 constexpr int kStageBytes = 4 * kTileBytes;
-constexpr int kOffP = kStages * kStageBytes, kOffDs = (kOffP + kPBytes + 1023) / 1024 * 1024;
-constexpr int kOffRanks = kOffDs + kPBytes;
+// P, the small things in the gap before the next 1024-byte boundary, dS, the row statistics of one tile.
+constexpr int kOffP = kStages * kStageBytes;
+constexpr int kOffRanks = kOffP + kPBytes;
 constexpr int kOffBars = kOffRanks + kStages * kMaxN;
+constexpr int kOffDs = (kOffP + kPBytes + 1023) / 1024 * 1024;
+constexpr int kOffStats = kOffDs + kPBytes, kStatsBytes = kMaxN * 8;
 constexpr int kMaskSlots = 4;  // mask steps built at once in the P buffer
 static_assert(kMaskSlots * kMaskOpBytes <= kPBytes, "mask operands fit the P buffer");
-enum { kFull = 0, kStaged = 2, kSMain = 4, kSRem, kPFull, kDvFull, kDsFull, kDqFull, kDkFull, kTFree, kInfo, kMaskMore,
-       kMaskEmpty, kDone, kNumBars };
-constexpr int kSmem = kOffBars + kNumBars * 8 + 64 + 1024;
+enum { kFull = 0, kStaged = 2, kSMain = 4, kSRem, kPFull, kDvFull, kDsFull, kDqFull, kDkFull, kTFree, kStats, kInfo,
+       kMaskMore, kMaskEmpty, kDone, kNumBars };
+static_assert(kOffBars + kNumBars * 8 + 24 <= kOffDs, "barriers and words fit the gap");
+constexpr int kSmem = kOffStats + kStatsBytes;  // no slack: the kernel checks the base's alignment
 static_assert(kSmem <= 227 * 1024, "shared memory budget");
 constexpr uint32_t kColS = 0, kColP = 144, kColS2 = 288, kColDv = 432, kColRem = 496;
 constexpr uint32_t kColDq = kColS2, kColDk = kColS2 + 64, kColDq2 = kColS2 + 128;
@@ -669,29 +675,29 @@ __device__ __forceinline__ void stage_rem(uint32_t taddr, uint32_t stg, int warp
   }
 }
 
-// The 16-column blocks of two accumulators in turn. Warps 4..11 keep the next block's loads in flight;
+// The 8-column blocks of two accumulators in turn. Warps 4..11 keep the next block's loads in flight;
 // warps 2 and 3, with fewer registers and half the rows, do not.
 template <bool kRem>
 struct TmemBlocks {
   uint32_t a, b;
-  uint32_t va[8], vb[8];
+  uint32_t va[4], vb[4];
   __device__ __forceinline__ TmemBlocks(uint32_t a_, uint32_t b_) : a(a_), b(b_) {
     if constexpr (!kRem) load(0);
   }
-  __device__ __forceinline__ void load(int q) {
-    tmem_ld_16x256b_r8(a + 16 * q, va);
-    tmem_ld_16x256b_r8(b + 16 * q, vb);
+  __device__ __forceinline__ void load(int j) {
+    tmem_ld_16x256b_r4(a + 8 * j, va);
+    tmem_ld_16x256b_r4(b + 8 * j, vb);
   }
-  __device__ __forceinline__ void next(int q, uint32_t (&ca)[8], uint32_t (&cb)[8]) {
-    if constexpr (kRem) load(q);
+  __device__ __forceinline__ void next(int j, uint32_t (&ca)[4], uint32_t (&cb)[4]) {
+    if constexpr (kRem) load(j);
     tmem_wait_ld();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4; ++e) {
       ca[e] = va[e];
       cb[e] = vb[e];
     }
     if constexpr (!kRem) {
-      if (q < 8) load(q + 1);
+      if (j < 17) load(j + 1);
     }
   }
 };
@@ -736,10 +742,11 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     }
     // Row statistics; +inf past N makes the rows' P zero.
     float2 mx[R], lg[R], d2[R];
-    const float2* st = p.stats + ((int64_t)w * p.H + h) * p.N;
+    if (!warp_wait(c.bar(kStats), par, c.abort, p.status, 120)) return;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float2 v = l.row[r] < p.N ? __ldg(st + l.row[r]) : make_float2(INFINITY, 0.f);
+      const float2 v = l.row[r] < p.N ? reinterpret_cast<const float2*>(c.smem + kOffStats)[l.row[r]]
+                                      : make_float2(INFINITY, 0.f);
       mx[r] = make_float2(-v.x, -v.x);
       lg[r] = make_float2(-v.y, -v.y);
       d2[r] = make_float2(0.f, 0.f);
@@ -748,32 +755,28 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     if constexpr (kMask == kMaskU8) mask.begin(p, l, w);
     if (!warp_wait(c.bar(kRem ? kSRem : kSMain), par, c.abort, p.status, 121)) return;
     tc_fence_after();
-    // Pass 1, 16 keys (two 8-key blocks) at a time, the next loads in flight.
+    // Pass 1.
     TmemBlocks<kRem> blk(tS, tP);
 #pragma unroll
-    for (int q = 0; q < 9; ++q) {
-      uint32_t cs[8], cg[8];
-      blk.next(q, cs, cg);
+    for (int j = 0; j < 18; ++j) {
+      uint32_t cs[4], cg[4];
+      blk.next(j, cs, cg);
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const int j = 2 * q + (e >> 2);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          float2 x = __ffma2_rn(l.pick(&cs[e], r), c2, bias.b[j][r]);
-          if constexpr (kMask == kMaskU8) mask.apply(p, l, j, r, x);
-          x = __fadd2_rn(__fadd2_rn(x, mx[r]), lg[r]);
-          const float2 pr = make_float2(ex2(x.x), ex2(x.y));
-          d2[r] = __ffma2_rn(pr, l.pick(&cg[e], r), d2[r]);
-          l.store_p(sP, j, r, pack_bf16x2(pr.x, pr.y));
-          cs[e + 2 * r] = __float_as_uint(pr.x);
-          cs[e + 2 * r + 1] = __float_as_uint(pr.y);
-          if constexpr (kRem) {  // the lanes' other row is nobody's
-            cs[e + 2] = cs[e];
-            cs[e + 3] = cs[e + 1];
-          }
+      for (int r = 0; r < R; ++r) {
+        float2 x = __ffma2_rn(l.pick(cs, r), c2, bias.b[j][r]);
+        if constexpr (kMask == kMaskU8) mask.apply(p, l, j, r, x);
+        x = __fadd2_rn(__fadd2_rn(x, mx[r]), lg[r]);
+        const float2 pr = make_float2(ex2(x.x), ex2(x.y));
+        d2[r] = __ffma2_rn(pr, l.pick(cg, r), d2[r]);
+        l.store_p(sP, j, r, pack_bf16x2(pr.x, pr.y));
+        cs[2 * r] = __float_as_uint(pr.x);
+        cs[2 * r + 1] = __float_as_uint(pr.y);
+        if constexpr (kRem) {  // the lanes' other row is nobody's
+          cs[2] = cs[0];
+          cs[3] = cs[1];
         }
       }
-      tmem_st_16x256b_r8(tS + 16 * q, cs);
+      tmem_st_16x256b_r4(tS + 8 * j, cs);
     }
     tmem_wait_st();
     fence_proxy_async_shared();
@@ -789,18 +792,14 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     // Pass 2.
     TmemBlocks<kRem> blk2(tS, tP);
 #pragma unroll
-    for (int q = 0; q < 9; ++q) {
-      uint32_t cs[8], cg[8];
-      blk2.next(q, cs, cg);
+    for (int j = 0; j < 18; ++j) {
+      uint32_t cs[4], cg[4];
+      blk2.next(j, cs, cg);
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const int j = 2 * q + (e >> 2);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float2 g = __fmul2_rn(l.pick(&cs[e], r), __fadd2_rn(l.pick(&cg[e], r), d2[r]));
-          grad[j][r] = __fadd2_rn(grad[j][r], g);
-          l.store_p(sDs, j, r, pack_bf16x2(g.x, g.y));
-        }
+      for (int r = 0; r < R; ++r) {
+        const float2 g = __fmul2_rn(l.pick(cs, r), __fadd2_rn(l.pick(cg, r), d2[r]));
+        grad[j][r] = __fadd2_rn(grad[j][r], g);
+        l.store_p(sDs, j, r, pack_bf16x2(g.x, g.y));
       }
     }
     fence_proxy_async_shared();
@@ -841,7 +840,7 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
                                          const CUtensorMap* tmk, const CUtensorMap* tmv, const CUtensorMap* tmg,
                                          const CUtensorMap* tmdq, const CUtensorMap* tmdk, const CUtensorMap* tmdv) {
   const int n = c.n_local;
-  int issued = 0, more = 0;
+  int issued = 0, stats_issued = 0, more = 0;
   auto load = [&](int i) {
     const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin;
     const uint32_t bar = c.bar(kFull + (i & 1)), slot = c.sbase + (i & 1) * kStageBytes;
@@ -861,7 +860,14 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
     tma_store_4d(tmdv, slot + kOffV, 0, 0, h, w);
     bulk_commit_group();
   };
+  auto load_stats = [&](int i) {
+    const int t = c.t_begin + i, h = t / p.Bwin;
+    mbar_arrive_expect_tx(c.bar(kStats), kStatsBytes);
+    bulk_load(c.sbase + kOffStats, p.stats + ((int64_t)(t - h * p.Bwin) * p.H + h) * kMaxN, kStatsBytes, c.bar(kStats));
+    ++stats_issued;
+  };
   if (lane == 0) {
+    if (n > 0) load_stats(0);
     for (int i = 0; i < kStages && i < n; ++i) load(i);
   }
   for (int i = 0; i < n; ++i) {
@@ -909,10 +915,19 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
       }
       if (!__shfl_sync(0xffffffffu, ok, 0)) break;
     }
+    if (i + 1 < n) {
+      // Every softmax warp has read tile i's statistics once its P is there.
+      if (lane == 0) {
+        ok = mbar_wait(c.bar(kPFull), (uint32_t)(i & 1), c.abort, p.status, 138, kTimeoutNs);
+        if (ok) load_stats(i + 1);
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+    }
   }
   if (lane == 0) {
     // Never leave with copies in flight (bounded, also after an abort).
     int no_abort = 0;
+    if (stats_issued > 0) mbar_wait(c.bar(kStats), (uint32_t)((stats_issued - 1) & 1), &no_abort, p.status, 139, kTimeoutNs);
     for (int j = issued > kStages ? issued - kStages : 0; j < issued; ++j)
       mbar_wait(c.bar(kFull + (j & 1)), (uint32_t)((j >> 1) & 1), &no_abort, p.status, 126, kTimeoutNs);
     for (int j = n > kStages ? n - kStages : 0; j < n; ++j) {
@@ -1029,8 +1044,11 @@ rel_bias_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
                        const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmg,
                        const __grid_constant__ CUtensorMap tmdq, const __grid_constant__ CUtensorMap tmdk,
                        const __grid_constant__ CUtensorMap tmdv, const Params p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // uniform; dynamic shared memory starts on such a boundary here
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, 140);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
   int* words = reinterpret_cast<int*>(bars + kNumBars);  // abort flag, TMEM address, mask steps
   Ctx c;

@@ -155,7 +155,7 @@ def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool):
     Bwin, H, N, Dh = q.shape
     dev = q.device
     with torch.cuda.device(dev):
-        stats = torch.empty(Bwin, H, N, 2, device=dev, dtype=torch.float32) if want_stats else None
+        stats = torch.empty(Bwin, H, _MAX_TOKENS, 2, device=dev, dtype=torch.float32) if want_stats else None
         lib = _lib.load()
         n = lib.fa_window_attention_rel_bias_state(H, call.nW if call.kind == "group_ids" else 0)
         if n < 0:

@@ -287,7 +287,7 @@ int fa_window_attention_bias_noalloc(int precision, int64_t Bwin, int64_t H, int
  * table (num_buckets, H) contiguous, FA_F32 or FA_BF16; index (N, N) int32, the bucket of (query,
  * key), every value in [0, num_buckets). Masks as in fa_window_attention (region ids of any form).
  * state (fa_window_attention_rel_bias_state(H, nW with region ids, else 0) bytes, 16-byte aligned)
- * receives the expanded bias and mask, stats (nullable, (Bwin, H, N, 2) fp32, 8-byte aligned) the row
+ * receives the expanded bias and mask, stats (nullable, (Bwin, H, 144, 2) fp32, 16-byte aligned) the row
  * statistics; the backward call reads both. scale must be finite, of magnitude 1e-30 to 1e30.
  *
  * The backward call takes dout with out's meaning and writes dq, dk, dv; strides are {q, k, v,
