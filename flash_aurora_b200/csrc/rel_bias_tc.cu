@@ -619,17 +619,20 @@ rel_bias_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
 //   pass 2   dS = P (dP - delta), added to the head's bias gradient (fp32, in registers: 72 of each
 //            thread of warps 4..11), and to shared memory in bf16
 //   dQ = dS K, dK = dS^T Q                     dV and dQ are drained meanwhile; then S and dP of the next tile,
-//                                              while dK is drained
+//                                              while dK is drained. Rows 128..143, whose S comes last, are the
+//                                              last K-step of dV and dK and no part of the M=128 dQ, so nothing
+//                                              waits for them early
 // dV, dK, dQ of keys / rows 0..127 are M=128 UMMAs (P and dS are read MN-major for dV and dK); those
 // of 128..143 are computed transposed, (64 head dims) x (16 rows), as M=64, N=16 UMMAs, at half
 // the cost of an M=64, N=64 block.
 // TMEM columns: S / P 0..143, dP 144..287, the M=64 blocks of S and dP in the two lane halves of 288..431,
-// and over them, once pass 2 has read them, dQ 288..351, dK 352..415 and dQ's transposed remainder
-// 416..431; dV 432..495; the transposed remainders of dV and dK in the lane halves of 496..511.
+// dV 432..495, the transposed remainders of dV and dK in the lane halves of 496..511. Over S, once pass 2 of
+// rows 0..127 has read it, dQ 0..63; over the M=64 blocks, once pass 2 of rows 128..143 has, dK 288..351 and
+// dQ's transposed remainder 416..431.
 // Outputs are staged in the tile's own slots (dV over V, dK over K, dQ over dO, which dV was the last to
 // read) and stored by warp 0 before it loads the tile after next into them. Two input slots, P and dS fill shared memory (230 KB);
-// the mask operands of a tile are built in the P buffer, which is free between dV of the tile before and
-// the tile's own pass 1.
+// the mask operands of a tile are built in the dS buffer, which is free between dK of the tile before and
+// the tile's own pass 2.
 // ------------------------------------------------------------------------------------------
 namespace bwd {
 
@@ -644,13 +647,13 @@ constexpr int kOffDs = (kOffP + kPBytes + 1023) / 1024 * 1024;
 constexpr int kOffStats = kOffDs + kPBytes, kStatsBytes = kMaxN * 8;
 constexpr int kMaskSlots = 4;  // mask steps built at once in the P buffer
 static_assert(kMaskSlots * kMaskOpBytes <= kPBytes, "mask operands fit the P buffer");
-enum { kFull = 0, kStaged = 2, kSMain = 4, kSRem, kPFull, kDvFull, kDsFull, kDqFull, kDkFull, kTFree, kStats, kInfo,
-       kMaskMore, kMaskEmpty, kDone, kNumBars };
+enum { kFull = 0, kStaged = 2, kSMain = 4, kSRem, kPMain, kPRem, kDvFull, kDsMain, kDsRem, kDqFull, kRemFull, kDkFull,
+       kDqFree, kTFree, kStats, kInfo, kMaskMore, kMaskEmpty, kDone, kNumBars };
 static_assert(kOffBars + kNumBars * 8 + 24 <= kOffDs, "barriers and words fit the gap");
 constexpr int kSmem = kOffStats + kStatsBytes;  // no slack: the kernel checks the base's alignment
 static_assert(kSmem <= 227 * 1024, "shared memory budget");
 constexpr uint32_t kColS = 0, kColP = 144, kColS2 = 288, kColDv = 432, kColRem = 496;
-constexpr uint32_t kColDq = kColS2, kColDk = kColS2 + 64, kColDq2 = kColS2 + 128;
+constexpr uint32_t kColDq = kColS, kColDk = kColS2, kColDq2 = kColS2 + 128;
 constexpr uint32_t kRegsSmall = 120, kRegsMain = 192;
 static_assert(4 * kRegsSmall + 8 * kRegsMain <= 12 * kRegsLaunch, "register split");
 constexpr uint32_t kIdescT = make_idesc(1, 128, 64, true, true);    // A and B MN-major: dV, dK
@@ -675,26 +678,34 @@ __device__ __forceinline__ void stage_rem(uint32_t taddr, uint32_t stg, int warp
   }
 }
 
-// The 8-column blocks of two accumulators in turn. Warps 4..11 keep the next block's loads in flight;
-// warps 2 and 3, with fewer registers and half the rows, do not.
+// The blocks of two accumulators in turn: 8 columns with the next block's loads in flight for warps 4..11,
+// 16 columns without for warps 2 and 3, which have half the rows and fewer registers.
 template <bool kRem>
 struct TmemBlocks {
+  static constexpr int kRegs = kRem ? 8 : 4;
   uint32_t a, b;
-  uint32_t va[4], vb[4];
+  uint32_t va[kRegs], vb[kRegs];
   __device__ __forceinline__ TmemBlocks(uint32_t a_, uint32_t b_) : a(a_), b(b_) {
     if constexpr (!kRem) load(0);
   }
   __device__ __forceinline__ void load(int j) {
-    tmem_ld_16x256b_r4(a + 8 * j, va);
-    tmem_ld_16x256b_r4(b + 8 * j, vb);
+    if constexpr (kRem) {
+      tmem_ld_16x256b_r8(a + 8 * j, va);
+      tmem_ld_16x256b_r8(b + 8 * j, vb);
+    } else {
+      tmem_ld_16x256b_r4(a + 8 * j, va);
+      tmem_ld_16x256b_r4(b + 8 * j, vb);
+    }
   }
+  // The registers of 8-key block j, j = 0..17 in order.
   __device__ __forceinline__ void next(int j, uint32_t (&ca)[4], uint32_t (&cb)[4]) {
-    if constexpr (kRem) load(j);
-    tmem_wait_ld();
+    const int o = kRem ? 4 * (j & 1) : 0;
+    if (kRem && (j & 1) == 0) load(j);
+    if (!kRem || (j & 1) == 0) tmem_wait_ld();
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      ca[e] = va[e];
-      cb[e] = vb[e];
+      ca[e] = va[o + e];
+      cb[e] = vb[o + e];
     }
     if constexpr (!kRem) {
       if (j < 17) load(j + 1);
@@ -727,10 +738,15 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
       }
     }
   };
-  for (int i = 0; i < c.n_local; ++i) {
-    const int t = c.t_begin + i, h = t / p.Bwin, w = t - h * p.Bwin, s = i & 1;
+  int h = c.t_begin / p.Bwin, w = c.t_begin - h * p.Bwin;
+  for (int i = 0; i < c.n_local; ++i, ++w) {
+    const int s = i & 1;
     const uint32_t par = (uint32_t)(i & 1);
     const uint32_t slot = c.sbase + s * kStageBytes;
+    if (w == p.Bwin) {
+      w = 0;
+      ++h;
+    }
     if (h != cur_h) {
       if (cur_h >= 0) flush(cur_h);
       cur_h = h;
@@ -781,7 +797,7 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     tmem_wait_st();
     fence_proxy_async_shared();
     __syncwarp();
-    if (lane == 0) mbar_arrive(c.bar(kPFull));
+    if (lane == 0) mbar_arrive(c.bar(kRem ? kPRem : kPMain));
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float d = d2[r].x + d2[r].y;
@@ -789,7 +805,8 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
       d += __shfl_xor_sync(0xffffffffu, d, 2);
       d2[r] = make_float2(-d, -d);
     }
-    // Pass 2.
+    // Pass 2. The dS buffer held the tile's mask operands until the last product of S was done.
+    if (kMask == kGroups && !kRem && !warp_wait(c.bar(kSRem), par, c.abort, p.status, 119)) return;
     TmemBlocks<kRem> blk2(tS, tP);
 #pragma unroll
     for (int j = 0; j < 18; ++j) {
@@ -805,7 +822,7 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
     fence_proxy_async_shared();
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(c.bar(kDsFull));
+    if (lane == 0) mbar_arrive(c.bar(kRem ? kDsRem : kDsMain));
     if constexpr (!kRem) {
       uint32_t o[32];
       auto drain = [&](int bar, int code, uint32_t col, uint32_t stg, float scale) -> bool {
@@ -820,9 +837,15 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
       if (!drain(kDvFull, 122, kColDv, slot + kOffV, 1.f)) return;
       if (warp < 8) stage_rem(c.tmem + kColRem, slot + kOffV, warp, lane, 1.f);
       if (!drain(kDqFull, 123, kColDq, slot + kOffG, p.scale)) return;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(c.bar(kDqFree));
+      if (!warp_wait(c.bar(kRemFull), par, c.abort, p.status, 118)) return;
+      tc_fence_after();
+      // The remainders; the K tile's last reader was dQ's.
       if (warp >= 8) stage_rem(c.tmem + kColDq2, slot + kOffG, warp, lane, p.scale);
+      else stage_rem(c.tmem + kColRem + kLaneHalf, slot + kOffK, warp, lane, p.scale);
       if (!drain(kDkFull, 124, kColDk, slot + kOffK, p.scale)) return;
-      if (warp < 8) stage_rem(c.tmem + kColRem + kLaneHalf, slot + kOffK, warp, lane, p.scale);
       fence_proxy_async_shared();
       tc_fence_before();
       __syncwarp();
@@ -876,8 +899,8 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
       if (!warp_wait(c.bar(kFull + (i & 1)), (uint32_t)((i >> 1) & 1), c.abort, p.status, 137)) break;
       Regions now;
       now.read(c.smem + kOffRanks + (i & 1) * kMaxN, lane);
-      // The P buffer is free once dV of the tile before is done.
-      if (i > 0 && !warp_wait(c.bar(kDvFull), (uint32_t)((i - 1) & 1), c.abort, p.status, 133)) break;
+      // The dS buffer is free once dK of the tile before is done.
+      if (now.steps > 0 && i > 0 && !warp_wait(c.bar(kDkFull), (uint32_t)((i - 1) & 1), c.abort, p.status, 133)) break;
       for (int st = 0; st < now.steps && ok; ++st) {
         if (st > 0 && st % kMaskSlots == 0) {  // more than 64 regions: wait until the slots have been read
           if (lane == 0) {
@@ -891,7 +914,7 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
           ok = warp_wait(c.bar(kMaskEmpty), (uint32_t)(more & 1), c.abort, p.status, 134);
           ++more;
         }
-        if (ok) now.build(c.sbase + kOffP + (st % kMaskSlots) * kMaskOpBytes, st, lane, p.mask_a, p.mask_b);
+        if (ok) now.build(c.sbase + kOffDs + (st % kMaskSlots) * kMaskOpBytes, st, lane, p.mask_a, p.mask_b);
       }
       if (!ok) break;
       if (lane == 0) {
@@ -918,7 +941,8 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
     if (i + 1 < n) {
       // Every softmax warp has read tile i's statistics once its P is there.
       if (lane == 0) {
-        ok = mbar_wait(c.bar(kPFull), (uint32_t)(i & 1), c.abort, p.status, 138, kTimeoutNs);
+        ok = mbar_wait(c.bar(kPMain), (uint32_t)(i & 1), c.abort, p.status, 138, kTimeoutNs) &&
+             mbar_wait(c.bar(kPRem), (uint32_t)(i & 1), c.abort, p.status, 138, kTimeoutNs);
         if (ok) load_stats(i + 1);
       }
       if (!__shfl_sync(0xffffffffu, ok, 0)) break;
@@ -946,7 +970,7 @@ __device__ __forceinline__ void issuer(const Params& p, const Ctx& c) {
   const uint64_t row0 = desc_sw128(c.sbase, 16, 1024), col0 = desc_sw128(c.sbase, kTileBytes, 1024);
   const uint64_t pT = desc_sw128(sP, kPChunk, 1024), p32 = desc_sw32(sP + 2 * kPChunk, 256);
   const uint64_t dsT = desc_sw128(sDs, kPChunk, 1024), ds = desc_sw128(sDs, 16, 1024);
-  const uint64_t ds32 = desc_sw32(sDs + 2 * kPChunk, 256), mask0 = desc_sw32(sP, 256);
+  const uint64_t ds32 = desc_sw32(sDs + 2 * kPChunk, 256), mask0 = desc_sw32(sDs, 256);
   int more = 0;
   for (int i = 0; i < c.n_local; ++i) {
     const int s = i & 1;
@@ -954,25 +978,32 @@ __device__ __forceinline__ void issuer(const Params& p, const Ctx& c) {
     const uint64_t qr = at(row0, slot + kOffQ), kr = at(row0, slot + kOffK), vr = at(row0, slot + kOffV),
                    gr = at(row0, slot + kOffG);
     const uint64_t qc = at(col0, slot + kOffQ), kc = at(col0, slot + kOffK), gc = at(col0, slot + kOffG);
-    // S and dP of rows 0..127 as soon as the inputs are there (their columns are free: pass 2 of the
-    // tile before is done); the M=64 blocks once dQ and dK have been drained. A masked tile issues
-    // both together: its mask operands are overwritten by P.
+    // S and dP of rows 0..127 as soon as the inputs are there and dQ of the tile before has been drained
+    // (pass 2 of that tile is done); the M=64 blocks once its dK has been.
     if (!warp_wait(c.bar(kFull + s), (uint32_t)((i >> 1) & 1), c.abort, p.status, 128)) break;
-    int steps = 0;
-    if constexpr (kMask == kGroups) {
-      if (!warp_wait(c.bar(kInfo), par, c.abort, p.status, 135)) break;
-      steps = c.steps[i & 1];
-      if (steps > 0 && !warp_wait(c.bar(kTFree), par ^ 1u, c.abort, p.status, 129)) break;
-    }
+    if (!warp_wait(c.bar(kDqFree), par ^ 1u, c.abort, p.status, 115)) break;
     tc_fence_after();
     if (leader) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) umma_f16(c.tmem + kColS, at(qr, e * 32), at(kr, e * 32), kIdescS, e > 0 ? 1u : 0u);
 #pragma unroll
       for (int e = 0; e < 4; ++e) umma_f16(c.tmem + kColP, at(gr, e * 32), at(vr, e * 32), kIdescS, e > 0 ? 1u : 0u);
-      if (steps == 0) umma_commit(c.bar(kSMain));
     }
-    if (steps == 0 && !warp_wait(c.bar(kTFree), par ^ 1u, c.abort, p.status, 129)) break;
+    int steps = 0;
+    if constexpr (kMask == kGroups) {
+      if (!warp_wait(c.bar(kInfo), par, c.abort, p.status, 135)) break;
+      tc_fence_after();
+      steps = c.steps[i & 1];
+    }
+    const bool together = steps > kMaskSlots;  // the operands come in rounds: both blocks take each
+    if (leader && !together) {
+      for (int st = 0; st < steps; ++st) {
+        const uint64_t a = at(mask0, st * kMaskOpBytes);
+        umma_f16(c.tmem + kColS, a, at(a, kRow32), kIdescS, 1u);
+      }
+      umma_commit(c.bar(kSMain));
+    }
+    if (!warp_wait(c.bar(kTFree), par ^ 1u, c.abort, p.status, 129)) break;
     tc_fence_after();
     if (leader) {
 #pragma unroll
@@ -993,42 +1024,57 @@ __device__ __forceinline__ void issuer(const Params& p, const Ctx& c) {
           tc_fence_after();
         }
         if (leader) {
-          const uint64_t a = at(mask0, (st % kMaskSlots) * kMaskOpBytes), b = at(a, kRow32);
-          umma_f16(c.tmem + kColS, a, b, kIdescS, 1u);
-          umma_f16(c.tmem + kColS2, at(a, kRemOff32), b, kIdescS2, 1u);
+          const uint64_t a = at(mask0, (st % kMaskSlots) * kMaskOpBytes), bb = at(a, kRow32);
+          if (together) umma_f16(c.tmem + kColS, a, bb, kIdescS, 1u);
+          umma_f16(c.tmem + kColS2, at(a, kRemOff32), bb, kIdescS2, 1u);
         }
       }
       if (!ok) break;
     }
     if (leader) {
-      if (steps > 0) umma_commit(c.bar(kSMain));
+      if (together) umma_commit(c.bar(kSMain));
       umma_commit(c.bar(kSRem));
     }
-    if (!warp_wait(c.bar(kPFull), par, c.abort, p.status, 130)) break;
+    // dV: queries 16e .. 16e + 15 at step e; those of warps 2 and 3 are the last step.
+    auto dv_step = [&](int e) {
+      umma_f16(c.tmem + kColDv, at(pT, e * 2048), at(gc, e * 2048), kIdescT, e > 0 ? 1u : 0u);
+      umma_f16(c.tmem + kColRem, at(gc, e * 2048), at(p32, e * 512), kIdescRemT, e > 0 ? 1u : 0u);
+    };
+    if (!warp_wait(c.bar(kPMain), par, c.abort, p.status, 130)) break;
     tc_fence_after();
     if (leader) {
 #pragma unroll
-      for (int e = 0; e < 9; ++e) {  // queries 16e .. 16e + 15
-        umma_f16(c.tmem + kColDv, at(pT, e * 2048), at(gc, e * 2048), kIdescT, e > 0 ? 1u : 0u);
-        umma_f16(c.tmem + kColRem, at(gc, e * 2048), at(p32, e * 512), kIdescRemT, e > 0 ? 1u : 0u);
-      }
+      for (int e = 0; e < 8; ++e) dv_step(e);
+    }
+    if (!warp_wait(c.bar(kPRem), par, c.abort, p.status, 117)) break;
+    tc_fence_after();
+    if (leader) {
+      dv_step(8);
       umma_commit(c.bar(kDvFull));
     }
-    if (!warp_wait(c.bar(kDsFull), par, c.abort, p.status, 131)) break;
+    // dQ of rows 0..127 needs only their dS; the transposed remainders and dK need all.
+    if (!warp_wait(c.bar(kDsMain), par, c.abort, p.status, 131)) break;
     tc_fence_after();
     if (leader) {
 #pragma unroll
-      for (int e = 0; e < 9; ++e) {  // keys 16e .. 16e + 15
-        const uint64_t a = e < 8 ? at(ds, (e >> 2) * kPChunk + (e & 3) * 32) : ds32;
-        umma_f16(c.tmem + kColDq, a, at(kc, e * 2048), kIdescO, e > 0 ? 1u : 0u);
-        umma_f16(c.tmem + kColDq2, at(kc, e * 2048), at(a, e < 8 ? 128 * 128 : 128 * 32), kIdescRemQ, e > 0 ? 1u : 0u);
-      }
+      for (int e = 0; e < 9; ++e)  // keys 16e .. 16e + 15
+        umma_f16(c.tmem + kColDq, e < 8 ? at(ds, (e >> 2) * kPChunk + (e & 3) * 32) : ds32, at(kc, e * 2048), kIdescO,
+                 e > 0 ? 1u : 0u);
       umma_commit(c.bar(kDqFull));
+    }
+    if (!warp_wait(c.bar(kDsRem), par, c.abort, p.status, 116)) break;
+    tc_fence_after();
+    if (leader) {
 #pragma unroll
       for (int e = 0; e < 9; ++e) {
-        umma_f16(c.tmem + kColDk, at(dsT, e * 2048), at(qc, e * 2048), kIdescT, e > 0 ? 1u : 0u);
+        umma_f16(c.tmem + kColDq2, at(kc, e * 2048),
+                 e < 8 ? at(ds, (e >> 2) * kPChunk + (e & 3) * 32 + 128 * 128) : at(ds32, 128 * 32), kIdescRemQ, e > 0 ? 1u : 0u);
         umma_f16(c.tmem + kColRem + kLaneHalf, at(qc, e * 2048), at(ds32, e * 512), kIdescRemT, e > 0 ? 1u : 0u);
       }
+      umma_commit(c.bar(kRemFull));
+#pragma unroll
+      for (int e = 0; e < 9; ++e)
+        umma_f16(c.tmem + kColDk, at(dsT, e * 2048), at(qc, e * 2048), kIdescT, e > 0 ? 1u : 0u);
       umma_commit(c.bar(kDkFull));
     }
   }
@@ -1063,8 +1109,8 @@ rel_bias_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_con
   if (threadIdx.x == 0) {
     *words = 0;
     for (int b = 0; b < kNumBars; ++b) {
-      const bool main = b == kStaged || b == kStaged + 1 || b == kTFree, all = b == kPFull || b == kDsFull;
-      mbar_init(c.bar(b), main ? 8 : all ? 10 : 1);
+      const bool main = b == kStaged || b == kStaged + 1 || b == kTFree || b == kDqFree || b == kPMain || b == kDsMain;
+      mbar_init(c.bar(b), main ? 8 : b == kPRem || b == kDsRem ? 2 : 1);
     }
     fence_mbarrier_init();
   }
