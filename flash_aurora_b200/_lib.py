@@ -68,7 +68,7 @@ SIGNATURES = {
                                              _u32, _vp]),
     "fa_window_attention_bias_noalloc": (_i32, [_i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64p, _vp,
                                                  _i64, _f32, _vp]),
-    "fa_window_attention_rel_bias_state": (_i64, [_i64, _i64]),
+    "fa_window_attention_rel_bias_state": (_i64, [_i32, _i64, _i64]),
     "fa_window_attention_rel_bias_workspace": (_i64, [_i64, _i64, _i64]),
     "fa_window_attention_rel_bias": (_i32, [_i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64p, _vp, _i32, _vp,
                                             _u8p, _u8p, _i64, _f32, _vp, _vp, _vp]),

@@ -71,145 +71,25 @@ __device__ __forceinline__ void rank_window(const uint8_t* ids, int N, int lane,
 }
 
 __global__ void __launch_bounds__(kExpandThreads)
-expand_bias_kernel(const void* table, int bf16, const int32_t* index, int H, int N, float4* out, const uint8_t* ids,
-                   int64_t nW, uint8_t* ranks) {
-  if ((int64_t)blockIdx.x >= (int64_t)H * kExpandBlocks) {
-    const int64_t w = ((int64_t)blockIdx.x - (int64_t)H * kExpandBlocks) * (kExpandThreads / 32) + (threadIdx.x >> 5);
+expand_bias_kernel(const void* table, int bf16, const int32_t* index, int H, int copies, int N, float4* out,
+                   const uint8_t* ids, int64_t nW, uint8_t* ranks) {
+  if ((int64_t)blockIdx.x >= (int64_t)copies * H * kExpandBlocks) {
+    const int64_t w = ((int64_t)blockIdx.x - (int64_t)copies * H * kExpandBlocks) * (kExpandThreads / 32) + (threadIdx.x >> 5);
     if (w < nW) rank_window(ids + w * N, N, threadIdx.x & 31, ranks + w * kMaxN);
     return;
   }
-  const int h = blockIdx.x / kExpandBlocks, e = (blockIdx.x % kExpandBlocks) * kExpandThreads + threadIdx.x;
+  const int hc = blockIdx.x / kExpandBlocks, e = (blockIdx.x % kExpandBlocks) * kExpandThreads + threadIdx.x;
   const int lane = e & 31, j = (e >> 5) % 18, blk = (e >> 5) / 18;
   const int i = 16 * blk + (lane >> 2), k = 8 * j + 2 * (lane & 3);
-  out[(int64_t)h * kBiasVecs + e] = make_float4(bias_log2(table, bf16, index, H, N, h, i, k),
-                                                bias_log2(table, bf16, index, H, N, h, i, k + 1),
-                                                bias_log2(table, bf16, index, H, N, h, i + 8, k),
-                                                bias_log2(table, bf16, index, H, N, h, i + 8, k + 1));
-}
-
-__device__ __forceinline__ float bias_at(const Params& p, int h, int i, int j) {
-  const int lane = ((i & 7) << 2) | ((j & 7) >> 1);
-  const float* f = reinterpret_cast<const float*>(bias_rows(p, h, i & ~15, lane) + (j >> 3) * 32);
-  return __ldg(f + ((i & 8) >> 2) + (j & 1));
-}
-
-constexpr int kThreads = 160;  // one thread per query row, then one per key row
-
-template <typename T>
-__device__ __forceinline__ void load_rows(float (*dst)[64], const void* src, const int64_t* st, int w, int h, int N) {
-  const T* base = reinterpret_cast<const T*>(src) + w * st[0] + h * st[1];
-  for (int e = threadIdx.x; e < N * 64; e += kThreads) dst[e >> 6][e & 63] = to_f32(base[(e >> 6) * st[2] + (e & 63)]);
-}
-
-__device__ __forceinline__ float dot64(const float* a, const float* b) {
-  float s = 0.f;
+  const bool transposed = hc >= H;  // rows are keys
+  const int h = transposed ? hc - H : hc;
+  float v[4];
 #pragma unroll
-  for (int d = 0; d < 64; ++d) s = fmaf(a[d], b[d], s);
-  return s;
-}
-
-template <int kMask>
-__device__ __forceinline__ float logit_log2(const Params& p, int h, int w, int i, int j, float s) {
-  float x = fmaf(s, p.scale_log2, bias_at(p, h, i, j));
-  const int64_t mw = w % p.nW;
-  if (kMask == kGroups && __ldg(p.mask + mw * p.N + i) != __ldg(p.mask + mw * p.N + j)) x += kMaskedLog2;
-  if (kMask == kMaskU8 && __ldg(p.mask + (mw * p.N + i) * p.N + j)) x += kMaskedLog2;
-  return x;
-}
-
-// One thread per query row: two passes over the keys (maximum, then sum and P v).
-template <typename T, int kMask>
-__global__ void __launch_bounds__(kThreads) rel_bias_fwd_kernel(const Params p) {
-  extern __shared__ float sm[];
-  auto sK = reinterpret_cast<float(*)[64]>(sm);
-  auto sV = sK + kMaxN;
-  const int i = threadIdx.x, t_end = tile_end(p.num_tiles);
-  for (int t = tile_begin(p.num_tiles); t < t_end; ++t) {
-    const int h = t / p.Bwin, w = t - h * p.Bwin;
-    __syncthreads();
-    load_rows<T>(sK, p.k, p.sk, w, h, p.N);
-    load_rows<T>(sV, p.v, p.sv, w, h, p.N);
-    __syncthreads();
-    if (i >= p.N) continue;
-    float q[64], o[64];
-    const T* qr = reinterpret_cast<const T*>(p.q) + w * p.sq[0] + h * p.sq[1] + i * p.sq[2];
-    for (int d = 0; d < 64; ++d) {
-      q[d] = to_f32(qr[d]);
-      o[d] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < p.N; ++j) m = fmaxf(m, logit_log2<kMask>(p, h, w, i, j, dot64(q, sK[j])));
-    for (int j = 0; j < p.N; ++j) {
-      const float e = exp2f(logit_log2<kMask>(p, h, w, i, j, dot64(q, sK[j])) - m);
-      l += e;
-      for (int d = 0; d < 64; ++d) o[d] = fmaf(e, sV[j][d], o[d]);
-    }
-    T* orow = reinterpret_cast<T*>(p.out) + w * p.so[0] + h * p.so[1] + i * p.so[2];
-    for (int d = 0; d < 64; ++d) orow[d] = from_f32<T>(o[d] / l);
-    if (p.stats) p.stats[((int64_t)w * p.H + h) * kMaxN + i] = make_float2(m, log2f(l));
+  for (int c = 0; c < 4; ++c) {
+    const int row = i + 8 * (c >> 1), col = k + (c & 1);
+    v[c] = transposed ? bias_log2(table, bf16, index, H, N, h, col, row) : bias_log2(table, bf16, index, H, N, h, row, col);
   }
-}
-
-// One thread per query row for dQ and the bias gradient, then one per key row for dK and dV.
-template <typename T, int kMask>
-__global__ void __launch_bounds__(kThreads) rel_bias_bwd_kernel(const Params p) {
-  extern __shared__ float sm[];
-  auto sQ = reinterpret_cast<float(*)[64]>(sm);
-  auto sK = sQ + kMaxN;
-  auto sV = sK + kMaxN;
-  auto sG = sV + kMaxN;
-  float2* sStat = reinterpret_cast<float2*>(sG + kMaxN);
-  float* sDelta = reinterpret_cast<float*>(sStat + kMaxN);
-  const int i = threadIdx.x, t_begin = tile_begin(p.num_tiles), t_end = tile_end(p.num_tiles);
-  for (int t = t_begin; t < t_end; ++t) {
-    const int h = t / p.Bwin, w = t - h * p.Bwin;
-    const bool first = t == t_begin || w == 0;  // first window of this head in this block
-    float* slot = p.slots + (int64_t)(blockIdx.x + h) * p.N * p.N;
-    __syncthreads();
-    load_rows<T>(sQ, p.q, p.sq, w, h, p.N);
-    load_rows<T>(sK, p.k, p.sk, w, h, p.N);
-    load_rows<T>(sV, p.v, p.sv, w, h, p.N);
-    load_rows<T>(sG, p.dout, p.so, w, h, p.N);
-    if (i < p.N) sStat[i] = p.stats[((int64_t)w * p.H + h) * kMaxN + i];
-    __syncthreads();
-    if (i < p.N) {
-      float acc[64];
-      float delta = 0.f;
-      for (int d = 0; d < 64; ++d) acc[d] = 0.f;
-      const float2 st = sStat[i];
-      for (int j = 0; j < p.N; ++j)
-        delta += exp2f(logit_log2<kMask>(p, h, w, i, j, dot64(sQ[i], sK[j])) - st.x - st.y) * dot64(sG[i], sV[j]);
-      for (int j = 0; j < p.N; ++j) {
-        const float e = exp2f(logit_log2<kMask>(p, h, w, i, j, dot64(sQ[i], sK[j])) - st.x - st.y);
-        const float ds = e * (dot64(sG[i], sV[j]) - delta);
-        if (p.slots) slot[i * p.N + j] = first ? ds : slot[i * p.N + j] + ds;
-        for (int d = 0; d < 64; ++d) acc[d] = fmaf(ds, sK[j][d], acc[d]);
-      }
-      sDelta[i] = delta;
-      T* row = reinterpret_cast<T*>(p.dq) + w * p.sdq[0] + h * p.sdq[1] + i * p.sdq[2];
-      for (int d = 0; d < 64; ++d) row[d] = from_f32<T>(acc[d] * p.scale);
-    }
-    __syncthreads();
-    if (i < p.N) {
-      const int j = i;
-      float gk[64], gv[64];
-      for (int d = 0; d < 64; ++d) gk[d] = gv[d] = 0.f;
-      for (int r = 0; r < p.N; ++r) {
-        const float e = exp2f(logit_log2<kMask>(p, h, w, r, j, dot64(sQ[r], sK[j])) - sStat[r].x - sStat[r].y);
-        const float ds = e * (dot64(sG[r], sV[j]) - sDelta[r]);
-        for (int d = 0; d < 64; ++d) {
-          gv[d] = fmaf(e, sG[r][d], gv[d]);
-          gk[d] = fmaf(ds, sQ[r][d], gk[d]);
-        }
-      }
-      T* kr = reinterpret_cast<T*>(p.dk) + w * p.sdk[0] + h * p.sdk[1] + j * p.sdk[2];
-      T* vr = reinterpret_cast<T*>(p.dv) + w * p.sdv[0] + h * p.sdv[1] + j * p.sdv[2];
-      for (int d = 0; d < 64; ++d) {
-        kr[d] = from_f32<T>(gk[d] * p.scale);
-        vr[d] = from_f32<T>(gv[d]);
-      }
-    }
-  }
+  out[(int64_t)hc * kBiasVecs + e] = make_float4(v[0], v[1], v[2], v[3]);
 }
 
 // dT[b, h] = sum over the pairs of bucket b (positions order[offsets[b]] .. in the N x N index) of
@@ -217,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) rel_bias_bwd_kernel(const Params p) 
 constexpr int kReduceThreads = 128;
 __global__ void __launch_bounds__(kReduceThreads)
 bias_grad_kernel(const float* slots, const int32_t* order, const int32_t* offsets, void* dtable, int dtable_bf16, int H,
-                 int NN, int Bwin, int num_tiles, int grid) {
+                 int N, int Bwin, int num_tiles, int grid) {
   const int b = blockIdx.x, h = blockIdx.y;
   // Blocks of the main kernel whose tile range meets [h * Bwin, (h + 1) * Bwin): block c covers
   // [c * T / G, (c + 1) * T / G).
@@ -231,8 +111,9 @@ bias_grad_kernel(const float* slots, const int32_t* order, const int32_t* offset
     while (c1 + 1 < grid && (int64_t)(c1 + 1) * num_tiles / grid <= hi - 1) ++c1;
     const int p0 = offsets[b], p1 = offsets[b + 1];
     for (int e = p0 + threadIdx.x; e < p1; e += kReduceThreads) {
-      const int pos = order[e];
-      for (int c = c0; c <= c1; ++c) acc += slots[(int64_t)(c + h) * NN + pos];
+      const int pos = order[e], i = pos / N;
+      const float* f = slots + frag_index(i, pos - i * N);
+      for (int c = c0; c <= c1; ++c) acc += f[(int64_t)(c + h) * (4 * kBiasVecs)];
     }
   }
   __shared__ float warp_acc[kReduceThreads / 32];
@@ -249,23 +130,8 @@ bias_grad_kernel(const float* slots, const int32_t* order, const int32_t* offset
   }
 }
 
-template <typename T, int kMask>
-int launch_fwd(const Params& p, int grid, cudaStream_t s) {
-  auto kern = rel_bias_fwd_kernel<T, kMask>;
-  constexpr int smem = 2 * kMaxN * 64 * 4;
-  FA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kern<<<grid, kThreads, smem, s>>>(p);
-  return check_launch("rel_bias_fwd_kernel");
-}
-
-template <typename T, int kMask>
-int launch_bwd(const Params& p, int grid, cudaStream_t s) {
-  auto kern = rel_bias_bwd_kernel<T, kMask>;
-  constexpr int smem = 4 * kMaxN * 64 * 4 + kMaxN * 12;
-  FA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kern<<<grid, kThreads, smem, s>>>(p);
-  return check_launch("rel_bias_bwd_kernel");
-}
+// Bias copies in the state: the fp32 backward pass reads the transposed one too.
+int bias_copies(int precision) { return precision == FA_ATTN_BF16 ? 1 : 2; }
 
 int grid_of(int64_t tiles) { return (int)(tiles < num_sms() ? tiles : num_sms()); }
 
@@ -326,17 +192,18 @@ void copy3(int64_t* dst, const int64_t* src) {
 using namespace fa;
 using namespace fa::relb;
 
-extern "C" int64_t fa_window_attention_rel_bias_state(int64_t H, int64_t nW_ids) {
-  if (H < 1 || H >= ((int64_t)1 << 31) || nW_ids < 0 || nW_ids >= ((int64_t)1 << 31))
+extern "C" int64_t fa_window_attention_rel_bias_state(int precision, int64_t H, int64_t nW_ids) {
+  if ((precision != FA_ATTN_BF16 && precision != FA_ATTN_FP32_3XTF32) || H < 1 || H >= ((int64_t)1 << 31) || nW_ids < 0 ||
+      nW_ids >= ((int64_t)1 << 31))
     return set_error(FA_ERR_INVALID, "invalid attention shape");
-  return H * kBiasVecs * 16 + nW_ids * kMaxN;
+  return bias_copies(precision) * H * kBiasVecs * 16 + nW_ids * kMaxN;
 }
 
 extern "C" int64_t fa_window_attention_rel_bias_workspace(int64_t Bwin, int64_t H, int64_t N) {
   if (Bwin < 0 || H < 1 || N < 1 || N > kMaxN || Bwin >= ((int64_t)1 << 31) || H >= ((int64_t)1 << 31) ||
       Bwin * H >= ((int64_t)1 << 31))
     return set_error(FA_ERR_INVALID, "invalid attention shape");
-  return (grid_of(Bwin * H) + H) * N * N * 4;
+  return (grid_of(Bwin * H) + H) * kBiasVecs * 16;
 }
 
 extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh,
@@ -358,25 +225,23 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
   p.q = q; p.k = k; p.v = v; p.out = out;
   copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
   p.bias = reinterpret_cast<const float4*>(state);
-  p.ranks = reinterpret_cast<const uint8_t*>(p.bias + H * kBiasVecs);
+  p.ranks = reinterpret_cast<const uint8_t*>(p.bias + bias_copies(precision) * H * kBiasVecs);
   p.mask = mask_u8 ? mask_u8 : group_ids;
   if (group_ids) split_mask_value(scale, &p.mask_a, &p.mask_b);
   p.stats = reinterpret_cast<float2*>(stats);
   cudaStream_t s = (cudaStream_t)stream;
-  const int64_t blocks = H * kExpandBlocks + (group_ids ? (nW + kExpandThreads / 32 - 1) / (kExpandThreads / 32) : 0);
+  const int copies = bias_copies(precision);
+  const int64_t blocks = copies * H * kExpandBlocks + (group_ids ? (nW + kExpandThreads / 32 - 1) / (kExpandThreads / 32) : 0);
   FA_REQUIRE(blocks < ((int64_t)1 << 31), FA_ERR_INVALID, "too many heads or mask windows");
-  expand_bias_kernel<<<(unsigned)blocks, kExpandThreads, 0, s>>>(table, table_dtype == FA_BF16, index, p.H, p.N,
+  expand_bias_kernel<<<(unsigned)blocks, kExpandThreads, 0, s>>>(table, table_dtype == FA_BF16, index, p.H, copies, p.N,
                                                                 reinterpret_cast<float4*>(state), group_ids,
                                                                 group_ids ? nW : 0, const_cast<uint8_t*>(p.ranks));
   if ((rc = check_launch("expand_bias_kernel")) != FA_OK) return rc;
   const int grid = grid_of(p.num_tiles);
   p.status = attn::status_ptr();
   FA_REQUIRE(p.status, FA_ERR_CUDA, "cannot resolve the attention status word");
-  if (precision == FA_ATTN_BF16)
-    return run_bf16_forward(p, mask_u8 ? kMaskU8 : group_ids ? kGroups : kNoMask, grid, s);
-  if (mask_u8) return launch_fwd<float, kMaskU8>(p, grid, s);
-  if (group_ids) return launch_fwd<float, kGroups>(p, grid, s);
-  return launch_fwd<float, kNoMask>(p, grid, s);
+  const int kind = mask_u8 ? kMaskU8 : group_ids ? kGroups : kNoMask;
+  return precision == FA_ATTN_BF16 ? run_bf16_forward(p, kind, grid, s) : run_f32_forward(p, kind, s);
 }
 
 extern "C" int fa_window_attention_rel_bias_backward(
@@ -408,25 +273,20 @@ extern "C" int fa_window_attention_rel_bias_backward(
     copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
     copy3(p.sdq, strides + 12); copy3(p.sdk, strides + 15); copy3(p.sdv, strides + 18);
     p.bias = reinterpret_cast<const float4*>(state);
-  p.ranks = reinterpret_cast<const uint8_t*>(p.bias + H * kBiasVecs);
+  p.ranks = reinterpret_cast<const uint8_t*>(p.bias + bias_copies(precision) * H * kBiasVecs);
     p.mask = mask_u8 ? mask_u8 : group_ids;
   if (group_ids) split_mask_value(scale, &p.mask_a, &p.mask_b);
     p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats));
     p.slots = dtable ? reinterpret_cast<float*>(workspace) : nullptr;
     p.status = attn::status_ptr();
     FA_REQUIRE(p.status, FA_ERR_CUDA, "cannot resolve the attention status word");
-    if (precision == FA_ATTN_BF16) {
-      rc = run_bf16_backward(p, mask_u8 ? kMaskU8 : group_ids ? kGroups : kNoMask, grid, s);
-    } else {
-      rc = mask_u8 ? launch_bwd<float, kMaskU8>(p, grid, s)
-                   : group_ids ? launch_bwd<float, kGroups>(p, grid, s)
-                               : launch_bwd<float, kNoMask>(p, grid, s);
-    }
+    const int kind = mask_u8 ? kMaskU8 : group_ids ? kGroups : kNoMask;
+    rc = precision == FA_ATTN_BF16 ? run_bf16_backward(p, kind, grid, s) : run_f32_backward(p, kind, grid, s);
     if (rc != FA_OK) return rc;
   }
   if (!dtable) return FA_OK;
   bias_grad_kernel<<<dim3((unsigned)num_buckets, (unsigned)H), kReduceThreads, 0, s>>>(
-      reinterpret_cast<const float*>(workspace), order, offsets, dtable, dtable_dtype == FA_BF16, (int)H, (int)(N * N),
+      reinterpret_cast<const float*>(workspace), order, offsets, dtable, dtable_dtype == FA_BF16, (int)H, (int)N,
       (int)Bwin, (int)(Bwin * H), grid);
   return check_launch("bias_grad_kernel");
 }

@@ -27,7 +27,7 @@ struct Params {
   const uint8_t* ranks;      // with region ids: (nW, 144) rank of each token's id in its window, kNoRank past N
   uint32_t mask_a, mask_b;   // bf16 bits: mask_a * mask_b = -100 / scale (region masks, bf16 kernels)
   float2* stats;             // (Bwin, H, 144): row maximum and log2 of the row sum, log2 domain
-  float* slots;              // backward: (gridDim.x + H - 1) partial bias gradients (N, N)
+  float* slots;              // backward: (gridDim.x + H - 1) partial bias gradients in fragment order
   int* status;
 };
 
@@ -46,6 +46,20 @@ constexpr int kBiasVecs = 9 * 18 * 32;  // float4 per head
 __device__ __forceinline__ const float4* bias_rows(const Params& p, int h, int row0, int lane) {
   return p.bias + ((int64_t)h * 9 + (row0 >> 4)) * (18 * 32) + lane;
 }
+
+// The same rows of a partial bias gradient.
+__device__ __forceinline__ float4* slot_rows(const Params& p, int slot, int row0, int lane) {
+  return reinterpret_cast<float4*>(p.slots) + ((int64_t)slot * 9 + (row0 >> 4)) * (18 * 32) + lane;
+}
+// Float index of pair (i, j) in fragment order.
+__device__ __forceinline__ int frag_index(int i, int j) {
+  return (((i >> 4) * 18 + (j >> 3)) * 32 + ((i & 7) << 2 | (j & 7) >> 1)) * 4 + ((i & 8) >> 2 | (j & 1));
+}
+
+// The fp32 kernels (rel_bias_f32.cu). Their backward pass also reads the transposed bias: heads H .. 2H - 1
+// of `bias` hold, in fragment order, the pairs with keys as rows.
+int run_f32_forward(const Params& p, int mask_kind, cudaStream_t s);
+int run_f32_backward(const Params& p, int mask_kind, int grid, cudaStream_t s);
 
 // The bf16 kernels (rel_bias_tc.cu); mask_kind: attn::kNoMask, kGroups or kMaskU8.
 int run_bf16_forward(const Params& p, int mask_kind, int grid, cudaStream_t s);

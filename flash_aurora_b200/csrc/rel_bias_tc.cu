@@ -726,16 +726,11 @@ __device__ __forceinline__ void softmax_warps(const Params& p, const Ctx& c, int
   int cur_h = -1;
   auto flush = [&](int h) {
     if (!p.slots) return;
-    float* slot = p.slots + (int64_t)(blockIdx.x + h) * p.N * p.N;
+    float4* slot = slot_rows(p, blockIdx.x + h, l.row[0], lane);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (l.row[r] >= p.N) continue;
-      float* dst = slot + l.row[r] * p.N + 2 * l.t0;
-#pragma unroll
-      for (int j = 0; j < 18; ++j) {
-        if (8 * j + 2 * l.t0 < p.N) dst[8 * j] = grad[j][r].x;
-        if (8 * j + 2 * l.t0 + 1 < p.N) dst[8 * j + 1] = grad[j][r].y;
-      }
+    for (int j = 0; j < 18; ++j) {
+      if constexpr (kRem) reinterpret_cast<float2*>(slot + j * 32)[l.row[0] >= 136 ? 1 : 0] = grad[j][0];
+      else slot[j * 32] = make_float4(grad[j][0].x, grad[j][0].y, grad[j][1].x, grad[j][1].y);
     }
   };
   int h = c.t_begin / p.Bwin, w = c.t_begin - h * p.Bwin;

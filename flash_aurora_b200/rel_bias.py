@@ -157,7 +157,7 @@ def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool):
     with torch.cuda.device(dev):
         stats = torch.empty(Bwin, H, _MAX_TOKENS, 2, device=dev, dtype=torch.float32) if want_stats else None
         lib = _lib.load()
-        n = lib.fa_window_attention_rel_bias_state(H, call.nW if call.kind == "group_ids" else 0)
+        n = lib.fa_window_attention_rel_bias_state(_precision(q.dtype), H, call.nW if call.kind == "group_ids" else 0)
         if n < 0:
             _lib.check(int(n), "window_attn_rel_bias")
         state = torch.empty(n, dtype=torch.uint8, device=dev)

@@ -286,7 +286,7 @@ int fa_window_attention_bias_noalloc(int precision, int64_t Bwin, int64_t H, int
  * head-dim stride 1, 16-byte aligned, strides multiples of 16 bytes; Dh == 64, 1 <= N <= 144.
  * table (num_buckets, H) contiguous, FA_F32 or FA_BF16; index (N, N) int32, the bucket of (query,
  * key), every value in [0, num_buckets). Masks as in fa_window_attention (region ids of any form).
- * state (fa_window_attention_rel_bias_state(H, nW with region ids, else 0) bytes, 16-byte aligned)
+ * state (fa_window_attention_rel_bias_state(precision, H, nW with region ids, else 0) bytes, 16-byte aligned)
  * receives the expanded bias and mask, stats (nullable, (Bwin, H, 144, 2) fp32, 16-byte aligned) the row
  * statistics; the backward call reads both. scale must be finite, of magnitude 1e-30 to 1e30.
  *
@@ -303,7 +303,7 @@ int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t H, int64_t
                                  const void* table, int table_dtype, const int32_t* index,
                                  const uint8_t* mask_u8, const uint8_t* group_ids, int64_t nW, float scale,
                                  void* state, float* stats, void* stream);
-int64_t fa_window_attention_rel_bias_state(int64_t H, int64_t nW_ids);
+int64_t fa_window_attention_rel_bias_state(int precision, int64_t H, int64_t nW_ids);
 int64_t fa_window_attention_rel_bias_workspace(int64_t Bwin, int64_t H, int64_t N);
 int fa_window_attention_rel_bias_backward(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh,
                                           const void* q, const void* k, const void* v, const void* dout,

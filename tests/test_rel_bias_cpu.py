@@ -120,8 +120,10 @@ def test_abi_refusals_without_a_gpu():
     assert fwd(strides=bad) == _lib.FA_ERR_INVALID and b"16 bytes" in lib.fa_last_error()
     for bad_scale in (0.0, float("nan"), float("inf"), 1e-35):
         assert fwd(scale=bad_scale) == _lib.FA_ERR_INVALID and b"scale" in lib.fa_last_error()
-    assert lib.fa_window_attention_rel_bias_state(3, 5) == 3 * 144 * 144 * 4 + 5 * 144
-    assert lib.fa_window_attention_rel_bias_state(0, 5) == _lib.FA_ERR_INVALID
+    assert lib.fa_window_attention_rel_bias_state(0, 3, 5) == 3 * 144 * 144 * 4 + 5 * 144
+    assert lib.fa_window_attention_rel_bias_state(1, 3, 0) == 2 * 3 * 144 * 144 * 4
+    assert lib.fa_window_attention_rel_bias_state(0, 0, 5) == _lib.FA_ERR_INVALID
+    assert lib.fa_window_attention_rel_bias_state(2, 1, 0) == _lib.FA_ERR_INVALID
     assert fwd(bias=None) == _lib.FA_ERR_INVALID and b"state buffer" in lib.fa_last_error()
     assert fwd(B=0, q=None) == _lib.FA_OK
 
