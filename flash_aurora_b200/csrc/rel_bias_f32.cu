@@ -7,14 +7,14 @@
 // pass would have to transpose, split and store five operands a tile; at three products a term both
 // paths are bound by their products, not by memory.
 //
-// A block holds a tile's operands in shared memory (144 x 64 fp32, 16-byte chunks XORed with the row: all
-// fragment reads are free of bank conflicts) and each of its 9 warps owns 16 rows.
-//   forward   48 keys at a time: S, online softmax, O; two blocks per SM, so that one loads while the other works.
+// A block holds a tile's operands in shared memory (144 rows of 68 floats: every fragment read hits 32
+// banks at a constant offset from one lane address) and each of its 9 warps owns 16 rows.
+//   forward   S, online softmax, O.
 //   backward  queries by rows: S, dP, delta, dS, dQ and the bias gradient (one partial per block and head in
-//             global memory, read and written in fragment order); then keys by rows: S^T and dP^T
-//             again, from which P^T and dS^T are at hand as A operands of dV = P^T dO and dK = dS^T Q. The two
-//             products computed again cost 2 of 7 and save 83 KB of shared memory for P and dS, and all
-//             exchange between warps but delta.
+//             global memory, read and written in fragment order); keys by rows: S^T and dP^T again, from which
+//             P^T and dS^T are at hand as A operands of dV = P^T dO and dK = dS^T Q. The two products computed
+//             again cost 2 of 7 and save 83 KB of shared memory for P and dS, and all exchange between warps
+//             but delta.
 #include "ptx.cuh"
 #include "rel_bias.cuh"
 
@@ -30,77 +30,94 @@ using attn::kMaxN;
 using attn::kNoMask;
 
 constexpr int kThreads = 32 * kMaxN / 16;
-constexpr int kTile = kMaxN * 64;  // floats
-
-// Shared-memory float index of (row, d).
-__device__ __forceinline__ int at(int row, int d) { return row * 64 + (d ^ ((row & 7) << 2)); }
+constexpr int kLd = 68;            // floats per row: fragment reads, 4 or 8 rows apart, hit 32 banks
+constexpr int kTile = kMaxN * kLd;  // floats
 
 // Rows 0..N-1 of a (token, 64) operand into shared memory.
 __device__ __forceinline__ void load_tile(float* dst, const void* src, const int64_t* st, int w, int h, int N) {
   const float* base = reinterpret_cast<const float*>(src) + w * st[0] + h * st[1];
   for (int e = threadIdx.x; e < N * 16; e += kThreads) {
     const int row = e >> 4, c = e & 15;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + row * 64 + ((c ^ (row & 7)) << 2))),
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + row * kLd + c * 4)),
                  "l"(base + row * st[2] + c * 4)
                  : "memory");
   }
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// x = hi + lo with hi rounded to tf32 (half away from zero) by integer arithmetic: the cvt that rounds to
+// tf32 issues at a quarter of this rate and bound these kernels. lo gets half a step added, since the tensor
+// core drops the bits that tf32 lacks.
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
+}
+
 // A 16 x 8 A operand, split.
 struct FragA {
   uint32_t h[4], l[4];
-  // Rows r0 .. r0 + 15, columns d0 .. d0 + 7 of a tile.
-  __device__ __forceinline__ void load(const float* t, int r0, int d0, int g, int q) {
-    split_tf32(t[at(r0 + g, d0 + q)], h[0], l[0]);
-    split_tf32(t[at(r0 + g + 8, d0 + q)], h[1], l[1]);
-    split_tf32(t[at(r0 + g, d0 + q + 4)], h[2], l[2]);
-    split_tf32(t[at(r0 + g + 8, d0 + q + 4)], h[3], l[3]);
+  // Rows g and g + 8, columns q and q + 4 of the 16 x 8 block whose element (g, q) is at t.
+  __device__ __forceinline__ void load(const float* t) {
+    split(t[0], h[0], l[0]);
+    split(t[8 * kLd], h[1], l[1]);
+    split(t[4], h[2], l[2]);
+    split(t[8 * kLd + 4], h[3], l[3]);
   }
   // An accumulator block (16 rows x 8) as the operand: its columns in the order 0, 2, 4, 6, 1, 3, 5, 7, which
-  // b_cols() follows.
+  // acc_by_cols() follows.
   __device__ __forceinline__ void take(const float (&c)[4]) {
-    split_tf32(c[0], h[0], l[0]);
-    split_tf32(c[2], h[1], l[1]);
-    split_tf32(c[1], h[2], l[2]);
-    split_tf32(c[3], h[3], l[3]);
+    split(c[0], h[0], l[0]);
+    split(c[2], h[1], l[1]);
+    split(c[1], h[2], l[2]);
+    split(c[3], h[3], l[3]);
   }
 };
 
-__device__ __forceinline__ void mma3(float (&c)[4], const FragA& a, float b0, float b1) {
-  uint32_t h0, l0, h1, l1;
-  split_tf32(b0, h0, l0);
-  split_tf32(b1, h1, l1);
-  mma_tf32_1688(c, a.l[0], a.l[1], a.l[2], a.l[3], h0, h1);
-  mma_tf32_1688(c, a.h[0], a.h[1], a.h[2], a.h[3], l0, l1);
-  mma_tf32_1688(c, a.h[0], a.h[1], a.h[2], a.h[3], h0, h1);
+// d = a b + c. Not volatile: the compiler interleaves independent products, whose latency is 24 cycles.
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1,
+                                         float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// c (16 rows r0.. of x) x (8 kJ rows n0.. of y) = x y^T over the 64 columns.
+// c += a b, 8 columns deep. The three products are summed from zero and added to c in fp32: the tensor core
+// truncates its accumulator at every product, which over the 24 products of a 64-long sum left errors of 1e-6.
+__device__ __forceinline__ void mma3(float (&c)[4], const FragA& a, float b0, float b1) {
+  uint32_t h0, l0, h1, l1;
+  split(b0, h0, l0);
+  split(b1, h1, l1);
+  float d[4];
+  mma_tf32(d, a.l, h0, h1, 0.f, 0.f, 0.f, 0.f);
+  mma_tf32(d, a.h, l0, l1, d[0], d[1], d[2], d[3]);
+  mma_tf32(d, a.h, h0, h1, d[0], d[1], d[2], d[3]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] += d[e];
+}
+
+// c (16 x 8 kJ) = x y^T over 64 columns; x: element (g, q) of the 16 rows, y: of the first of the 8 kJ rows.
 template <int kJ>
-__device__ __forceinline__ void rows_by_rows(float (&c)[kJ][4], const float* x, int r0, const float* y, int n0, int g, int q) {
+__device__ __forceinline__ void rows_by_rows(float (&c)[kJ][4], const float* x, const float* y) {
 #pragma unroll
   for (int j = 0; j < kJ; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
 #pragma unroll 2
   for (int k = 0; k < 8; ++k) {
     FragA a;
-    a.load(x, r0, 8 * k, g, q);
+    a.load(x + 8 * k);
 #pragma unroll
-    for (int j = 0; j < kJ; ++j)
-      mma3(c[j], a, y[at(n0 + 8 * j + g, 8 * k + q)], y[at(n0 + 8 * j + g, 8 * k + q + 4)]);
+    for (int j = 0; j < kJ; ++j) mma3(c[j], a, y[8 * j * kLd + 8 * k], y[8 * j * kLd + 8 * k + 4]);
   }
 }
 
-// o (16 x 64) += c (16 x 8 kJ, an accumulator) times rows n0 .. of y.
+// o (16 x 64) += c (16 x 8 kJ, an accumulator) times 8 kJ rows of 64; y: element (2 q, g) of the first.
 template <int kJ>
-__device__ __forceinline__ void acc_by_cols(float (&o)[8][4], const float (&c)[kJ][4], const float* y, int n0, int g, int q) {
+__device__ __forceinline__ void acc_by_cols(float (&o)[8][4], const float (&c)[kJ][4], const float* y) {
 #pragma unroll
   for (int j = 0; j < kJ; ++j) {
     FragA a;
     a.take(c[j]);
-    const int r = n0 + 8 * j + 2 * q;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) mma3(o[d], a, y[at(r, 8 * d + g)], y[at(r + 1, 8 * d + g)]);
+    for (int d = 0; d < 8; ++d) mma3(o[d], a, y[8 * j * kLd + 8 * d], y[(8 * j + 1) * kLd + 8 * d]);
   }
 }
 
@@ -168,10 +185,11 @@ constexpr int kFwdSmem = 3 * kTile * 4;
 constexpr int kChunk = 6;  // 8-key blocks at a time
 
 template <int kMask>
-__global__ void __launch_bounds__(kThreads, 2) rel_bias_fwd_f32_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 1) rel_bias_fwd_f32_kernel(const Params p) {
   extern __shared__ __align__(16) float sm[];
   float *sQ = sm, *sK = sm + kTile, *sV = sm + 2 * kTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, r0 = 16 * warp;
+  const int rc = g * kLd + q, cr = 2 * q * kLd + g;  // lane offsets of the two kinds of fragment
   for (int e = threadIdx.x; e < 3 * kTile; e += kThreads) sm[e] = 0.f;  // rows past N stay zero
   __syncthreads();
   const int t_end = tile_end(p.num_tiles);
@@ -192,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 2) rel_bias_fwd_f32_kernel(const Par
 #pragma unroll 1
       for (int n0 = 0; n0 < p.N; n0 += 8 * kChunk) {
         float c[kChunk][4];
-        rows_by_rows<kChunk>(c, sQ, r0, sK, n0, g, q);
+        rows_by_rows<kChunk>(c, sQ + r0 * kLd + rc, sK + n0 * kLd + rc);
         logits<kMask, false, kChunk>(c, bias, p.scale_log2, mask, r0, n0, g, q);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -216,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 2) rel_bias_fwd_f32_kernel(const Par
             l[i] += c[j][2 * i] + c[j][2 * i + 1];
           }
         }
-        acc_by_cols<kChunk>(o, c, sV, n0, g, q);
+        acc_by_cols<kChunk>(o, c, sV + n0 * kLd + cr);
       }
       const float la = quad_sum(l[0]), lb = quad_sum(l[1]);
       store_rows(p.out, p.so, w, h, p.N, r0, g, q, o, 1.f / la, 1.f / lb);
@@ -239,6 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) rel_bias_bwd_f32_kernel(const Par
   float *sQ = sm, *sK = sm + kTile, *sV = sm + 2 * kTile, *sG = sm + 3 * kTile;
   float *sMax = sm + 4 * kTile, *sLog = sMax + kMaxN, *sDelta = sLog + kMaxN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, r0 = 16 * warp;
+  const int rc = g * kLd + q, cr = 2 * q * kLd + g;  // lane offsets of the two kinds of fragment
   for (int e = threadIdx.x; e < 4 * kTile; e += kThreads) sm[e] = 0.f;  // rows past N stay zero
   __syncthreads();
   const int t_begin = tile_begin(p.num_tiles), t_end = tile_end(p.num_tiles);
@@ -260,27 +279,27 @@ __global__ void __launch_bounds__(kThreads, 1) rel_bias_bwd_f32_kernel(const Par
     if (r0 < p.N) {
       // Queries by rows.
       float c[18][4], d[18][4];
-      rows_by_rows<18>(c, sQ, r0, sK, 0, g, q);
+      rows_by_rows<18>(c, sQ + r0 * kLd + rc, sK + rc);
       logits<kMask, false, 18>(c, bias_rows(p, h, r0, lane), p.scale_log2, mask, r0, 0, g, q);
-      rows_by_rows<18>(d, sG, r0, sV, 0, g, q);
-      float delta[2] = {0.f, 0.f};
+      rows_by_rows<18>(d, sG + r0 * kLd + rc, sV + rc);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float mx = sMax[r0 + g + 8 * i], lg = sLog[r0 + g + 8 * i];
+        float delta = 0.f;
 #pragma unroll
         for (int j = 0; j < 18; ++j)
 #pragma unroll
           for (int e = 2 * i; e < 2 * i + 2; ++e) {
             c[j][e] = exp2f(c[j][e] + mx + lg);
-            delta[i] = fmaf(c[j][e], d[j][e], delta[i]);
+            delta = fmaf(c[j][e], d[j][e], delta);
           }
-        delta[i] = quad_sum(delta[i]);
-        if (q == 0) sDelta[r0 + g + 8 * i] = delta[i];
+        delta = quad_sum(delta);
+        if (q == 0) sDelta[r0 + g + 8 * i] = delta;
+#pragma unroll
+        for (int j = 0; j < 18; ++j)
+#pragma unroll
+          for (int e = 2 * i; e < 2 * i + 2; ++e) c[j][e] *= d[j][e] - delta;  // dS
       }
-#pragma unroll
-      for (int j = 0; j < 18; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[j][e] *= d[j][e] - delta[e >> 1];  // dS
       if (p.slots) {
         float4* slot = slot_rows(p, blockIdx.x + h, r0, lane);
         const bool first = t == t_begin || w == 0;  // of this head in this block
@@ -297,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) rel_bias_bwd_f32_kernel(const Par
       float o[8][4];
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
-      acc_by_cols<18>(o, c, sK, 0, g, q);
+      acc_by_cols<18>(o, c, sK + cr);
       store_rows(p.dq, p.sdq, w, h, p.N, r0, g, q, o, p.scale, p.scale);
     }
     __syncthreads();
@@ -309,28 +328,28 @@ __global__ void __launch_bounds__(kThreads, 1) rel_bias_bwd_f32_kernel(const Par
         gv[e][0] = gv[e][1] = gv[e][2] = gv[e][3] = 0.f;
         gk[e][0] = gk[e][1] = gk[e][2] = gk[e][3] = 0.f;
       }
+      const float4* bias = bias_rows(p, p.H + h, r0, lane);
 #pragma unroll 1
       for (int n0 = 0; n0 < p.N; n0 += 8 * kChunk) {
         float c[kChunk][4], d[kChunk][4];
-        rows_by_rows<kChunk>(c, sK, r0, sQ, n0, g, q);
-        logits<kMask, true, kChunk>(c, bias_rows(p, p.H + h, r0, lane), p.scale_log2, mask, r0, n0, g, q);
-        rows_by_rows<kChunk>(d, sV, r0, sG, n0, g, q);
+        rows_by_rows<kChunk>(c, sK + r0 * kLd + rc, sQ + n0 * kLd + rc);
+        logits<kMask, true, kChunk>(c, bias, p.scale_log2, mask, r0, n0, g, q);
+        rows_by_rows<kChunk>(d, sV + r0 * kLd + rc, sG + n0 * kLd + rc);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int n = n0 + 8 * j + 2 * q + e;
-            const bool in = n < p.N;
-            const float mx = sMax[n], lg = sLog[n], dl = in ? sDelta[n] : 0.f;
+            const int n = n0 + 8 * j + 2 * q + e;  // queries past N: sMax is -inf, so P = dS = 0
+            const float mxn = sMax[n], lgn = sLog[n], dln = n < p.N ? sDelta[n] : 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const float pr = in ? exp2f(c[j][2 * i + e] + mx + lg) : 0.f;
+              const float pr = exp2f(c[j][2 * i + e] + mxn + lgn);
               c[j][2 * i + e] = pr;
-              d[j][2 * i + e] = pr * (d[j][2 * i + e] - dl);
+              d[j][2 * i + e] = pr * (d[j][2 * i + e] - dln);
             }
           }
-        acc_by_cols<kChunk>(gv, c, sG, n0, g, q);
-        acc_by_cols<kChunk>(gk, d, sQ, n0, g, q);
+        acc_by_cols<kChunk>(gv, c, sG + n0 * kLd + cr);
+        acc_by_cols<kChunk>(gk, d, sQ + n0 * kLd + cr);
       }
       store_rows(p.dv, p.sdv, w, h, p.N, r0, g, q, gv, 1.f, 1.f);
       store_rows(p.dk, p.sdk, w, h, p.N, r0, g, q, gk, p.scale, p.scale);
@@ -343,7 +362,7 @@ template <int kMask>
 int launch_fwd(const Params& p, cudaStream_t s) {
   auto kern = rel_bias_fwd_f32_kernel<kMask>;
   FA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdSmem));
-  const int grid = p.num_tiles < 2 * num_sms() ? p.num_tiles : 2 * num_sms();
+  const int grid = p.num_tiles < num_sms() ? p.num_tiles : num_sms();
   kern<<<grid, kThreads, kFwdSmem, s>>>(p);
   return check_launch("rel_bias_fwd_f32_kernel");
 }
