@@ -89,7 +89,8 @@ struct Column {
   }
   // Elements u .. u + 7 of the thread.
   static __device__ __forceinline__ void get8(uint32_t ring, int threads, const T* row, int t, int tpr, int D, bool on, int u,
-                                              float* v) {
+                                              float2* v2) {
+    float v[8];
     if constexpr (!kRing) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -121,6 +122,8 @@ struct Column {
         }
       }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v2[k] = make_float2(v[2 * k], v[2 * k + 1]);
   }
 };
 
@@ -130,10 +133,16 @@ __device__ __forceinline__ void ring_wait() { asm volatile("cp.async.wait_group 
 __device__ __forceinline__ void ring_drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <typename T, bool kVec, int kN>
-__device__ __forceinline__ void store_row(T* row, int t, int tpr, int D, bool on, const float (&v)[kN]) {
+__device__ __forceinline__ void store_row(T* row, int t, int tpr, int D, bool on, const float2 (&v2)[kN]) {
   if (!on) return;
+  float v[2 * kN];
 #pragma unroll
-  for (int u = 0; u < kN; u += 8) {
+  for (int k = 0; k < kN; ++k) {
+    v[2 * k] = v2[k].x;
+    v[2 * k + 1] = v2[k].y;
+  }
+#pragma unroll
+  for (int u = 0; u < 2 * kN; u += 8) {
     if constexpr (kVec) {
       const int c = col_of<true>(t, tpr, u);
       if (c < D) Vec8<T>::store(row + c, &v[u]);
@@ -149,7 +158,8 @@ __device__ __forceinline__ void store_row(T* row, int t, int tpr, int D, bool on
 
 // Columns u .. u+7 of this thread of a parameter row (null: `fill` everywhere).
 template <bool kVec>
-__device__ __forceinline__ void param8(const float* p, int t, int tpr, int D, int u, float add, float fill, float* v) {
+__device__ __forceinline__ void param8(const float* p, int t, int tpr, int D, int u, float add, float fill, float2* v2) {
+  float v[8];
   if (!p) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = fill;
@@ -170,6 +180,8 @@ __device__ __forceinline__ void param8(const float* p, int t, int tpr, int D, in
       v[k] = c < D ? __ldg(p + c) + add : 0.f;
     }
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v2[k] = make_float2(v[2 * k], v[2 * k + 1]);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -197,39 +209,66 @@ __device__ __forceinline__ void group_sum(Group& g, float (&v)[kVals]) {
     g.par ^= 1;
     if ((g.t & 31) == 0) {
 #pragma unroll
-      for (int i = 0; i < kVals; ++i) b[i * warps + (g.t >> 5)] = v[i];
+      for (int i = 0; i < kVals; ++i) b[(g.t >> 5) * kVals + i] = v[i];
     }
     asm volatile("bar.sync %0, %1;" ::"r"(g.id + 1), "r"(g.tpr) : "memory");
-#pragma unroll
-    for (int i = 0; i < kVals; ++i) {
-      float s = 0.f;
-      for (int w = 0; w < warps; ++w) s += b[i * warps + w];
-      v[i] = s;
+    // Two partial sums (of one value) or one (of two) per 8-byte read, in the same order for every thread.
+    const float2* b2 = reinterpret_cast<const float2*>(b);
+    float2 s = b2[0];
+    const int reads = warps * kVals / 2;
+    for (int w = 1; w < reads; ++w) {
+      const float2 e = b2[w];
+      s.x += e.x;
+      s.y += e.y;
+    }
+    if constexpr (kVals == 1) {
+      v[0] = s.x + s.y;
+    } else {
+      v[0] = s.x;
+      v[1] = s.y;
     }
   }
 }
 
-// Mean and 1 / deviation of a row held by a group; v becomes the normalised row.
-template <bool kVec, int kN>
-__device__ __forceinline__ float2 normalise(Group& g, const NormArgs& a, float (&v)[kN]) {
+__device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float total(float2 v) { return v.x + v.y; }
+
+// 1 for the pair (2 k, 2 k + 1) of this thread's columns that lie in the row, 0 for the others. Vector
+// rows are in or out 8 columns at a time.
+template <bool kVec>
+__device__ __forceinline__ float2 in_row(const Group& g, int D, int k) {
+  if constexpr (kVec) return dup(col_of<true>(g.t, g.tpr, 2 * k & ~7) < D ? 1.f : 0.f);
+  else
+    return make_float2(col_of<false>(g.t, g.tpr, 2 * k) < D ? 1.f : 0.f,
+                       col_of<false>(g.t, g.tpr, 2 * k + 1) < D ? 1.f : 0.f);
+}
+
+// Mean and 1 / deviation of a row held by a group; v becomes the normalised row (0 past D, where it
+// must come in as 0).
+template <bool kVec, int kP>
+__device__ __forceinline__ float2 normalise(Group& g, const NormArgs& a, float2 (&v)[kP]) {
   float s[1] = {0.f};
   float mean = 0.f;
   if (!a.rms) {
+    float2 t = v[0];
 #pragma unroll
-    for (int k = 0; k < kN; ++k) s[0] += v[k];
+    for (int k = 1; k < kP; ++k) t = __fadd2_rn(t, v[k]);
+    s[0] = total(t);
     group_sum<1>(g, s);
     mean = s[0] * a.inv_d;
-  }
-  s[0] = 0.f;
+    const float2 m2 = dup(-mean);
 #pragma unroll
-  for (int k = 0; k < kN; ++k) {
-    v[k] = col_of<kVec>(g.t, g.tpr, k) < a.D ? v[k] - mean : 0.f;
-    s[0] = fmaf(v[k], v[k], s[0]);
+    for (int k = 0; k < kP; ++k) v[k] = __ffma2_rn(in_row<kVec>(g, a.D, k), m2, v[k]);
   }
+  float2 q = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < kP; ++k) q = __ffma2_rn(v[k], v[k], q);
+  s[0] = total(q);
   group_sum<1>(g, s);
   const float rstd = rsqrtf(fmaf(s[0], a.inv_d, a.eps));
+  const float2 r2 = dup(rstd);
 #pragma unroll
-  for (int k = 0; k < kN; ++k) v[k] *= rstd;
+  for (int k = 0; k < kP; ++k) v[k] = __fmul2_rn(v[k], r2);
   return make_float2(mean, rstd);
 }
 
@@ -266,26 +305,26 @@ __global__ void __launch_bounds__(kFwdThreads, kVpt == 2 ? 3 : 2) block_norm_ker
     };
 #pragma unroll
     for (int i = 0; i < kStages; ++i) fetch(i, i);
-    float gs[kForm == kBefore ? 1 : kN], gt[kForm == kBefore ? 1 : kN], rs[kForm == kBefore ? 1 : kN];
-    float s2[kForm == kAfter ? 1 : kN], t2[kForm == kAfter ? 1 : kN];
+    constexpr int kP = kN / 2, kPost = kForm == kBefore ? 1 : kP, kPre = kForm == kAfter ? 1 : kP;
+    float2 gs[kPost], gt[kPost], rs[kPost], s2[kPre], t2[kPre];
     auto par = [&](int i) { return a.par[i] ? a.par[i] + b * a.par_stride[i] : nullptr; };
 #pragma unroll
-    for (int u = 0; u < kN; u += 8) {
-      float p[8];
+    for (int u = 0; u < kP; u += 4) {
       if constexpr (kForm != kBefore) {
-        param8<kVec>(par(kGate), g.t, g.tpr, D, u, 0.f, 1.f, p);
-        param8<kVec>(par(kPostScale), g.t, g.tpr, D, u, a.scale_bias, a.scale_bias, &gs[u]);
-        param8<kVec>(par(kPostShift), g.t, g.tpr, D, u, 0.f, 0.f, &gt[u]);
-        param8<kVec>(par(kResScale), g.t, g.tpr, D, u, 0.f, a.res_scale, &rs[u]);
+        float2 p[4];
+        param8<kVec>(par(kGate), g.t, g.tpr, D, 2 * u, 0.f, 1.f, p);
+        param8<kVec>(par(kPostScale), g.t, g.tpr, D, 2 * u, a.scale_bias, a.scale_bias, &gs[u]);
+        param8<kVec>(par(kPostShift), g.t, g.tpr, D, 2 * u, 0.f, 0.f, &gt[u]);
+        param8<kVec>(par(kResScale), g.t, g.tpr, D, 2 * u, 0.f, a.res_scale, &rs[u]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          gs[u + k] *= p[k];
-          gt[u + k] *= p[k];
+        for (int k = 0; k < 4; ++k) {
+          gs[u + k] = __fmul2_rn(gs[u + k], p[k]);
+          gt[u + k] = __fmul2_rn(gt[u + k], __fmul2_rn(p[k], in_row<kVec>(g, D, u + k)));
         }
       }
       if constexpr (kForm != kAfter) {
-        param8<kVec>(par(kPreScale), g.t, g.tpr, D, u, a.pre_scale_bias, a.pre_scale_bias, &s2[u]);
-        param8<kVec>(par(kPreShift), g.t, g.tpr, D, u, 0.f, 0.f, &t2[u]);
+        param8<kVec>(par(kPreScale), g.t, g.tpr, D, 2 * u, a.pre_scale_bias, a.pre_scale_bias, &s2[u]);
+        param8<kVec>(par(kPreShift), g.t, g.tpr, D, 2 * u, 0.f, 0.f, &t2[u]);
       }
     }
     int stage = 0;
@@ -295,21 +334,22 @@ __global__ void __launch_bounds__(kFwdThreads, kVpt == 2 ? 3 : 2) block_norm_ker
       const int64_t row = base + row0 + g.id, off = row * D;
       const uint32_t at = ring + stage * kStage;
       ring_wait();
-      float v[kN];
+      float2 v[kP];
 #pragma unroll
-      for (int u = 0; u < kN; u += 8)
-        ColX::get8(at, kFwdThreads, reinterpret_cast<const XT*>(a.x) + off, g.t, g.tpr, D, on, u, &v[u]);
+      for (int u = 0; u < kP; u += 4)
+        ColX::get8(at, kFwdThreads, reinterpret_cast<const XT*>(a.x) + off, g.t, g.tpr, D, on, 2 * u, &v[u]);
       float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
       const float2 sx = normalise<kVec>(g, a, v);
       st.x = sx.x;
       st.y = sx.y;
       if constexpr (kForm != kBefore) {
 #pragma unroll
-        for (int u = 0; u < kN; u += 8) {
-          float r[8];
-          ColR::get8(at + ColX::kBytes * kFwdThreads, kFwdThreads, reinterpret_cast<const YT*>(a.r) + off, g.t, g.tpr, D, on, u, r);
+        for (int u = 0; u < kP; u += 4) {
+          float2 r[4];
+          ColR::get8(at + ColX::kBytes * kFwdThreads, kFwdThreads, reinterpret_cast<const YT*>(a.r) + off, g.t, g.tpr, D, on,
+                     2 * u, r);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[u + k] = fmaf(v[u + k], gs[u + k], fmaf(rs[u + k], r[k], gt[u + k]));
+          for (int k = 0; k < 4; ++k) v[u + k] = __ffma2_rn(v[u + k], gs[u + k], __ffma2_rn(rs[u + k], r[k], gt[u + k]));
         }
         store_row<YT, kVec>(reinterpret_cast<YT*>(a.y) + off, g.t, g.tpr, D, on, v);
         if constexpr (kForm == kBetween) {
@@ -322,7 +362,7 @@ __global__ void __launch_bounds__(kFwdThreads, kVpt == 2 ? 3 : 2) block_norm_ker
       stage = stage + 1 == kStages ? 0 : stage + 1;
       if constexpr (kForm != kAfter) {
 #pragma unroll
-        for (int k = 0; k < kN; ++k) v[k] = fmaf(v[k], s2[k], t2[k]);
+        for (int k = 0; k < kP; ++k) v[k] = __ffma2_rn(v[k], s2[k], t2[k]);
         using ZT = typename std::conditional<kForm == kBefore, YT, XT>::type;
         store_row<ZT, kVec>(reinterpret_cast<ZT*>(a.z) + off, g.t, g.tpr, D, on, v);
       }
@@ -382,11 +422,11 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
     const float* par[kParams];
 #pragma unroll
     for (int i = 0; i < kParams; ++i) par[i] = a.par[i] ? a.par[i] + b * a.par_stride[i] : nullptr;
-    float acc[kS][8];
+    float2 acc[kS][4];
 #pragma unroll
     for (int i = 0; i < kS; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) acc[i][k] = 0.f;
+      for (int k = 0; k < 4; ++k) acc[i][k] = make_float2(0.f, 0.f);
     int stage = 0;
     int64_t it = 0;
     const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -398,10 +438,10 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
       next = row0 + step + g.id < a.L ? __ldg(a.stats + row + step) : none;
       ring_wait();
       uint32_t at = ring + stage * stage_bytes;
-      float n[8];  // x, then the normalised row
+      float2 n[4];  // x, then the normalised row
       ColX::get8(at, threads, reinterpret_cast<const XT*>(a.x) + off, g.t, g.tpr, D, on, 0, n);
       at += kX * threads;
-      float r[8], d[8], z[8];
+      float2 r[4], d[4], z[4];
       if constexpr (kForm != kBefore) {
         ColY::get8(at, threads, reinterpret_cast<const YT*>(a.r) + off, g.t, g.tpr, D, on, 0, r);
         at += kR * threads;
@@ -409,7 +449,7 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
           ColY::get8(at, threads, reinterpret_cast<const YT*>(a.dy) + off, g.t, g.tpr, D, on, 0, d);
         } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) d[k] = 0.f;
+          for (int k = 0; k < 4; ++k) d[k] = make_float2(0.f, 0.f);
         }
         at += kR * threads;
       }
@@ -418,72 +458,83 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
           ColZ::get8(at, threads, reinterpret_cast<const ZT*>(a.dz) + off, g.t, g.tpr, D, on, 0, z);
         } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) z[k] = 0.f;
+          for (int k = 0; k < 4; ++k) z[k] = make_float2(0.f, 0.f);
         }
       }
+      // Columns past D come in as zeros and stay so: their 1 / deviation is 0.
+      float2 rho[kVec ? 1 : 4], rho2[kVec ? 1 : 4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) n[k] = col_of<kVec>(g.t, g.tpr, k) < D ? (n[k] - st.x) * st.y : 0.f;
-      float dn[8];
+      for (int k = 0; k < (kVec ? 1 : 4); ++k) {
+        rho[k] = __fmul2_rn(dup(st.y), in_row<kVec>(g, D, k));
+        rho2[k] = __fmul2_rn(dup(st.w), in_row<kVec>(g, D, k));
+      }
+      const float2 mean = dup(-st.x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n[k] = __fmul2_rn(__fadd2_rn(n[k], mean), rho[kVec ? 0 : k]);
+      float2 dn[4];
       if constexpr (kForm == kBefore) {
-        float s2[8];
+        float2 s2[4];
         param8<kVec>(par[kPreScale], g.t, g.tpr, D, 0, a.pre_scale_bias, a.pre_scale_bias, s2);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          acc[kPre][k] = fmaf(z[k], n[k], acc[kPre][k]);
-          acc[kPre + 1][k] += z[k];
-          dn[k] = z[k] * s2[k];
+        for (int k = 0; k < 4; ++k) {
+          acc[kPre][k] = __ffma2_rn(z[k], n[k], acc[kPre][k]);
+          acc[kPre + 1][k] = __fadd2_rn(acc[kPre + 1][k], z[k]);
+          dn[k] = __fmul2_rn(z[k], s2[k]);
         }
       } else {
-        float s[8], gt[8], rs[8], p[8];
+        float2 s[4], gt[4], rs[4], p[4];
         param8<kVec>(par[kPostScale], g.t, g.tpr, D, 0, a.scale_bias, a.scale_bias, s);
         param8<kVec>(par[kPostShift], g.t, g.tpr, D, 0, 0.f, 0.f, p);
         param8<kVec>(par[kGate], g.t, g.tpr, D, 0, 0.f, 1.f, gt);
         param8<kVec>(par[kResScale], g.t, g.tpr, D, 0, 0.f, a.res_scale, rs);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) p[k] = fmaf(n[k], s[k], p[k]);
+        for (int k = 0; k < 4; ++k) p[k] = __ffma2_rn(n[k], s[k], p[k]);
         if constexpr (kForm == kBetween) {
-          float s2[8], m[8], sum[2] = {0.f, 0.f};
+          float2 s2[4], m[4], q0 = make_float2(0.f, 0.f), q1 = q0;
           param8<kVec>(par[kPreScale], g.t, g.tpr, D, 0, a.pre_scale_bias, a.pre_scale_bias, s2);
+          const float2 mean2 = dup(-st.z);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            m[k] = (fmaf(gt[k], p[k], rs[k] * r[k]) - st.z) * st.w;
-            acc[kPre][k] = fmaf(z[k], m[k], acc[kPre][k]);
-            acc[kPre + 1][k] += z[k];
-            z[k] *= s2[k];  // dm
-            if (col_of<kVec>(g.t, g.tpr, k) >= D) z[k] = 0.f;
-            sum[0] += z[k];
-            sum[1] = fmaf(z[k], m[k], sum[1]);
+          for (int k = 0; k < 4; ++k) {
+            m[k] = __fmul2_rn(__fadd2_rn(__ffma2_rn(gt[k], p[k], __fmul2_rn(rs[k], r[k])), mean2), rho2[kVec ? 0 : k]);
+            acc[kPre][k] = __ffma2_rn(z[k], m[k], acc[kPre][k]);
+            acc[kPre + 1][k] = __fadd2_rn(acc[kPre + 1][k], z[k]);
+            z[k] = __fmul2_rn(z[k], s2[k]);  // dm
+            q0 = __fadd2_rn(q0, z[k]);
+            q1 = __ffma2_rn(z[k], m[k], q1);
           }
+          float sum[2] = {total(q0), total(q1)};
           group_sum<2>(g, sum);
-          const float c0 = a.rms ? 0.f : sum[0] * a.inv_d, c1 = sum[1] * a.inv_d;
+          const float2 c0 = dup(a.rms ? 0.f : -sum[0] * a.inv_d), c1 = dup(-sum[1] * a.inv_d);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) d[k] = fmaf(st.w, z[k] - c0 - m[k] * c1, d[k]);
+          for (int k = 0; k < 4; ++k)
+            d[k] = __ffma2_rn(rho2[kVec ? 0 : k], __ffma2_rn(m[k], c1, __fadd2_rn(z[k], c0)), d[k]);
         }
-        float dr[8];
+        float2 dr[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          acc[kPost + kGate][k] = fmaf(d[k], p[k], acc[kPost + kGate][k]);
-          acc[kPost + kResScale][k] = fmaf(d[k], r[k], acc[kPost + kResScale][k]);
-          dr[k] = rs[k] * d[k];
-          const float dp = gt[k] * d[k];
-          acc[kPost + kPostScale][k] = fmaf(dp, n[k], acc[kPost + kPostScale][k]);
-          acc[kPost + kPostShift][k] += dp;
-          dn[k] = dp * s[k];
+        for (int k = 0; k < 4; ++k) {
+          acc[kPost + kGate][k] = __ffma2_rn(d[k], p[k], acc[kPost + kGate][k]);
+          acc[kPost + kResScale][k] = __ffma2_rn(d[k], r[k], acc[kPost + kResScale][k]);
+          dr[k] = __fmul2_rn(rs[k], d[k]);
+          const float2 dp = __fmul2_rn(gt[k], d[k]);
+          acc[kPost + kPostScale][k] = __ffma2_rn(dp, n[k], acc[kPost + kPostScale][k]);
+          acc[kPost + kPostShift][k] = __fadd2_rn(acc[kPost + kPostShift][k], dp);
+          dn[k] = __fmul2_rn(dp, s[k]);
         }
         if (a.dr) store_row<YT, kVec>(reinterpret_cast<YT*>(a.dr) + off, g.t, g.tpr, D, on, dr);
       }
       if (a.dx) {
-        float sum[2] = {0.f, 0.f};
+        float2 q0 = make_float2(0.f, 0.f), q1 = q0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (col_of<kVec>(g.t, g.tpr, k) >= D) dn[k] = 0.f;
-          sum[0] += dn[k];
-          sum[1] = fmaf(dn[k], n[k], sum[1]);
+        for (int k = 0; k < 4; ++k) {
+          q0 = __fadd2_rn(q0, dn[k]);
+          q1 = __ffma2_rn(dn[k], n[k], q1);
         }
+        float sum[2] = {total(q0), total(q1)};
         group_sum<2>(g, sum);
-        const float c0 = a.rms ? 0.f : sum[0] * a.inv_d, c1 = sum[1] * a.inv_d;
+        const float2 c0 = dup(a.rms ? 0.f : -sum[0] * a.inv_d), c1 = dup(-sum[1] * a.inv_d);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) dn[k] = st.y * (dn[k] - c0 - n[k] * c1);
+        for (int k = 0; k < 4; ++k)
+          dn[k] = __fmul2_rn(rho[kVec ? 0 : k], __ffma2_rn(n[k], c1, __fadd2_rn(dn[k], c0)));
         store_row<XT, kVec>(reinterpret_cast<XT*>(a.dx) + off, g.t, g.tpr, D, on, dn);
       }
       fetch(it + kStages, stage);  // this thread is done with its part of the stage
@@ -498,7 +549,7 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int c = col_of<kVec>(g.t, g.tpr, k);
-          if (c < D) ws[(int64_t)i * D + c] = acc[i][k];
+          if (c < D) ws[(int64_t)i * D + c] = k & 1 ? acc[i][k >> 1].y : acc[i][k >> 1].x;
         }
     } else {
       for (int q = 0; q < groups; ++q) {
@@ -509,7 +560,8 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const int c = col_of<kVec>(g.t, g.tpr, k);
-              if (c < D) comb[i * D + c] = q == 0 ? acc[i][k] : comb[i * D + c] + acc[i][k];
+              const float e = k & 1 ? acc[i][k >> 1].y : acc[i][k >> 1].x;
+              if (c < D) comb[i * D + c] = q == 0 ? e : comb[i * D + c] + e;
             }
         }
       }
