@@ -36,6 +36,11 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -53,135 +58,129 @@ struct NormArgs {
   int B;
   float4* stats;  // per row: mean and 1 / deviation of x, and of y
   float* ws;      // backward: (B, gridDim.x, sums, D) partial column sums
+  int param_off;  // backward: byte offset of the parameters in shared memory
 };
 
 // ------------------------------------------------------------------------------------------
-// A row's elements of one thread: kVec: 8 consecutive ones per unit, units tpr apart; else single
-// elements tpr apart (both coalesced). kN elements per thread; columns past D read as zero.
+// A row's elements of one thread: kVec: 4 consecutive ones per unit, units tpr apart (so that a warp's
+// accesses are whole consecutive sectors in fp32 and bf16); else single elements tpr apart. kN per thread.
 // ------------------------------------------------------------------------------------------
 template <bool kVec>
 __device__ __forceinline__ int col_of(int t, int tpr, int k) {
-  return kVec ? (t + tpr * (k >> 3)) * 8 + (k & 7) : t + tpr * k;
+  return kVec ? (t + tpr * (k >> 2)) * 4 + (k & 3) : t + tpr * k;
 }
 
-// One tensor's share of the ring: kN elements per thread and stage. Vector rows go 16 bytes at a time,
-// other fp32 rows 4; other bf16 rows, which cp.async cannot copy, are read when they are used.
+// One tensor's share of the ring: kN elements per thread and stage. Vector rows go a unit at a time (16
+// or 8 bytes), other fp32 rows 4 bytes; other bf16 rows, which cp.async cannot copy, are read when used.
 template <typename T, bool kVec, int kN>
 struct Column {
   static constexpr bool kRing = kVec || sizeof(T) == 4;
   static constexpr int kBytes = kRing ? kN * (int)sizeof(T) : 0;  // per thread
-  static constexpr int kUnit = kVec ? 16 : 4;
   static __device__ __forceinline__ void fetch(uint32_t ring, int threads, const T* row, int t, int tpr, int D, bool on) {
     if constexpr (kRing) {
+      constexpr int kEls = kVec ? 4 : 1, kUnit = kEls * (int)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < kBytes / kUnit; ++i) {
-        // Copy i holds elements i * kUnit / sizeof(T) .. of the thread; out of range: zeros.
-        const int c = col_of<kVec>(t, tpr, i * kUnit / (int)sizeof(T));
-        const bool in = on && c < D;
+      for (int i = 0; i < kN / kEls; ++i) {
+        const int c = col_of<kVec>(t, tpr, i * kEls);
+        const bool in = on && c < D;  // out of range: zeros
         const uint32_t dst = ring + (uint32_t)(i * threads + threadIdx.x) * kUnit;
         const T* src = in ? row + c : row;
         if constexpr (kUnit == 16)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
         else
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(in ? kUnit : 0), "n"(kUnit)
+                       : "memory");
       }
     }
   }
   // Elements u .. u + 7 of the thread.
   static __device__ __forceinline__ void get8(uint32_t ring, int threads, const T* row, int t, int tpr, int D, bool on, int u,
-                                              float2* v2) {
-    float v[8];
+                                              float2* v) {
     if constexpr (!kRing) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int c = col_of<false>(t, tpr, u + k);
-        v[k] = on && c < D ? to_f32(row[c]) : 0.f;
+      for (int k = 0; k < 4; ++k) {
+        const int c0 = col_of<false>(t, tpr, u + 2 * k), c1 = col_of<false>(t, tpr, u + 2 * k + 1);
+        v[k] = make_float2(on && c0 < D ? to_f32(row[c0]) : 0.f, on && c1 < D ? to_f32(row[c1]) : 0.f);
       }
     } else if constexpr (!kVec) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        v[k] = __uint_as_float(lds32(ring + (uint32_t)((u + k) * threads + threadIdx.x) * 4));
+      for (int k = 0; k < 4; ++k)
+        v[k] = make_float2(__uint_as_float(lds32(ring + (uint32_t)((u + 2 * k) * threads + threadIdx.x) * 4)),
+                           __uint_as_float(lds32(ring + (uint32_t)((u + 2 * k + 1) * threads + threadIdx.x) * 4)));
     } else {
-      constexpr int kPer = 16 / (int)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < 8 / kPer; ++i) {
-        const uint4 q = lds128(ring + (uint32_t)((u / kPer + i) * threads + threadIdx.x) * 16);
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t at = ring + (uint32_t)((u / 4 + i) * threads + threadIdx.x) * (4 * (int)sizeof(T));
         if constexpr (sizeof(T) == 4) {
-          v[4 * i] = __uint_as_float(q.x);
-          v[4 * i + 1] = __uint_as_float(q.y);
-          v[4 * i + 2] = __uint_as_float(q.z);
-          v[4 * i + 3] = __uint_as_float(q.w);
+          const uint4 q = lds128(at);
+          v[2 * i] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+          v[2 * i + 1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
         } else {
-          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = unpack_bf16x2(w[k]);
-            v[2 * k] = f.x;
-            v[2 * k + 1] = f.y;
-          }
+          const uint2 q = lds64(at);
+          v[2 * i] = unpack_bf16x2(q.x);
+          v[2 * i + 1] = unpack_bf16x2(q.y);
         }
       }
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v2[k] = make_float2(v[2 * k], v[2 * k + 1]);
   }
 };
 
-constexpr int kStages = 3;
+constexpr int kStages = 3, kBwdStages = 2;  // rows of a group in flight
 __device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void ring_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+template <int kDepth>
+__device__ __forceinline__ void ring_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+}
 __device__ __forceinline__ void ring_drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-template <typename T, bool kVec, int kN>
-__device__ __forceinline__ void store_row(T* row, int t, int tpr, int D, bool on, const float2 (&v2)[kN]) {
+template <typename T, bool kVec, int kP>
+__device__ __forceinline__ void store_row(T* row, int t, int tpr, int D, bool on, const float2 (&v)[kP]) {
   if (!on) return;
-  float v[2 * kN];
 #pragma unroll
-  for (int k = 0; k < kN; ++k) {
-    v[2 * k] = v2[k].x;
-    v[2 * k + 1] = v2[k].y;
-  }
-#pragma unroll
-  for (int u = 0; u < 2 * kN; u += 8) {
+  for (int k = 0; k < kP; k += 2) {
     if constexpr (kVec) {
-      const int c = col_of<true>(t, tpr, u);
-      if (c < D) Vec8<T>::store(row + c, &v[u]);
+      const int c = col_of<true>(t, tpr, 2 * k);
+      if (c >= D) continue;
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4*>(row + c) = make_float4(v[k].x, v[k].y, v[k + 1].x, v[k + 1].y);
+      else
+        *reinterpret_cast<uint2*>(row + c) = make_uint2(pack_bf16x2(v[k].x, v[k].y), pack_bf16x2(v[k + 1].x, v[k + 1].y));
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int c = col_of<false>(t, tpr, u + k);
-        if (c < D) row[c] = from_f32<T>(v[u + k]);
+      for (int e = 0; e < 4; ++e) {
+        const int c = col_of<false>(t, tpr, 2 * k + e);
+        if (c < D) row[c] = from_f32<T>(e & 1 ? v[k + (e >> 1)].y : v[k + (e >> 1)].x);
       }
     }
   }
 }
 
-// Columns u .. u+7 of this thread of a parameter row (null: `fill` everywhere).
+// Columns u .. u+7 of this thread of a parameter row plus `add` (null: `fill`; past D: 0).
 template <bool kVec>
-__device__ __forceinline__ void param8(const float* p, int t, int tpr, int D, int u, float add, float fill, float2* v2) {
-  float v[8];
-  if (!p) {
+__device__ __forceinline__ void param8(const float* p, int t, int tpr, int D, int u, float add, float fill, float2* v) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = fill;
-  } else if constexpr (kVec) {
-    const int c = col_of<true>(t, tpr, u);
-    if (c < D) {
-      Vec8<float>::load(p + c, v);
+  for (int k = 0; k < 4; k += 2) {
+    float e[4];
+    const int c0 = col_of<kVec>(t, tpr, u + 2 * k);
+    if (!p) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += add;
+      for (int i = 0; i < 4; ++i) e[i] = fill;
+    } else if constexpr (kVec) {
+      const float4 q = c0 < D ? __ldg(reinterpret_cast<const float4*>(p + c0)) : make_float4(-add, -add, -add, -add);
+      e[0] = q.x + add;
+      e[1] = q.y + add;
+      e[2] = q.z + add;
+      e[3] = q.w + add;
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+      for (int i = 0; i < 4; ++i) {
+        const int c = col_of<false>(t, tpr, u + 2 * k + i);
+        e[i] = c < D ? __ldg(p + c) + add : 0.f;
+      }
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int c = col_of<false>(t, tpr, u + k);
-      v[k] = c < D ? __ldg(p + c) + add : 0.f;
-    }
+    v[k] = make_float2(e[0], e[1]);
+    v[k + 1] = make_float2(e[2], e[3]);
   }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) v2[k] = make_float2(v[2 * k], v[2 * k + 1]);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -233,11 +232,11 @@ __device__ __forceinline__ void group_sum(Group& g, float (&v)[kVals]) {
 __device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float total(float2 v) { return v.x + v.y; }
 
-// 1 for the pair (2 k, 2 k + 1) of this thread's columns that lie in the row, 0 for the others. Vector
-// rows are in or out 8 columns at a time.
+// 1 for each of the pair (2 k, 2 k + 1) of this thread's columns that lies in the row, 0 for the others.
+// Vector rows are in or out 4 columns at a time.
 template <bool kVec>
 __device__ __forceinline__ float2 in_row(const Group& g, int D, int k) {
-  if constexpr (kVec) return dup(col_of<true>(g.t, g.tpr, 2 * k & ~7) < D ? 1.f : 0.f);
+  if constexpr (kVec) return dup(col_of<true>(g.t, g.tpr, 2 * k) < D ? 1.f : 0.f);
   else
     return make_float2(col_of<false>(g.t, g.tpr, 2 * k) < D ? 1.f : 0.f,
                        col_of<false>(g.t, g.tpr, 2 * k + 1) < D ? 1.f : 0.f);
@@ -333,7 +332,7 @@ __global__ void __launch_bounds__(kFwdThreads, kVpt == 2 ? 3 : 2) block_norm_ker
       const bool on = row0 + g.id < a.L;
       const int64_t row = base + row0 + g.id, off = row * D;
       const uint32_t at = ring + stage * kStage;
-      ring_wait();
+      ring_wait<kStages>();
       float2 v[kP];
 #pragma unroll
       for (int u = 0; u < kP; u += 4)
@@ -391,6 +390,8 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
   __shared__ float buf[4 * kBwdMaxThreads / 32];
   float* comb = reinterpret_cast<float*>(ring_mem);  // after the rows
   const uint32_t ring = smem_addr(ring_mem), stage_bytes = (kX + 2 * kR + kZ) * blockDim.x;
+  // After the ring (or the sums, whichever is larger): the parameters.
+  float4* params = reinterpret_cast<float4*>(ring_mem + a.param_off);
   Group g;
   g.tpr = a.tpr;
   g.id = threadIdx.x / a.tpr;
@@ -418,10 +419,37 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
       ring_commit();
     };
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) fetch(i, i);
-    const float* par[kParams];
+    for (int i = 0; i < kBwdStages; ++i) fetch(i, i);
+    // The parameters that a row needs, once per batch element, into shared memory in the order in which the
+    // group's threads read them (fetched from global memory row by row, 40 KB a row of 2048, they missed L1
+    // and cost two thirds of the kernel's time).
+    if (g.id == 0) {
+      auto put = [&](int slot, int i, float add, float fill) {
+        float2 v[4];
+        param8<kVec>(a.par[i] ? a.par[i] + b * a.par_stride[i] : nullptr, g.t, g.tpr, D, 0, add, fill, v);
 #pragma unroll
-    for (int i = 0; i < kParams; ++i) par[i] = a.par[i] ? a.par[i] + b * a.par_stride[i] : nullptr;
+        for (int k = 0; k < 2; ++k)
+          params[(2 * slot + k) * g.tpr + g.t] = make_float4(v[2 * k].x, v[2 * k].y, v[2 * k + 1].x, v[2 * k + 1].y);
+      };
+      if constexpr (kForm == kBefore) {
+        put(0, kPreScale, a.pre_scale_bias, a.pre_scale_bias);
+      } else {
+        put(0, kPostScale, a.scale_bias, a.scale_bias);
+        put(1, kPostShift, 0.f, 0.f);
+        put(2, kGate, 0.f, 1.f);
+        put(3, kResScale, 0.f, a.res_scale);
+        if constexpr (kForm == kBetween) put(4, kPreScale, a.pre_scale_bias, a.pre_scale_bias);
+      }
+    }
+    __syncthreads();
+    auto pget = [&](int slot, float2 (&v)[4]) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float4 q = params[(2 * slot + k) * g.tpr + g.t];
+        v[2 * k] = make_float2(q.x, q.y);
+        v[2 * k + 1] = make_float2(q.z, q.w);
+      }
+    };
     float2 acc[kS][4];
 #pragma unroll
     for (int i = 0; i < kS; ++i)
@@ -436,7 +464,7 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
       const int64_t row = base + row0 + g.id, off = row * D;
       const float4 st = next;
       next = row0 + step + g.id < a.L ? __ldg(a.stats + row + step) : none;
-      ring_wait();
+      ring_wait<kBwdStages>();
       uint32_t at = ring + stage * stage_bytes;
       float2 n[4];  // x, then the normalised row
       ColX::get8(at, threads, reinterpret_cast<const XT*>(a.x) + off, g.t, g.tpr, D, on, 0, n);
@@ -462,19 +490,20 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
         }
       }
       // Columns past D come in as zeros and stay so: their 1 / deviation is 0.
-      float2 rho[kVec ? 1 : 4], rho2[kVec ? 1 : 4];
+      constexpr int kU = kVec ? 2 : 1;  // pairs per unit
+      float2 rho[4 / kU], rho2[4 / kU];
 #pragma unroll
-      for (int k = 0; k < (kVec ? 1 : 4); ++k) {
-        rho[k] = __fmul2_rn(dup(st.y), in_row<kVec>(g, D, k));
-        rho2[k] = __fmul2_rn(dup(st.w), in_row<kVec>(g, D, k));
+      for (int k = 0; k < 4; k += kU) {
+        rho[k / kU] = __fmul2_rn(dup(st.y), in_row<kVec>(g, D, k));
+        rho2[k / kU] = __fmul2_rn(dup(st.w), in_row<kVec>(g, D, k));
       }
       const float2 mean = dup(-st.x);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) n[k] = __fmul2_rn(__fadd2_rn(n[k], mean), rho[kVec ? 0 : k]);
+      for (int k = 0; k < 4; ++k) n[k] = __fmul2_rn(__fadd2_rn(n[k], mean), rho[k / kU]);
       float2 dn[4];
       if constexpr (kForm == kBefore) {
         float2 s2[4];
-        param8<kVec>(par[kPreScale], g.t, g.tpr, D, 0, a.pre_scale_bias, a.pre_scale_bias, s2);
+        pget(kForm == kBefore ? 0 : 4, s2);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           acc[kPre][k] = __ffma2_rn(z[k], n[k], acc[kPre][k]);
@@ -483,19 +512,19 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
         }
       } else {
         float2 s[4], gt[4], rs[4], p[4];
-        param8<kVec>(par[kPostScale], g.t, g.tpr, D, 0, a.scale_bias, a.scale_bias, s);
-        param8<kVec>(par[kPostShift], g.t, g.tpr, D, 0, 0.f, 0.f, p);
-        param8<kVec>(par[kGate], g.t, g.tpr, D, 0, 0.f, 1.f, gt);
-        param8<kVec>(par[kResScale], g.t, g.tpr, D, 0, 0.f, a.res_scale, rs);
+        pget(0, s);
+        pget(1, p);
+        pget(2, gt);
+        pget(3, rs);
 #pragma unroll
         for (int k = 0; k < 4; ++k) p[k] = __ffma2_rn(n[k], s[k], p[k]);
         if constexpr (kForm == kBetween) {
           float2 s2[4], m[4], q0 = make_float2(0.f, 0.f), q1 = q0;
-          param8<kVec>(par[kPreScale], g.t, g.tpr, D, 0, a.pre_scale_bias, a.pre_scale_bias, s2);
+          pget(kForm == kBefore ? 0 : 4, s2);
           const float2 mean2 = dup(-st.z);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            m[k] = __fmul2_rn(__fadd2_rn(__ffma2_rn(gt[k], p[k], __fmul2_rn(rs[k], r[k])), mean2), rho2[kVec ? 0 : k]);
+            m[k] = __fmul2_rn(__fadd2_rn(__ffma2_rn(gt[k], p[k], __fmul2_rn(rs[k], r[k])), mean2), rho2[k / kU]);
             acc[kPre][k] = __ffma2_rn(z[k], m[k], acc[kPre][k]);
             acc[kPre + 1][k] = __fadd2_rn(acc[kPre + 1][k], z[k]);
             z[k] = __fmul2_rn(z[k], s2[k]);  // dm
@@ -507,7 +536,7 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
           const float2 c0 = dup(a.rms ? 0.f : -sum[0] * a.inv_d), c1 = dup(-sum[1] * a.inv_d);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            d[k] = __ffma2_rn(rho2[kVec ? 0 : k], __ffma2_rn(m[k], c1, __fadd2_rn(z[k], c0)), d[k]);
+            d[k] = __ffma2_rn(rho2[k / kU], __ffma2_rn(m[k], c1, __fadd2_rn(z[k], c0)), d[k]);
         }
         float2 dr[4];
 #pragma unroll
@@ -534,11 +563,11 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
         const float2 c0 = dup(a.rms ? 0.f : -sum[0] * a.inv_d), c1 = dup(-sum[1] * a.inv_d);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          dn[k] = __fmul2_rn(rho[kVec ? 0 : k], __ffma2_rn(n[k], c1, __fadd2_rn(dn[k], c0)));
+          dn[k] = __fmul2_rn(rho[k / kU], __ffma2_rn(n[k], c1, __fadd2_rn(dn[k], c0)));
         store_row<XT, kVec>(reinterpret_cast<XT*>(a.dx) + off, g.t, g.tpr, D, on, dn);
       }
-      fetch(it + kStages, stage);  // this thread is done with its part of the stage
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      fetch(it + kBwdStages, stage);  // this thread is done with its part of the stage
+      stage = stage + 1 == kBwdStages ? 0 : stage + 1;
     }
     ring_drain();
     // This block's column sums of batch element b: over its row groups in turn, then to the workspace.
@@ -567,8 +596,8 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
       }
       __syncthreads();
       for (int e = threadIdx.x; e < kS * D; e += blockDim.x) ws[e] = comb[e];
-      __syncthreads();  // the next batch element's rows use the ring again
     }
+    __syncthreads();  // the next batch element uses the ring and the parameters again
   }
 }
 
@@ -658,15 +687,17 @@ int launch_fwd(NormArgs& a, bool vec, cudaStream_t s) {
 }
 
 template <typename XT, typename YT, int kForm>
-int launch_bwd(const NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
+int launch_bwd(NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
   auto kern = vec ? block_norm_bwd_kernel<XT, YT, kForm, true> : block_norm_bwd_kernel<XT, YT, kForm, false>;
   constexpr int kY = (int)sizeof(YT), kX = (int)sizeof(XT), kZ = kForm == kBefore ? kY : kX;
   int per_el = vec || kX == 4 ? kX : 0;
   if (kForm != kBefore && (vec || kY == 4)) per_el += 2 * kY;
   if (kForm != kAfter && (vec || kZ == 4)) per_el += kZ;
-  int smem = kStages * sh.threads * 8 * per_el;
+  int smem = kBwdStages * sh.threads * 8 * per_el;
   const int combine = sh.threads > sh.tpr ? kSums<kForm> * a.D * 4 : 0;
-  if (smem < combine) smem = combine;
+  if (smem < combine) smem = (combine + 15) / 16 * 16;
+  a.param_off = smem;
+  smem += (kForm == kBefore ? 1 : kForm == kAfter ? 4 : 5) * 8 * sh.tpr * 4;
   FA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kern<<<dim3((unsigned)sh.blocks, (unsigned)(sh.B < 65535 ? sh.B : 65535)), sh.threads, smem, s>>>(a);
   return check_launch("block_norm_bwd_kernel");
@@ -723,7 +754,7 @@ int fwd_form(int form, NormArgs& a, bool vec, cudaStream_t s) {
   return launch_fwd<XT, YT, kBetween>(a, vec, s);
 }
 template <typename XT, typename YT>
-int bwd_form(int form, const NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
+int bwd_form(int form, NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
   if (form == kBefore) return launch_bwd<XT, YT, kBefore>(a, sh, vec, s);
   if (form == kAfter) return launch_bwd<XT, YT, kAfter>(a, sh, vec, s);
   return launch_bwd<XT, YT, kBetween>(a, sh, vec, s);
@@ -734,7 +765,7 @@ int bwd_form(int form, const NormArgs& a, const BwdShape& sh, bool vec, cudaStre
 int dispatch_fwd(int x_dtype, int y_dtype, int form, NormArgs& a, bool vec, cudaStream_t s) {
   FA_NORM_DISPATCH(FA_FWD, form, a, vec, s);
 }
-int dispatch_bwd(int x_dtype, int y_dtype, int form, const NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
+int dispatch_bwd(int x_dtype, int y_dtype, int form, NormArgs& a, const BwdShape& sh, bool vec, cudaStream_t s) {
   FA_NORM_DISPATCH(FA_BWD, form, a, sh, vec, s);
 }
 
@@ -754,7 +785,7 @@ extern "C" int fa_block_norm(int form, int norm, const void* x, int x_dtype, con
   NormArgs a{};
   fill(a, norm, x, residual, params, param_strides, scale_bias, pre_scale_bias, residual_scale, eps, B, L, D);
   a.y = y; a.z = z; a.stats = reinterpret_cast<float4*>(stats);
-  const bool vec = D % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(y) && aligned16(z) &&
+  const bool vec = D % 4 == 0 && aligned16(x) && aligned16(residual) && aligned16(y) && aligned16(z) &&
                    params_aligned(params);
   return dispatch_fwd(x_dtype, y_dtype, form, a, vec, (cudaStream_t)stream);
 }
@@ -793,7 +824,7 @@ extern "C" int fa_block_norm_backward(int form, int norm, const void* x, int x_d
   a.stats = const_cast<float4*>(reinterpret_cast<const float4*>(stats));
   a.ws = reinterpret_cast<float*>(workspace);
   a.tpr = sh.tpr;
-  const bool vec = D % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(dy) && aligned16(dz) &&
+  const bool vec = D % 4 == 0 && aligned16(x) && aligned16(residual) && aligned16(dy) && aligned16(dz) &&
                    aligned16(dx) && aligned16(dresidual) && params_aligned(params);
   const int rc2 = dispatch_bwd(x_dtype, y_dtype, form, a, sh, vec, s);
   if (rc2 != FA_OK) return rc2;
