@@ -7,6 +7,7 @@ The library is the only compute path of this package: when it is missing, every 
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -137,6 +138,14 @@ def dtype_code(t: torch.dtype) -> int:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is current (no context at all when it already is)."""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:

@@ -34,6 +34,9 @@ _NORMS = {"layer": _lib.FA_NORM_LAYER, "rms": _lib.FA_NORM_RMS}
 _PARAMS = ("scale", "shift", "gate", "residual_scale", "pre_scale", "pre_shift")
 
 
+_PTRS, _STRIDES = ctypes.c_void_p * 6, ctypes.c_int64 * 6
+
+
 class _Call:
     """One call's plain arguments."""
 
@@ -52,16 +55,17 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _param_args(params, B: int, D: int):
     """fp32 copies where needed, and the C arrays of pointers and batch strides."""
-    held = [None if p is None else p.reshape(-1, D).to(torch.float32).contiguous() for p in params]
-    ptrs = (ctypes.c_void_p * 6)(*(_ptr(p) for p in held))
-    strides = (ctypes.c_int64 * 6)(*(0 if p is None or p.ndim == 1 else D for p in params))
+    held = [p if p is None or p.dtype == torch.float32 and p.is_contiguous() else p.to(torch.float32).contiguous()
+            for p in params]
+    ptrs = _PTRS(*[p if p is None else p.data_ptr() for p in held])
+    strides = _STRIDES(*[0 if p is None or p.ndim == 1 else D for p in params])
     return held, ptrs, strides
 
 
 def _forward(x, residual, params, call: _Call, want_stats: bool):
     B, L, D = x.shape
     dev = x.device
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         held, ptrs, strides = _param_args(params, B, D)
         y = torch.empty_like(residual) if call.form != _lib.FA_NORM_BEFORE else None
         z = torch.empty(B, L, D, device=dev, dtype=call.z_dtype) if call.form != _lib.FA_NORM_AFTER else None
@@ -98,7 +102,7 @@ class _BlockNorm(torch.autograd.Function):
         dy, dz = (None if g is None else g.contiguous() for g in (dy, dz))
         B, L, D = x.shape
         dev = x.device
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             held, ptrs, strides = _param_args(params, B, D)
             dx = torch.empty_like(x) if need[1] else None
             dr = torch.empty_like(residual) if need[2] else None
@@ -112,7 +116,7 @@ class _BlockNorm(torch.autograd.Function):
             rc = lib.fa_block_norm_backward(
                 call.form, call.norm, x.data_ptr(), _lib.dtype_code(x.dtype), _ptr(residual),
                 _lib.dtype_code(call.y_dtype(residual)), ptrs, strides, *call.biases, _ptr(dy), _ptr(dz),
-                stats.data_ptr(), _ptr(dx), _ptr(dr), (ctypes.c_void_p * 6)(*(_ptr(g) for g in dp)), B, L, D,
+                stats.data_ptr(), _ptr(dx), _ptr(dr), _PTRS(*[_ptr(g) for g in dp]), B, L, D,
                 ws.data_ptr(), n, _lib.stream_ptr(dev))
             _lib.check(rc, "block_norm backward")
         del held

@@ -465,45 +465,42 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
       const float4 st = next;
       next = row0 + step + g.id < a.L ? __ldg(a.stats + row + step) : none;
       ring_wait<kBwdStages>();
-      uint32_t at = ring + stage * stage_bytes;
+      const uint32_t at = ring + stage * stage_bytes;
+      // Values that two phases need (r, the parameters) are read from shared memory in each: the sums take 48
+      // registers, and what is held over a reduction comes on top.
       float2 n[4];  // x, then the normalised row
       ColX::get8(at, threads, reinterpret_cast<const XT*>(a.x) + off, g.t, g.tpr, D, on, 0, n);
-      at += kX * threads;
-      float2 r[4], d[4], z[4];
-      if constexpr (kForm != kBefore) {
-        ColY::get8(at, threads, reinterpret_cast<const YT*>(a.r) + off, g.t, g.tpr, D, on, 0, r);
-        at += kR * threads;
-        if (a.dy) {
-          ColY::get8(at, threads, reinterpret_cast<const YT*>(a.dy) + off, g.t, g.tpr, D, on, 0, d);
-        } else {
+      const uint32_t at_r = at + kX * threads, at_d = at_r + kR * threads, at_z = at_d + kR * threads;
+      auto get_r = [&](float2 (&v)[4]) {
+        ColY::get8(at_r, threads, reinterpret_cast<const YT*>(a.r) + off, g.t, g.tpr, D, on, 0, v);
+      };
+      // Columns past D come in as zeros and stay so: their 1 / deviation is 0.
+      constexpr int kU = kVec ? 2 : 1;  // pairs per unit
+      float2 rho[4 / kU];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) d[k] = make_float2(0.f, 0.f);
-        }
-        at += kR * threads;
-      }
+      for (int k = 0; k < 4; k += kU) rho[k / kU] = __fmul2_rn(dup(st.y), in_row<kVec>(g, D, k));
+      const float2 mean = dup(-st.x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n[k] = __fmul2_rn(__fadd2_rn(n[k], mean), rho[k / kU]);
+      auto get_p = [&](float2 (&v)[4]) {
+        float2 s[4];
+        pget(0, s);
+        pget(1, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = __ffma2_rn(n[k], s[k], v[k]);
+      };
+      float2 z[4], dn[4];
       if constexpr (kForm != kAfter) {
         if (a.dz) {
-          ColZ::get8(at, threads, reinterpret_cast<const ZT*>(a.dz) + off, g.t, g.tpr, D, on, 0, z);
+          ColZ::get8(at_z, threads, reinterpret_cast<const ZT*>(a.dz) + off, g.t, g.tpr, D, on, 0, z);
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k) z[k] = make_float2(0.f, 0.f);
         }
       }
-      // Columns past D come in as zeros and stay so: their 1 / deviation is 0.
-      constexpr int kU = kVec ? 2 : 1;  // pairs per unit
-      float2 rho[4 / kU], rho2[4 / kU];
-#pragma unroll
-      for (int k = 0; k < 4; k += kU) {
-        rho[k / kU] = __fmul2_rn(dup(st.y), in_row<kVec>(g, D, k));
-        rho2[k / kU] = __fmul2_rn(dup(st.w), in_row<kVec>(g, D, k));
-      }
-      const float2 mean = dup(-st.x);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) n[k] = __fmul2_rn(__fadd2_rn(n[k], mean), rho[k / kU]);
-      float2 dn[4];
       if constexpr (kForm == kBefore) {
         float2 s2[4];
-        pget(kForm == kBefore ? 0 : 4, s2);
+        pget(0, s2);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           acc[kPre][k] = __ffma2_rn(z[k], n[k], acc[kPre][k]);
@@ -511,20 +508,25 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
           dn[k] = __fmul2_rn(z[k], s2[k]);
         }
       } else {
-        float2 s[4], gt[4], rs[4], p[4];
-        pget(0, s);
-        pget(1, p);
-        pget(2, gt);
-        pget(3, rs);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) p[k] = __ffma2_rn(n[k], s[k], p[k]);
         if constexpr (kForm == kBetween) {
-          float2 s2[4], m[4], q0 = make_float2(0.f, 0.f), q1 = q0;
-          pget(kForm == kBefore ? 0 : 4, s2);
-          const float2 mean2 = dup(-st.z);
+          float2 m[4], q0 = make_float2(0.f, 0.f), q1 = q0;
+          {
+            float2 r[4], e[4];
+            get_p(m);
+            pget(2, e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m[k] = __fmul2_rn(m[k], e[k]);
+            get_r(r);
+            pget(3, e);
+            const float2 mean2 = dup(-st.z), rstd2 = dup(st.w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              m[k] = __fmul2_rn(__fadd2_rn(__ffma2_rn(e[k], r[k], m[k]), mean2), __fmul2_rn(rstd2, in_row<kVec>(g, D, k)));
+          }
+          float2 s2[4];
+          pget(4, s2);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            m[k] = __fmul2_rn(__fadd2_rn(__ffma2_rn(gt[k], p[k], __fmul2_rn(rs[k], r[k])), mean2), rho2[k / kU]);
             acc[kPre][k] = __ffma2_rn(z[k], m[k], acc[kPre][k]);
             acc[kPre + 1][k] = __fadd2_rn(acc[kPre + 1][k], z[k]);
             z[k] = __fmul2_rn(z[k], s2[k]);  // dm
@@ -533,23 +535,43 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
           }
           float sum[2] = {total(q0), total(q1)};
           group_sum<2>(g, sum);
-          const float2 c0 = dup(a.rms ? 0.f : -sum[0] * a.inv_d), c1 = dup(-sum[1] * a.inv_d);
+          const float2 c0 = dup(a.rms ? 0.f : -sum[0] * a.inv_d), c1 = dup(-sum[1] * a.inv_d), rstd2 = dup(st.w);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            d[k] = __ffma2_rn(rho2[k / kU], __ffma2_rn(m[k], c1, __fadd2_rn(z[k], c0)), d[k]);
+            z[k] = __fmul2_rn(__fmul2_rn(rstd2, in_row<kVec>(g, D, k)), __ffma2_rn(m[k], c1, __fadd2_rn(z[k], c0)));
         }
-        float2 dr[4];
+        float2 d[4];
+        if (a.dy) {
+          ColY::get8(at_d, threads, reinterpret_cast<const YT*>(a.dy) + off, g.t, g.tpr, D, on, 0, d);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) d[k] = make_float2(0.f, 0.f);
+        }
+        if constexpr (kForm == kBetween) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) d[k] = __fadd2_rn(d[k], z[k]);
+        }
+        float2 e[4], f[4];
+        get_r(e);
+        pget(3, f);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          acc[kPost + kGate][k] = __ffma2_rn(d[k], p[k], acc[kPost + kGate][k]);
-          acc[kPost + kResScale][k] = __ffma2_rn(d[k], r[k], acc[kPost + kResScale][k]);
-          dr[k] = __fmul2_rn(rs[k], d[k]);
-          const float2 dp = __fmul2_rn(gt[k], d[k]);
-          acc[kPost + kPostScale][k] = __ffma2_rn(dp, n[k], acc[kPost + kPostScale][k]);
-          acc[kPost + kPostShift][k] = __fadd2_rn(acc[kPost + kPostShift][k], dp);
-          dn[k] = __fmul2_rn(dp, s[k]);
+          acc[kPost + kResScale][k] = __ffma2_rn(d[k], e[k], acc[kPost + kResScale][k]);
+          f[k] = __fmul2_rn(f[k], d[k]);
         }
-        if (a.dr) store_row<YT, kVec>(reinterpret_cast<YT*>(a.dr) + off, g.t, g.tpr, D, on, dr);
+        if (a.dr) store_row<YT, kVec>(reinterpret_cast<YT*>(a.dr) + off, g.t, g.tpr, D, on, f);
+        get_p(e);
+        pget(2, f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          acc[kPost + kGate][k] = __ffma2_rn(d[k], e[k], acc[kPost + kGate][k]);
+          d[k] = __fmul2_rn(f[k], d[k]);  // dp
+          acc[kPost + kPostScale][k] = __ffma2_rn(d[k], n[k], acc[kPost + kPostScale][k]);
+          acc[kPost + kPostShift][k] = __fadd2_rn(acc[kPost + kPostShift][k], d[k]);
+        }
+        pget(0, f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dn[k] = __fmul2_rn(d[k], f[k]);
       }
       if (a.dx) {
         float2 q0 = make_float2(0.f, 0.f), q1 = q0;
@@ -619,8 +641,10 @@ __global__ void __launch_bounds__(32 * kSumRows) block_norm_sum_kernel(const Sum
   for (int b = blockIdx.y; b < (own ? a.B : 1); b += gridDim.y) {
     const int64_t lo = own ? (int64_t)b * a.blocks : 0, hi = own ? lo + a.blocks : (int64_t)a.B * a.blocks;
     double s = 0.0;
-    if (c < a.D)
+    if (c < a.D) {
+#pragma unroll 8
       for (int64_t e = lo + threadIdx.y; e < hi; e += kSumRows) s += (double)a.ws[(e * a.sums + i) * a.D + c];
+    }
     __shared__ double part[kSumRows][32];
     __syncthreads();
     part[threadIdx.y][threadIdx.x] = s;

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -47,20 +48,20 @@ class RelativeBuckets:
         num_buckets = int(num_buckets)
         if not 1 <= num_buckets <= 2 ** 31 - 1:
             raise ValueError(f"num_buckets must be positive, got {num_buckets}")
-        flat = index.detach().reshape(-1).to("cpu", torch.int64)
-        if int(flat.min()) < 0 or int(flat.max()) >= num_buckets:
-            raise ValueError(f"index holds values outside [0, {num_buckets})")
         dev = index.device if device is None else torch.device(device)
         if dev.type == "cuda" and dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
-        offsets = torch.zeros(num_buckets + 1, dtype=torch.int64)
-        offsets[1:] = torch.cumsum(torch.bincount(flat, minlength=num_buckets), 0)
+        flat = index.detach().reshape(-1).to(dev, torch.int64)
+        lo, hi = torch.stack(torch.aminmax(flat)).tolist()
+        if lo < 0 or hi >= num_buckets:
+            raise ValueError(f"index holds values outside [0, {num_buckets})")
+        values, order = torch.sort(flat, stable=True)
         self.tokens = int(index.shape[0])
         self.num_buckets = num_buckets
         self.device = dev
-        self.index = flat.view(self.tokens, self.tokens).to(torch.int32).to(dev)
-        self.order = torch.argsort(flat, stable=True).to(torch.int32).to(dev)
-        self.offsets = offsets.to(torch.int32).to(dev)
+        self.index = flat.view(self.tokens, self.tokens).to(torch.int32)
+        self.order = order.to(torch.int32)
+        self.offsets = torch.searchsorted(values, torch.arange(num_buckets + 1, device=dev)).to(torch.int32)
 
     def to(self, device) -> "RelativeBuckets":
         """These buckets on ``device`` (this object if it is there already)."""
@@ -123,25 +124,49 @@ def _strided(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _precision(dtype: torch.dtype) -> int:
-    return _lib.FA_ATTN_BF16 if dtype == torch.bfloat16 else _lib.FA_ATTN_FP32_3XTF32
-
-
 def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
 
-def _strides(*tensors: torch.Tensor):
-    """Window, head and token strides of each tensor; an axis of one entry gets a legal stride."""
-    flat = [s if n > 1 else _HEAD_DIM for t in tensors for s, n in zip(t.stride()[:3], t.shape[:3])]
+@lru_cache(maxsize=64)
+def _bytes(which: str, device: int, *args: int) -> int:
+    """Size of a buffer; ``device``, the current one, keeps the cached sizes of unlike devices apart."""
+    n = getattr(_lib.load(), "fa_window_attention_rel_bias_" + which)(*args)
+    if n < 0:
+        _lib.check(int(n), "window_attn_rel_bias")
+    return int(n)
+
+
+# An operand of the kernels: its address and the strides of window, head and token (elements).
+def _heads(t: torch.Tensor) -> tuple:
+    """``(Bwin, H, N, Dh)``; an axis of one entry gets a legal stride."""
+    n, s = t.shape, t.stride()
+    return (t.data_ptr(), *(s[i] if n[i] > 1 else _HEAD_DIM for i in range(3)))
+
+
+def _bnc(t: torch.Tensor) -> tuple:
+    """Contiguous ``(Bwin, N, H * Dh)``."""
+    return t.data_ptr(), t.shape[1] * t.shape[2], _HEAD_DIM, t.shape[2]
+
+
+def _qkv(t: torch.Tensor) -> tuple:
+    """q, k and v of a contiguous ``(Bwin, N, 3 * H * Dh)``."""
+    row = t.shape[2]
+    step = row // 3 * t.element_size()
+    return tuple((t.data_ptr() + i * step, t.shape[1] * row, _HEAD_DIM, row) for i in range(3))
+
+
+def _strides(*ops: tuple):
+    flat = [s for o in ops for s in o[1:]]
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
 class _Call:
     """One attention call's arguments besides its tensors. ``kind``: None, "mask_u8" or "group_ids"."""
 
-    def __init__(self, buckets, kind, nW, scale) -> None:
-        self.buckets, self.kind, self.nW, self.scale = buckets, kind, nW, scale
+    def __init__(self, dtype, device, shape, buckets, kind, nW, scale) -> None:
+        self.precision = _lib.FA_ATTN_BF16 if dtype == torch.bfloat16 else _lib.FA_ATTN_FP32_3XTF32
+        self.device, self.shape, self.buckets, self.kind, self.nW, self.scale = device, shape, buckets, kind, nW, scale
 
     def masks(self, mask: Optional[torch.Tensor]):
         """The C arguments mask_u8, group_ids, nW, scale."""
@@ -150,59 +175,47 @@ class _Call:
 
 
 def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool):
-    """Launch the forward kernels into ``out``; returns the state that the backward pass reads, and the
+    """Launch the forward kernels into the operand ``out``; returns the state that the backward pass reads, and the
     row statistics when asked for."""
-    Bwin, H, N, Dh = q.shape
-    dev = q.device
-    with torch.cuda.device(dev):
+    Bwin, H, N = call.shape
+    dev = call.device
+    with _lib.on_device(dev):
         stats = torch.empty(Bwin, H, _MAX_TOKENS, 2, device=dev, dtype=torch.float32) if want_stats else None
-        lib = _lib.load()
-        n = lib.fa_window_attention_rel_bias_state(_precision(q.dtype), H, call.nW if call.kind == "group_ids" else 0)
-        if n < 0:
-            _lib.check(int(n), "window_attn_rel_bias")
+        n = _bytes("state", dev.index, call.precision, H, call.nW if call.kind == "group_ids" else 0)
         state = torch.empty(n, dtype=torch.uint8, device=dev)
-        rc = lib.fa_window_attention_rel_bias(
-            _precision(q.dtype), Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-            _strides(q, k, v, out), table.data_ptr(), _lib.dtype_code(table.dtype), call.buckets.index.data_ptr(),
-            *call.masks(mask), state.data_ptr(), _ptr(stats), _lib.stream_ptr(dev))
+        rc = _lib.load().fa_window_attention_rel_bias(
+            call.precision, Bwin, H, N, _HEAD_DIM, q[0], k[0], v[0], out[0], _strides(q, k, v, out), table.data_ptr(),
+            _lib.dtype_code(table.dtype), call.buckets.index.data_ptr(), *call.masks(mask), state.data_ptr(),
+            _ptr(stats), _lib.stream_ptr(dev))
         _lib.check(rc, "window_attn_rel_bias")
     return state, stats
 
 
 def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, state, stats, table_dtype) -> Optional[torch.Tensor]:
-    """Launch the backward kernels into ``dq``, ``dk``, ``dv``; returns the table's gradient, in ``table_dtype``
-    (None: not asked for)."""
-    Bwin, H, N, Dh = q.shape
-    dev = q.device
+    """Launch the backward kernels into the operands ``dq``, ``dk``, ``dv``; returns the table's gradient, in
+    ``table_dtype`` (None: not asked for)."""
+    Bwin, H, N = call.shape
+    dev = call.device
     b = call.buckets
-    with torch.cuda.device(dev):
-        lib = _lib.load()
+    with _lib.on_device(dev):
         dtable = None if table_dtype is None else torch.empty(b.num_buckets, H, device=dev, dtype=table_dtype)
-        n = lib.fa_window_attention_rel_bias_workspace(Bwin, H, N)
-        if n < 0:
-            _lib.check(int(n), "window_attn_rel_bias backward")
+        n = _bytes("workspace", dev.index, Bwin, H, N)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        rc = lib.fa_window_attention_rel_bias_backward(
-            _precision(q.dtype), Bwin, H, N, Dh, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr(), _strides(q, k, v, dout, dq, dk, dv), *call.masks(mask), state.data_ptr(),
-            stats.data_ptr(), b.order.data_ptr(), b.offsets.data_ptr(), b.num_buckets, _ptr(dtable),
+        rc = _lib.load().fa_window_attention_rel_bias_backward(
+            call.precision, Bwin, H, N, _HEAD_DIM, q[0], k[0], v[0], dout[0], dq[0], dk[0], dv[0],
+            _strides(q, k, v, dout, dq, dk, dv), *call.masks(mask), state.data_ptr(), stats.data_ptr(),
+            b.order.data_ptr(), b.offsets.data_ptr(), b.num_buckets, _ptr(dtable),
             _lib.dtype_code(table_dtype or torch.float32), ws.data_ptr(), n, _lib.stream_ptr(dev))
         _lib.check(rc, "window_attn_rel_bias backward")
     return dtable
-
-
-def _same_heads(t: torch.Tensor, bnc: bool, H: int) -> torch.Tensor:
-    """``(Bwin, H, N, Dh)`` view of an output or its gradient in either layout."""
-    if bnc:
-        return t.view(t.shape[0], t.shape[1], H, _HEAD_DIM).permute(0, 2, 1, 3)
-    return t
 
 
 class _Attn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, mask, call):
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        ctx.save_for_backward(q, k, v, mask, *_forward(q, k, v, out, table, mask, call, True))
+        state = _forward(_heads(q), _heads(k), _heads(v), _heads(out), table, mask, call, True)
+        ctx.save_for_backward(q, k, v, mask, *state)
         ctx.call, ctx.table_dtype = call, table.dtype
         return out
 
@@ -211,18 +224,19 @@ class _Attn(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, mask, state, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
+        dout = _strided(dout)
         dq, dk, dv = (torch.empty(q.shape, device=q.device, dtype=q.dtype) for _ in range(3))
-        dtable = _backward(q, k, v, _strided(dout), dq, dk, dv, mask, ctx.call, state, stats,
+        dtable = _backward(*(_heads(t) for t in (q, k, v, dout, dq, dk, dv)), mask, ctx.call, state, stats,
                            ctx.table_dtype if need[3] else None)
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None
 
 
 class _AttnPacked(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, table, mask, call, H, bnc):
-        out, saved = _packed_forward(qkv, table, mask, call, H, bnc, True)
-        ctx.save_for_backward(qkv, mask, *saved)
-        ctx.call, ctx.table_dtype, ctx.H, ctx.bnc = call, table.dtype, H, bnc
+    def forward(ctx, qkv, table, mask, call, bnc):
+        out, state = _packed_forward(qkv, table, mask, call, bnc, True)
+        ctx.save_for_backward(qkv, mask, *state)
+        ctx.call, ctx.table_dtype, ctx.bnc = call, table.dtype, bnc
         return out
 
     @staticmethod
@@ -230,23 +244,21 @@ class _AttnPacked(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, mask, state, stats = ctx.saved_tensors
         dqkv = torch.empty_like(qkv)
-        dout = _strided(_same_heads(dout.contiguous() if ctx.bnc else dout, ctx.bnc, ctx.H))
-        dtable = _backward(*_heads_of(qkv, ctx.H), dout, *_heads_of(dqkv, ctx.H), mask, ctx.call, state, stats,
+        if ctx.bnc:
+            dout = dout.contiguous()
+            dout = dout if dout.data_ptr() % 16 == 0 else dout.clone()
+        else:
+            dout = _strided(dout)
+        dtable = _backward(*_qkv(qkv), _bnc(dout) if ctx.bnc else _heads(dout), *_qkv(dqkv), mask, ctx.call, state, stats,
                            ctx.table_dtype if ctx.needs_input_grad[1] else None)
-        return dqkv if ctx.needs_input_grad[0] else None, dtable, None, None, None, None
+        return dqkv if ctx.needs_input_grad[0] else None, dtable, None, None, None
 
 
-def _heads_of(qkv: torch.Tensor, H: int):
-    """q, k, v as ``(Bwin, H, N, Dh)`` views of a packed ``(Bwin, N, 3 * H * Dh)`` tensor."""
-    Bwin, N, _ = qkv.shape
-    return qkv.view(Bwin, N, 3, H, _HEAD_DIM).permute(2, 0, 3, 1, 4).unbind(0)
-
-
-def _packed_forward(qkv, table, mask, call, H, bnc, want_stats):
-    Bwin, N, _ = qkv.shape
+def _packed_forward(qkv, table, mask, call, bnc, want_stats):
+    Bwin, H, N = call.shape
     shape = (Bwin, N, H * _HEAD_DIM) if bnc else (Bwin, H, N, _HEAD_DIM)
     out = torch.empty(shape, device=qkv.device, dtype=qkv.dtype)
-    return out, _forward(*_heads_of(qkv, H), _same_heads(out, bnc, H), table, mask, call, want_stats)
+    return out, _forward(*_qkv(qkv), _bnc(out) if bnc else _heads(out), table, mask, call, want_stats)
 
 
 def _check_window(N: int, Dh: int) -> None:
@@ -256,11 +268,11 @@ def _check_window(N: int, Dh: int) -> None:
         raise ValueError(f"window attention supports 1 to {_MAX_TOKENS} tokens per window, got {N}")
 
 
-def _call_args(t, N, H, table, buckets, bias, group_ids, scale_qk):
+def _call_args(t, Bwin, H, N, table, buckets, bias, group_ids, scale_qk):
     if bias is not None and group_ids is not None:
         raise ValueError("pass at most one of bias / group_ids")
     _check_bias(table, buckets, H, N, t.device)
-    with torch.cuda.device(t.device):
+    with _lib.on_device(t.device):
         mask_u8, gids, nW, _ = _mask_args(bias, group_ids, t.device, N)
     if (mask_u8 is not None or gids is not None) and nW < 1:
         raise ValueError("a mask needs at least one window")
@@ -268,7 +280,8 @@ def _call_args(t, N, H, table, buckets, bias, group_ids, scale_qk):
     if not 1e-30 <= abs(scale) <= 1e30:
         raise ValueError(f"scale_qk must be finite and at least 1e-30 in magnitude, got {scale}")
     kind = "mask_u8" if mask_u8 is not None else "group_ids" if gids is not None else None
-    return table.contiguous(), mask_u8 if mask_u8 is not None else gids, _Call(buckets, kind, nW, scale)
+    return table.contiguous(), mask_u8 if mask_u8 is not None else gids, _Call(
+        t.dtype, t.device, (Bwin, H, N), buckets, kind, nW, scale)
 
 
 def window_attn_rel_bias(
@@ -299,12 +312,12 @@ def window_attn_rel_bias(
         raise RuntimeError("B200 window attention requires CUDA tensors.")
     if k.device != q.device or v.device != q.device:
         raise ValueError("q, k and v must be on one device")
-    table, mask, call = _call_args(q, N, H, table, buckets, bias, group_ids, scale_qk)
+    table, mask, call = _call_args(q, Bwin, H, N, table, buckets, bias, group_ids, scale_qk)
     q, k, v = _strided(q), _strided(k), _strided(v)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table)):
         return _Attn.apply(q, k, v, table, mask, call)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    _forward(q, k, v, out, table, mask, call, False)
+    _forward(_heads(q), _heads(k), _heads(v), _heads(out), table, mask, call, False)
     return out
 
 
@@ -336,10 +349,10 @@ def window_attn_rel_bias_qkvpacked(
     _check_window(N, three_c // (3 * H))
     if not qkv.is_cuda:
         raise RuntimeError("B200 window attention requires CUDA tensors.")
-    table, mask, call = _call_args(qkv, N, H, table, buckets, bias, group_ids, scale_qk)
+    table, mask, call = _call_args(qkv, Bwin, H, N, table, buckets, bias, group_ids, scale_qk)
     if qkv.data_ptr() % 16:
         qkv = qkv.clone()
     bnc = output_layout == "bnc"
     if torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad):
-        return _AttnPacked.apply(qkv, table, mask, call, H, bnc)
-    return _packed_forward(qkv, table, mask, call, H, bnc, False)[0]
+        return _AttnPacked.apply(qkv, table, mask, call, bnc)
+    return _packed_forward(qkv, table, mask, call, bnc, False)[0]
