@@ -92,41 +92,72 @@ expand_bias_kernel(const void* table, int bf16, const int32_t* index, int H, int
   out[(int64_t)hc * kBiasVecs + e] = make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// dT[b, h] = sum over the pairs of bucket b (positions order[offsets[b]] .. in the N x N index) of
-// the head's partials. One block per (bucket, head); every thread adds its share in a fixed order.
-constexpr int kReduceThreads = 128;
+// The blocks of a main kernel of `grid` blocks whose tile ranges meet head h: block c covers tiles
+// [c T / G, (c + 1) T / G), head h tiles [h Bwin, (h + 1) Bwin).
+__device__ __forceinline__ int2 blocks_of_head(int h, int Bwin, int num_tiles, int grid) {
+  auto block_of = [&](int64_t tile) {
+    int c = (int)(tile * grid / num_tiles);
+    while (c > 0 && (int64_t)c * num_tiles / grid > tile) --c;
+    while (c + 1 < grid && (int64_t)(c + 1) * num_tiles / grid <= tile) ++c;
+    return c;
+  };
+  const int64_t lo = (int64_t)h * Bwin;
+  return make_int2(block_of(lo), block_of(lo + Bwin - 1));
+}
+
+// Adds a head's partials, coalesced, into its first one, one thread per pair; without this pass the
+// gather below reads a sector per pair and partial.
+constexpr int kSumThreads = 128;
+__global__ void __launch_bounds__(kSumThreads) sum_slots_kernel(float* slots, int H, int Bwin, int num_tiles, int grid) {
+  const int e = blockIdx.x * kSumThreads + threadIdx.x;
+  for (int h = blockIdx.y; h < H; h += gridDim.y) {
+    const int2 c = blocks_of_head(h, Bwin, num_tiles, grid);
+    float* p = slots + (int64_t)(c.x + h) * (4 * kBiasVecs) + e;
+    float s = *p;
+#pragma unroll 8
+    for (int i = 1; i <= c.y - c.x; ++i) s += __ldg(p + (int64_t)i * (4 * kBiasVecs));
+    *p = s;
+  }
+}
+static_assert(4 * kBiasVecs % kSumThreads == 0, "whole blocks");
+
+// dT[b, h] = sum over the pairs of bucket b (positions order[offsets[b]] .. in the N x N index) of the
+// head's first partial (summed: it is the sum of all) or of each, by kPer threads, a warp or a block, each
+// adding its share in a fixed order.
+constexpr int kReduceThreads = 256;
+template <int kPer>
 __global__ void __launch_bounds__(kReduceThreads)
 bias_grad_kernel(const float* slots, const int32_t* order, const int32_t* offsets, void* dtable, int dtable_bf16, int H,
-                 int N, int Bwin, int num_tiles, int grid) {
-  const int b = blockIdx.x, h = blockIdx.y;
-  // Blocks of the main kernel whose tile range meets [h * Bwin, (h + 1) * Bwin): block c covers
-  // [c * T / G, (c + 1) * T / G).
-  float acc = 0.f;
-  if (num_tiles > 0) {
-    const int64_t lo = (int64_t)h * Bwin, hi = lo + Bwin;
-    int c0 = (int)(lo * grid / num_tiles), c1 = (int)((hi - 1) * grid / num_tiles);
-    while (c0 > 0 && (int64_t)c0 * num_tiles / grid > lo) --c0;
-    while (c0 + 1 < grid && (int64_t)(c0 + 1) * num_tiles / grid <= lo) ++c0;
-    while (c1 > 0 && (int64_t)c1 * num_tiles / grid > hi - 1) --c1;
-    while (c1 + 1 < grid && (int64_t)(c1 + 1) * num_tiles / grid <= hi - 1) ++c1;
-    const int p0 = offsets[b], p1 = offsets[b + 1];
-    for (int e = p0 + threadIdx.x; e < p1; e += kReduceThreads) {
-      const int pos = order[e], i = pos / N;
-      const float* f = slots + frag_index(i, pos - i * N);
-      for (int c = c0; c <= c1; ++c) acc += f[(int64_t)(c + h) * (4 * kBiasVecs)];
+                 int num_buckets, int N, int Bwin, int num_tiles, int grid, int summed) {
+  const int b = blockIdx.x * (kReduceThreads / kPer) + threadIdx.x / kPer, t = threadIdx.x % kPer;
+  if (b >= num_buckets) return;  // whole warps
+  for (int h = blockIdx.y; h < H; h += gridDim.y) {
+    float acc = 0.f;
+    if (num_tiles > 0) {
+      int2 c = blocks_of_head(h, Bwin, num_tiles, grid);
+      if (summed) c.y = c.x;
+      const int p1 = offsets[b + 1];
+      for (int e = offsets[b] + t; e < p1; e += kPer) {
+        const int pos = order[e], i = pos / N;
+        const float* f = slots + (int64_t)(c.x + h) * (4 * kBiasVecs) + frag_index(i, pos - i * N);
+        for (int k = 0; k <= c.y - c.x; ++k) acc += f[(int64_t)k * (4 * kBiasVecs)];
+      }
     }
-  }
-  __shared__ float warp_acc[kReduceThreads / 32];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if ((threadIdx.x & 31) == 0) warp_acc[threadIdx.x >> 5] = acc;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float s = 0.f;
-    for (int i = 0; i < kReduceThreads / 32; ++i) s += warp_acc[i];
-    const int64_t e = (int64_t)b * H + h;
-    if (dtable_bf16) reinterpret_cast<__nv_bfloat16*>(dtable)[e] = __float2bfloat16_rn(s);
-    else reinterpret_cast<float*>(dtable)[e] = s;
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if constexpr (kPer > 32) {
+      __shared__ float warp_acc[kPer / 32];
+      __syncthreads();
+      if ((t & 31) == 0) warp_acc[t >> 5] = acc;
+      __syncthreads();
+      acc = 0.f;
+      for (int i = 0; i < kPer / 32; ++i) acc += warp_acc[i];
+    }
+    if (t == 0) {
+      const int64_t e = (int64_t)b * H + h;
+      if (dtable_bf16) reinterpret_cast<__nv_bfloat16*>(dtable)[e] = __float2bfloat16_rn(acc);
+      else reinterpret_cast<float*>(dtable)[e] = acc;
+    }
   }
 }
 
@@ -258,8 +289,8 @@ extern "C" int fa_window_attention_rel_bias_backward(
              "the row statistics must be given, 16-byte aligned");
   FA_REQUIRE(!dtable || dtable_dtype == FA_F32 || dtable_dtype == FA_BF16, FA_ERR_INVALID,
              "table dtype must be FA_F32 or FA_BF16");
-  FA_REQUIRE(!dtable || (order && offsets && num_buckets >= 1 && num_buckets < ((int64_t)1 << 31) && H <= 65535),
-             FA_ERR_INVALID, "a bias gradient needs the bucket lists (and at most 65535 heads)");
+  FA_REQUIRE(!dtable || (order && offsets && num_buckets >= 1 && num_buckets < ((int64_t)1 << 31)),
+             FA_ERR_INVALID, "a bias gradient needs the bucket lists");
   cudaStream_t s = (cudaStream_t)stream;
   const int64_t need = fa_window_attention_rel_bias_workspace(Bwin, H, N);
   FA_REQUIRE(Bwin == 0 || (workspace && workspace_bytes >= need), FA_ERR_INVALID, "workspace too small");
@@ -285,8 +316,21 @@ extern "C" int fa_window_attention_rel_bias_backward(
     if (rc != FA_OK) return rc;
   }
   if (!dtable) return FA_OK;
-  bias_grad_kernel<<<dim3((unsigned)num_buckets, (unsigned)H), kReduceThreads, 0, s>>>(
-      reinterpret_cast<const float*>(workspace), order, offsets, dtable, dtable_dtype == FA_BF16, (int)H, (int)N,
-      (int)Bwin, (int)(Bwin * H), grid);
+  const unsigned heads = (unsigned)(H < 65535 ? H : 65535);
+  // Up to about three partials a head are gathered directly: a second launch costs more than it saves.
+  const bool sum = Bwin > 0 && grid > 2 * H;
+  if (sum) {
+    sum_slots_kernel<<<dim3(4 * kBiasVecs / kSumThreads, heads), kSumThreads, 0, s>>>(
+        reinterpret_cast<float*>(workspace), (int)H, (int)Bwin, (int)(Bwin * H), grid);
+    if ((rc = check_launch("sum_slots_kernel")) != FA_OK) return rc;
+  }
+  // A warp per bucket where buckets are small (the 3-D offsets of a window: 27 pairs each on average, 20 us
+  // with a block each), a block where they are large (32 log-distance buckets: 18 us with two warps each).
+  const bool small = N * N <= 64 * num_buckets;
+  auto kern = small ? bias_grad_kernel<32> : bias_grad_kernel<kReduceThreads>;
+  const unsigned per_block = small ? kReduceThreads / 32 : 1;
+  kern<<<dim3(((unsigned)num_buckets + per_block - 1) / per_block, heads), kReduceThreads, 0, s>>>(
+      reinterpret_cast<const float*>(workspace), order, offsets, dtable, dtable_dtype == FA_BF16, (int)H, (int)num_buckets,
+      (int)N, (int)Bwin, (int)(Bwin * H), grid, sum ? 1 : 0);
   return check_launch("bias_grad_kernel");
 }
