@@ -14,7 +14,8 @@ Tensors are ``(B, L, D)``, float32 or bfloat16, ``D <= 4096``. Scales, shifts, g
 ``None`` counts as zero for a scale or shift and as one for a gate. With ``scale_bias=0`` a scale is
 an ordinary norm weight; with the default of one it is a modulation. Everything is computed in fp32
 and each output is rounded once; sums over rows run in a fixed order, so equal calls give equal bits.
-Gradients of gradients are not available.
+Gradients of gradients are not available. A step may be captured in a CUDA graph; as for any differentiable
+torch call, no eager autograd graph of the same leaves may be alive then (torch refuses such a capture).
 """
 
 from __future__ import annotations

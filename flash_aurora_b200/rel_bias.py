@@ -9,6 +9,9 @@ q, k, v (or the packed qkv) and the table. Windows hold 1 to 144 tokens, head_di
 bfloat16 or float32 (3xTF32 products, fp32 accuracy); masks as in ``window_attn``: region ids or a
 float bias below -50, each adding -100 to a masked logit.
 
+A step may be captured in a CUDA graph; as for any differentiable torch call, no eager autograd graph of the same
+leaves may be alive then (torch refuses such a capture).
+
 Nothing is kept between calls: the backward pass recomputes the probabilities from q, k, the table
 and the row statistics of its own forward call. Sums run in a fixed order, so equal calls give equal
 bits. Gradients of gradients are not available.
@@ -71,15 +74,19 @@ class RelativeBuckets:
         return self if dev == self.device else RelativeBuckets(self.index, self.num_buckets, dev)
 
     @classmethod
-    def window(cls, window_size, device: Optional[torch.device] = None) -> "RelativeBuckets":
+    def window(cls, window_size, device: Optional[torch.device] = None, table_window=None) -> "RelativeBuckets":
         """One bucket per 3-D offset of a ``(wc, wh, ww)`` window, ``(2wc-1)(2wh-1)(2ww-1)`` in all, in
-        the order of Swin's ``relative_position_index``."""
+        the order of Swin's ``relative_position_index``. ``table_window``: the buckets are those of this window,
+        at least as large on each axis (a window clamped to a small grid reads the table of its full size)."""
         w = tuple(int(v) for v in window_size)
-        if len(w) != 3 or min(w) < 1:
+        full = w if table_window is None else tuple(int(v) for v in table_window)
+        if len(w) != 3 or len(full) != 3 or min(w) < 1:
             raise ValueError(f"window_size must be three positive integers, got {tuple(window_size)}")
+        if any(f < v for f, v in zip(full, w)):
+            raise ValueError(f"table_window {full} is smaller than the window {w}")
         pos = torch.cartesian_prod(*(torch.arange(v) for v in w)).view(-1, 3)
-        rel = pos[:, None, :] - pos[None, :, :] + torch.tensor([v - 1 for v in w])
-        span = [2 * v - 1 for v in w]
+        rel = pos[:, None, :] - pos[None, :, :] + torch.tensor([v - 1 for v in full])
+        span = [2 * v - 1 for v in full]
         index = (rel[..., 0] * span[1] + rel[..., 1]) * span[2] + rel[..., 2]
         return cls(index, span[0] * span[1] * span[2], device if device is not None else torch.device("cpu"))
 

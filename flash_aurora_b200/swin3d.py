@@ -50,6 +50,7 @@ from . import _lib
 from . import recorder as _rec
 from .activation import gelu_erf
 from .linear import linear_adaln_film_add_residual, linear_bias_act
+from .rel_bias import RelativeBuckets, window_attn_rel_bias_qkvpacked
 from .sharding import BandContext
 from .swin3d_layout import band_halo_extract, roll_pad_partition_windows, roll_pad_partition_windows_band
 from .util import maybe_adjust_windows, window_geometry
@@ -155,9 +156,12 @@ class MLP(nn.Module):
 
 
 class WindowAttention(nn.Module):
-    """W-MSA / SW-MSA parameters (upstream swin3d.py:112-409): ``qkv`` and ``proj`` linears."""
+    """W-MSA / SW-MSA parameters (upstream swin3d.py:112-409): ``qkv`` and ``proj`` linears, and with
+    ``rel_pos_bias`` (no upstream counterpart) the learned bias of every window offset and head,
+    ``relative_position_bias_table``, zero at first."""
 
-    def __init__(self, dim: int, window_size, num_heads: int, qkv_bias: bool = True) -> None:
+    def __init__(self, dim: int, window_size, num_heads: int, qkv_bias: bool = True,
+                 rel_pos_bias: bool = False) -> None:
         super().__init__()
         assert dim % num_heads == 0, f"dim ({dim}) should be divisible by num_heads ({num_heads})."
         self.dim = dim
@@ -166,6 +170,18 @@ class WindowAttention(nn.Module):
         self.head_dim = dim // num_heads
         self.qkv = nn.Linear(dim, dim * 3, bias=qkv_bias)
         self.proj = nn.Linear(dim, dim)
+        self.relative_position_bias_table = None
+        if rel_pos_bias:
+            offsets = math.prod(2 * w - 1 for w in self.window_size)
+            self.relative_position_bias_table = nn.Parameter(torch.zeros(offsets, num_heads))
+        self._buckets: dict = {}
+
+    def buckets(self, window_size, device: torch.device) -> RelativeBuckets:
+        """Bias buckets of a window of this size (the configured one, or clamped to a small grid)."""
+        key = (tuple(window_size), str(device))
+        if key not in self._buckets:
+            self._buckets[key] = RelativeBuckets.window(window_size, device, table_window=self.window_size)
+        return self._buckets[key]
 
 
 class Swin3DTransformerBlock(nn.Module):
@@ -173,7 +189,7 @@ class Swin3DTransformerBlock(nn.Module):
 
     def __init__(self, dim: int, num_heads: int, time_dim: int, window_size=(2, 7, 7),
                  shift_size=(0, 0, 0), mlp_ratio: float = 4.0, qkv_bias: bool = True,
-                 scale_bias: float = 0.0, precision: str = "bf16_mixed") -> None:
+                 scale_bias: float = 0.0, precision: str = "bf16_mixed", rel_pos_bias: bool = False) -> None:
         super().__init__()
         self.dim = dim
         self.window_size = tuple(window_size)
@@ -182,7 +198,7 @@ class Swin3DTransformerBlock(nn.Module):
         self.mlp_ratio = mlp_ratio
         self.precision = _check_precision(precision)
         self.norm1 = AdaptiveLayerNorm(dim, time_dim, scale_bias=scale_bias)
-        self.attn = WindowAttention(dim, self.window_size, num_heads, qkv_bias=qkv_bias)
+        self.attn = WindowAttention(dim, self.window_size, num_heads, qkv_bias=qkv_bias, rel_pos_bias=rel_pos_bias)
         self.norm2 = AdaptiveLayerNorm(dim, time_dim, scale_bias=scale_bias)
         self.mlp = MLP(dim, int(dim * mlp_ratio))
         self._bf16 = _CastCache()
@@ -280,7 +296,12 @@ class Swin3DTransformerBlock(nn.Module):
             qkv = self._linear(xw, wq, bq, bf16)
             _rec.end("qkv_gemm", ev, (T * D + 3 * D * D + 3 * T * D) * e, 2 * T * D * 3 * D)
             ev = _rec.begin()
-            a = window_attn_fwd_cute_qkvpacked(qkv, heads, group_ids=gids, output_layout="bnc")
+            table = self.attn.relative_position_bias_table
+            if table is None:
+                a = window_attn_fwd_cute_qkvpacked(qkv, heads, group_ids=gids, output_layout="bnc")
+            else:
+                a = window_attn_rel_bias_qkvpacked(qkv, heads, table.detach(), self.attn.buckets(ws, x.device),
+                                                   group_ids=gids, output_layout="bnc")
             Nw = xw.shape[1]
             _rec.end("attention", ev, 4 * T * D * e, 4 * xw.shape[0] * heads * Nw * Nw * (D // heads))
             wp, bp = self._w(self.attn.proj, bf16)
@@ -457,7 +478,7 @@ class BasicLayer3D(nn.Module):
 
     def __init__(self, dim: int, depth: int, num_heads: int, ws, time_dim: int, mlp_ratio: float = 4.0,
                  qkv_bias: bool = True, downsample: Optional[type] = None, upsample: Optional[type] = None,
-                 scale_bias: float = 0.0, precision: str = "bf16_mixed") -> None:
+                 scale_bias: float = 0.0, precision: str = "bf16_mixed", rel_pos_bias: bool = False) -> None:
         super().__init__()
         if downsample is not None and upsample is not None:
             raise ValueError("Cannot set both `downsample` and `upsample`.")
@@ -469,7 +490,7 @@ class BasicLayer3D(nn.Module):
                 dim=dim, num_heads=num_heads, window_size=ws,
                 shift_size=(0, 0, 0) if i % 2 == 0 else (ws[0] // 2, ws[1] // 2, ws[2] // 2),
                 time_dim=time_dim, mlp_ratio=mlp_ratio, qkv_bias=qkv_bias, scale_bias=scale_bias,
-                precision=precision)
+                precision=precision, rel_pos_bias=rel_pos_bias)
             for i in range(depth)
         ])
         self.downsample = downsample(dim=dim) if downsample is not None else None
@@ -553,7 +574,7 @@ class Swin3DTransformerBackbone(nn.Module):
     def __init__(self, embed_dim: int = 96, encoder_depths=(2, 2, 6, 2), encoder_num_heads=(3, 6, 12, 24),
                  decoder_depths=(2, 6, 2, 2), decoder_num_heads=(24, 12, 6, 3), window_size=7,
                  mlp_ratio: float = 4.0, qkv_bias: bool = True, precision: str = "bf16_mixed",
-                 workspace_pool: Optional[InferenceWorkspacePool] = None) -> None:
+                 workspace_pool: Optional[InferenceWorkspacePool] = None, rel_pos_bias: bool = False) -> None:
         super().__init__()
         self.precision = _check_precision(precision)
         self.workspace_pool = workspace_pool
@@ -571,7 +592,7 @@ class Swin3DTransformerBackbone(nn.Module):
             Basic3DEncoderLayer(dim=int(embed_dim * 2 ** i), depth=encoder_depths[i], num_heads=encoder_num_heads[i],
                                 ws=self.window_size, time_dim=embed_dim, mlp_ratio=mlp_ratio, qkv_bias=qkv_bias,
                                 downsample=PatchMerging3D if i < self.num_encoder_layers - 1 else None,
-                                precision=precision)
+                                precision=precision, rel_pos_bias=rel_pos_bias)
             for i in range(self.num_encoder_layers)
         ])
         self.decoder_layers = nn.ModuleList()
@@ -580,7 +601,8 @@ class Swin3DTransformerBackbone(nn.Module):
             self.decoder_layers.append(Basic3DDecoderLayer(
                 dim=int(embed_dim * 2 ** e), depth=decoder_depths[i], num_heads=decoder_num_heads[i],
                 ws=self.window_size, time_dim=embed_dim, mlp_ratio=mlp_ratio, qkv_bias=qkv_bias,
-                upsample=PatchSplitting3D if i < self.num_decoder_layers - 1 else None, precision=precision))
+                upsample=PatchSplitting3D if i < self.num_decoder_layers - 1 else None, precision=precision,
+                rel_pos_bias=rel_pos_bias))
 
     def set_precision(self, precision: str) -> None:
         self.precision = _check_precision(precision)

@@ -140,3 +140,13 @@ def test_abi_refusals_without_a_gpu():
     assert bwd(nbytes=16) == _lib.FA_ERR_INVALID and b"workspace" in lib.fa_last_error()
     assert lib.fa_window_attention_rel_bias_workspace(4, 2, 145) == _lib.FA_ERR_INVALID
     assert lib.fa_window_attention_rel_bias_workspace(4, 2, 16) >= (4 * 2 + 1) * 16 * 16 * 4
+
+
+def test_clamped_window_reads_the_full_windows_buckets():
+    full, small = fa.RelativeBuckets.window((2, 6, 12)), fa.RelativeBuckets.window((2, 3, 4), table_window=(2, 6, 12))
+    assert small.num_buckets == full.num_buckets and small.tokens == 24
+    # tokens of the small window sit at the same offsets inside the full one
+    pos = [(c * 6 + h) * 12 + w for c in range(2) for h in range(3) for w in range(4)]
+    assert torch.equal(small.index, full.index[pos][:, pos])
+    with pytest.raises(ValueError, match="smaller than the window"):
+        fa.RelativeBuckets.window((2, 6, 12), table_window=(2, 6, 11))
