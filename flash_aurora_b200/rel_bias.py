@@ -6,7 +6,7 @@ beside :mod:`flash_aurora_b200.window_attn`, whose kernels take only the 0 / -10
 ``(num_buckets, H)`` is the learned parameter (the ``relative_position_bias_table`` of Swin models);
 :class:`RelativeBuckets` says which bucket each (query, key) pair of a window reads. Gradients reach
 q, k, v (or the packed qkv) and the table. Windows hold 1 to 144 tokens, head_dim is 64, tensors are
-bfloat16 or float32 (3xTF32 products, fp32 accuracy); masks as in ``window_attn``: region ids or a
+bfloat16 or float32 (products of 22-bit operands, fp32 accuracy); masks as in ``window_attn``: region ids or a
 float bias below -50, each adding -100 to a masked logit.
 
 A step may be captured in a CUDA graph; as for any differentiable torch call, no eager autograd graph of the same
@@ -65,6 +65,8 @@ class RelativeBuckets:
         self.index = flat.view(self.tokens, self.tokens).to(torch.int32)
         self.order = order.to(torch.int32)
         self.offsets = torch.searchsorted(values, torch.arange(num_buckets + 1, device=dev)).to(torch.int32)
+        if dev.type == "cuda":  # ready for every stream from here on
+            torch.cuda.current_stream(dev).synchronize()
 
     def to(self, device) -> "RelativeBuckets":
         """These buckets on ``device`` (this object if it is there already)."""

@@ -7,7 +7,7 @@ Tolerances are on the relative L2 norm of each output.
   is 1, 2^-8 at worst), and P, respectively dS, once more before its product: two roundings of at
   most 2^-8 each in quadrature, 1.42 * 2^-8 = 5.6e-3, if every rounding error were the largest one
   and none cancelled.
-* fp32 tensors: 3xTF32 products keep about 2^-21 of a product and the logits reach a few tens, whose
+* fp32 tensors: operands of 22 bits keep about 2^-21 of a product and the logits reach a few tens, whose
   rounding (2^-24 * 32 = 2e-6 of a logit, so of a probability) dominates: 1e-5.
 * the table's gradient of bf16 tensors has no rounding but the fp32 ones: 1e-5 too. A sum that
   cancels to a small part of its terms is measured against the terms: the bound is on the norm over all
@@ -260,3 +260,64 @@ def test_captured_forward_and_backward():
     want = _run(q * 0.5, k, v, table, index, dout)
     for o in outs:
         assert all(torch.equal(x, y) for x, y in zip(o, want))
+
+
+def _uneven(shape, g, bits):
+    """Normal values times a power of two per row, 2^-bits to 2^bits."""
+    x = torch.randn(*shape, device="cuda", generator=g)
+    return x * torch.exp2(torch.randint(-bits, bits + 1, (*shape[:-1], 1), device="cuda", generator=g).float())
+
+
+@pytest.mark.parametrize("N", [5, 33, 144])
+@pytest.mark.parametrize("bits", [20, 40])
+def test_rows_of_any_size_fp32(N, bits):
+    """Rows of v and dout from 2^-bits to 2^bits, one of zeros, one of denormals, and the largest that dP
+    allows (64 terms, 4 deviations of dout's 2^bits, below 2^127) in rows that the mask takes from the others: every element against the sum of the magnitudes of its own terms.
+
+    A logit is off by at most 2^-21 of its terms' magnitudes (a split loses up to 2^-23 per operand, the dropped
+    lo lo 2^-22, the sums' roundings as much again), which q and k of deviation 0.5 keep below 4 in sum
+    after the scale: 2e-6 of a probability, twice that with the row's sum; a product over tokens adds 2^-21 and
+    the roundings of its nine partial sums, 1e-6: 6e-6 for the output and dV. dS takes three such factors (P, dP
+    and delta) and the product one more: 2e-5 for dQ and dK. A masked probability (e^-100 and less) is an fp32
+    number below 2^-126 with a resolution of 2^-149, half of which is 6e-6 of 2^-133: the terms count it with
+    2^-132 more."""
+    g = torch.Generator(device="cuda").manual_seed(N + bits)
+    B, H = 3, 2
+    q, k = (0.5 * torch.randn(B, H, N, 64, device="cuda", generator=g) for _ in range(2))
+    v, dout = _uneven((B, H, N, 64), g, bits), _uneven((B, H, N, 64), g, bits)
+    v[0, 0, 0] = 0
+    dout[1, 0, 1] = 0
+    v[1, 1, 2] = 1e-40
+    ids = torch.zeros(1, N, dtype=torch.uint8, device="cuda")
+    ids[0, N - 1] = 1  # a key for itself only
+    v[2, :, N - 1] = 2.0 ** (127 - 6 - 2 - bits)
+    dout[2, :, N - 1] = 0
+    table = torch.randn(2 * N - 1, H, device="cuda", generator=g)
+    index = torch.randint(0, 2 * N - 1, (N, N), device="cuda", generator=g)
+    got = _run(q, k, v, table, index, dout, group_ids=ids)
+    Q, K, V, G = (t.double() for t in (q, k, v, dout))
+    x = Q @ K.transpose(-1, -2) * 0.125 + table.double()[index].permute(2, 0, 1) - 100.0 * (ids[:, :, None] != ids[:, None, :]).double()
+    P = torch.softmax(x, -1)
+    P_size = P + 2.0 ** -132
+    dP = G @ V.transpose(-1, -2)
+    size = G.abs() @ V.abs().transpose(-1, -2)  # of dP's terms
+    dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+    dS_size = P_size * (size + (P_size * size).sum(-1, keepdim=True))
+    T = lambda t: t.transpose(-1, -2)  # noqa: E731
+    want = {"out": (P @ V, P_size @ V.abs(), 6e-6), "dq": (0.125 * dS @ K, 0.125 * dS_size @ K.abs(), 2e-5),
+            "dk": (0.125 * T(dS) @ Q, 0.125 * T(dS_size) @ Q.abs(), 2e-5), "dv": (T(P) @ G, T(P_size) @ G.abs(), 6e-6)}
+    for x, (name, (ref, terms, tol)) in zip(got, want.items()):
+        assert torch.isfinite(x).all(), name
+        worst = ((x.double() - ref).abs() / (terms + 1e-37)).max()
+        assert float(worst) <= tol, (name, float(worst))
+
+
+def test_infinity_and_nan_reach_their_own_rows_only():
+    q, k, v, dout, table, index = _inputs(2, 2, 40, FP32)
+    clean = _run(q, k, v, table, index, dout)[0]
+    q2 = q.clone()
+    q2[0, 1, 3, 5], q2[1, 0, 7, 0] = float("nan"), float("inf")
+    out = _run(q2, k, v, table, index, dout)[0]
+    bad = torch.zeros(2, 2, 40, dtype=torch.bool, device="cuda")
+    bad[0, 1, 3] = bad[1, 0, 7] = True
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[~bad])
