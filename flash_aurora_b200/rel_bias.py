@@ -126,6 +126,8 @@ def _check_bias(table: torch.Tensor, buckets: RelativeBuckets, H: int, N: int, d
 def _strided(t: torch.Tensor) -> torch.Tensor:
     """``t (Bwin, H, N, Dh)`` as the kernels can read it: unit head-dim stride, positive strides of
     whole 16-byte units, an aligned base; anything else is copied."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     unit = 16 // t.element_size()
     if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
             and all(s > 0 and s % unit == 0 or n == 1 for s, n in zip(t.stride()[:3], t.shape[:3]))):
@@ -149,8 +151,9 @@ def _bytes(which: str, device: int, *args: int) -> int:
 # An operand of the kernels: its address and the strides of window, head and token (elements).
 def _heads(t: torch.Tensor) -> tuple:
     """``(Bwin, H, N, Dh)``; an axis of one entry gets a legal stride."""
-    n, s = t.shape, t.stride()
-    return (t.data_ptr(), *(s[i] if n[i] > 1 else _HEAD_DIM for i in range(3)))
+    w, h, n, _ = t.shape
+    sw, sh, sn, _ = t.stride()
+    return (t.data_ptr(), sw if w > 1 else _HEAD_DIM, sh if h > 1 else _HEAD_DIM, sn if n > 1 else _HEAD_DIM)
 
 
 def _bnc(t: torch.Tensor) -> tuple:
@@ -165,9 +168,11 @@ def _qkv(t: torch.Tensor) -> tuple:
     return tuple((t.data_ptr() + i * step, t.shape[1] * row, _HEAD_DIM, row) for i in range(3))
 
 
+_STRIDES4, _STRIDES7 = ctypes.c_int64 * 12, ctypes.c_int64 * 21
+
+
 def _strides(*ops: tuple):
-    flat = [s for o in ops for s in o[1:]]
-    return (ctypes.c_int64 * len(flat))(*flat)
+    return (_STRIDES4 if len(ops) == 4 else _STRIDES7)(*[s for o in ops for s in o[1:]])
 
 
 class _Call:
@@ -222,7 +227,7 @@ def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, state, stats, table_
 class _Attn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, mask, call):
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         state = _forward(_heads(q), _heads(k), _heads(v), _heads(out), table, mask, call, True)
         ctx.save_for_backward(q, k, v, mask, *state)
         ctx.call, ctx.table_dtype = call, table.dtype
@@ -234,7 +239,7 @@ class _Attn(torch.autograd.Function):
         q, k, v, mask, state, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         dout = _strided(dout)
-        dq, dk, dv = (torch.empty(q.shape, device=q.device, dtype=q.dtype) for _ in range(3))
+        dq, dk, dv = (torch.empty_like(q, memory_format=torch.contiguous_format) for _ in range(3))
         dtable = _backward(*(_heads(t) for t in (q, k, v, dout, dq, dk, dv)), mask, ctx.call, state, stats,
                            ctx.table_dtype if need[3] else None)
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None
