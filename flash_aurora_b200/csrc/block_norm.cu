@@ -623,7 +623,10 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
   }
 }
 
-// Column sums over blocks (and batch elements, for a shared parameter), in double.
+// Column sums over blocks (and batch elements, for a shared parameter), in double, by blockDim.y rows of threads:
+// 32 for more than 128 blocks, else 8. Bound by the latency of the loads where each thread makes many (296
+// blocks of 771 columns: 7.5 us with 32 rows, 22 with 8), by the threads where it makes few (2 x 74 blocks of
+// 2048 columns: 32 us with 32 rows, 24 with 8).
 struct SumArgs {
   const float* ws;
   float* out[kParams];
@@ -631,7 +634,7 @@ struct SumArgs {
   int first;  // parameter of sum 0
   int sums, blocks, B, D;
 };
-constexpr int kSumRows = 8;
+constexpr int kSumRows = 32;  // at most
 
 __global__ void __launch_bounds__(32 * kSumRows) block_norm_sum_kernel(const SumArgs a) {
   const int i = blockIdx.z, c = blockIdx.x * 32 + threadIdx.x;
@@ -643,14 +646,14 @@ __global__ void __launch_bounds__(32 * kSumRows) block_norm_sum_kernel(const Sum
     double s = 0.0;
     if (c < a.D) {
 #pragma unroll 8
-      for (int64_t e = lo + threadIdx.y; e < hi; e += kSumRows) s += (double)a.ws[(e * a.sums + i) * a.D + c];
+      for (int64_t e = lo + threadIdx.y; e < hi; e += blockDim.y) s += (double)a.ws[(e * a.sums + i) * a.D + c];
     }
     __shared__ double part[kSumRows][32];
     __syncthreads();
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && c < a.D) {
-      for (int y = 1; y < kSumRows; ++y) s += part[y][threadIdx.x];
+      for (int y = 1; y < blockDim.y; ++y) s += part[y][threadIdx.x];
       out[(int64_t)b * a.D + c] = (float)s;
     }
   }
@@ -694,7 +697,10 @@ int sums_of(int form) { return form == kBefore ? 2 : form == kAfter ? 4 : 6; }
 
 template <typename XT, typename YT, int kForm>
 int launch_fwd(NormArgs& a, bool vec, cudaStream_t s) {
-  const bool wide = a.D > 512;
+  // 16 elements per thread or 32. Vector rows above 512 columns take 32, since a reduction over fewer warps costs
+  // less than the occupancy gains; element-wise rows, bound by their instructions and with spills at 32,
+  // keep 16 as long as a block covers a row (21003 fp32 rows of 771: 58 us against 103).
+  const bool wide = a.D > (vec ? 512 : 16 * kFwdThreads);
   a.tpr = pow2_at_least((int)ceil_div(a.D, wide ? 32 : 16));
   const int groups = kFwdThreads / a.tpr;
   auto kern = vec ? (wide ? block_norm_kernel<XT, YT, kForm, true, 4> : block_norm_kernel<XT, YT, kForm, true, 2>)
@@ -865,6 +871,7 @@ extern "C" int fa_block_norm_backward(int form, int norm, const void* x, int x_d
   }
   if (!any) return FA_OK;
   const unsigned gy = own ? (unsigned)(sh.B < 65535 ? sh.B : 65535) : 1u;
-  block_norm_sum_kernel<<<dim3((unsigned)ceil_div(D, 32), gy, (unsigned)m.sums), dim3(32, kSumRows), 0, s>>>(m);
+  const unsigned rows = (own ? sh.blocks : sh.B * sh.blocks) > 128 ? kSumRows : 8;
+  block_norm_sum_kernel<<<dim3((unsigned)ceil_div(D, 32), gy, (unsigned)m.sums), dim3(32, rows), 0, s>>>(m);
   return check_launch("block_norm_sum_kernel");
 }
