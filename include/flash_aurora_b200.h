@@ -283,7 +283,8 @@ int fa_window_attention_bias_noalloc(int precision, int64_t Bwin, int64_t H, int
  * counterpart in the reference, whose attention takes only the 0 / -100 mask):
  *   out = softmax(q k^T * scale + table[index, h] + mask) v
  * q, k, v, out: (Bwin, H, N, Dh) with element strides {q, k, v, out} x {window, head, token},
- * head-dim stride 1, 16-byte aligned, strides multiples of 16 bytes; Dh == 64, 1 <= N <= 144.
+ * head-dim stride 1, 16-byte aligned, strides multiples of 16 bytes; Dh == 64, 1 <= N <= 144. precision:
+ * FA_ATTN_BF16 or FA_ATTN_FP32_3XTF32 (fp32 tensors; here the operands are pairs of halves, 22 bits).
  * table (num_buckets, H) contiguous, FA_F32 or FA_BF16; index (N, N) int32, the bucket of (query,
  * key), every value in [0, num_buckets). Masks as in fa_window_attention (region ids of any form).
  * state (fa_window_attention_rel_bias_state(precision, H, nW with region ids, else 0) bytes, 16-byte aligned)
