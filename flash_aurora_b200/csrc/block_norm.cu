@@ -623,10 +623,8 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
   }
 }
 
-// Column sums over blocks (and batch elements, for a shared parameter), in double, by blockDim.y rows of threads:
-// 32 for more than 128 blocks, else 8. Bound by the latency of the loads where each thread makes many (296
-// blocks of 771 columns: 7.5 us with 32 rows, 22 with 8), by the threads where it makes few (2 x 74 blocks of
-// 2048 columns: 32 us with 32 rows, 24 with 8).
+// Column sums over blocks (and batch elements, for a shared parameter), in double; the partials are still in L2.
+// Eight rows of threads: 9 us for 2 x 148 partials of 6 x 2048 columns (19 with 32 rows), 8 us for 296 of 4 x 771 (9).
 struct SumArgs {
   const float* ws;
   float* out[kParams];
@@ -634,7 +632,7 @@ struct SumArgs {
   int first;  // parameter of sum 0
   int sums, blocks, B, D;
 };
-constexpr int kSumRows = 32;  // at most
+constexpr int kSumRows = 8;
 
 __global__ void __launch_bounds__(32 * kSumRows) block_norm_sum_kernel(const SumArgs a) {
   const int i = blockIdx.z, c = blockIdx.x * 32 + threadIdx.x;
@@ -646,14 +644,14 @@ __global__ void __launch_bounds__(32 * kSumRows) block_norm_sum_kernel(const Sum
     double s = 0.0;
     if (c < a.D) {
 #pragma unroll 8
-      for (int64_t e = lo + threadIdx.y; e < hi; e += blockDim.y) s += (double)a.ws[(e * a.sums + i) * a.D + c];
+      for (int64_t e = lo + threadIdx.y; e < hi; e += kSumRows) s += (double)a.ws[(e * a.sums + i) * a.D + c];
     }
     __shared__ double part[kSumRows][32];
     __syncthreads();
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && c < a.D) {
-      for (int y = 1; y < blockDim.y; ++y) s += part[y][threadIdx.x];
+      for (int y = 1; y < kSumRows; ++y) s += part[y][threadIdx.x];
       out[(int64_t)b * a.D + c] = (float)s;
     }
   }
@@ -871,7 +869,6 @@ extern "C" int fa_block_norm_backward(int form, int norm, const void* x, int x_d
   }
   if (!any) return FA_OK;
   const unsigned gy = own ? (unsigned)(sh.B < 65535 ? sh.B : 65535) : 1u;
-  const unsigned rows = (own ? sh.blocks : sh.B * sh.blocks) > 128 ? kSumRows : 8;
-  block_norm_sum_kernel<<<dim3((unsigned)ceil_div(D, 32), gy, (unsigned)m.sums), dim3(32, rows), 0, s>>>(m);
+  block_norm_sum_kernel<<<dim3((unsigned)ceil_div(D, 32), gy, (unsigned)m.sums), dim3(32, kSumRows), 0, s>>>(m);
   return check_launch("block_norm_sum_kernel");
 }
