@@ -695,10 +695,14 @@ int sums_of(int form) { return form == kBefore ? 2 : form == kAfter ? 4 : 6; }
 
 template <typename XT, typename YT, int kForm>
 int launch_fwd(NormArgs& a, bool vec, cudaStream_t s) {
-  // 16 elements per thread or 32. Vector rows above 512 columns take 32, since a reduction over fewer warps costs
-  // less than the occupancy gains; element-wise rows, bound by their instructions and with spills at 32,
-  // keep 16 as long as a block covers a row (21003 fp32 rows of 771: 58 us against 103).
-  const bool wide = a.D > (vec ? 512 : 16 * kFwdThreads);
+  // 16 elements per thread or 32 (fewer warps a reduction, fewer warps an SM). 64M bf16 elements with an fp32
+  // residual, in us at 32 / 16:      520        768        1024       1536       2048 columns
+  //   before                       114 / 134   82 / 92    68 / 74    92 / 113   74 / 89
+  //   after                        111 / 131  124 / 107  121 / 120  120 / 119  125 / 103
+  //   between                      216 / 244  157 / 171  142 / 138  179 / 205  150 / 165
+  // so 32 above 512 columns, but for `after` below 768 only. Element-wise rows, bound by their instructions and with
+  // spills at 32, keep 16 as long as a block covers a row (21003 fp32 rows of 771: 57 us against 103).
+  const bool wide = a.D > (!vec || (kForm == kAfter && a.D >= 768) ? 16 * kFwdThreads : 512);
   a.tpr = pow2_at_least((int)ceil_div(a.D, wide ? 32 : 16));
   const int groups = kFwdThreads / a.tpr;
   auto kern = vec ? (wide ? block_norm_kernel<XT, YT, kForm, true, 4> : block_norm_kernel<XT, YT, kForm, true, 2>)
