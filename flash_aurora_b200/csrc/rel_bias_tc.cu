@@ -645,8 +645,8 @@ constexpr int kOffRanks = kOffP + kPBytes;
 constexpr int kOffBars = kOffRanks + kStages * kMaxN;
 constexpr int kOffDs = (kOffP + kPBytes + 1023) / 1024 * 1024;
 constexpr int kOffStats = kOffDs + kPBytes, kStatsBytes = kMaxN * 8;
-constexpr int kMaskSlots = 4;  // mask steps built at once in the P buffer
-static_assert(kMaskSlots * kMaskOpBytes <= kPBytes, "mask operands fit the P buffer");
+constexpr int kMaskSlots = 4;  // mask steps built at once in the dS buffer
+static_assert(kMaskSlots * kMaskOpBytes <= kPBytes, "mask operands fit the dS buffer");
 enum { kFull = 0, kStaged = 2, kSMain = 4, kSRem, kPMain, kPRem, kDvFull, kDsMain, kDsRem, kDqFull, kRemFull, kDkFull,
        kDqFree, kTFree, kStats, kInfo, kMaskMore, kMaskEmpty, kDone, kNumBars };
 static_assert(kOffBars + kNumBars * 8 + 24 <= kOffDs, "barriers and words fit the gap");

@@ -164,3 +164,50 @@ def test_training_step(dtype, tol):
     for name, a, b in zip(own, grads, grads_ref):
         assert a.dtype == own[name].dtype and rel_l2(a, b) <= tol, (name, rel_l2(a, b))
     assert fa.device_status() == {"attention": 0, "gemm": 0}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_calls_at_once(dtype):
+    """Steps on two streams that run at the same time give the bits that they give alone."""
+    B, H = 48, 4
+    buckets = fa.RelativeBuckets.window(WS, "cuda")
+    ids = (torch.arange(144, device="cuda") >= 72).to(torch.uint8).view(1, -1)
+
+    def step(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        qkv = torch.randn(B, 144, 3 * H * 64, device="cuda", generator=g).to(dtype).requires_grad_(True)
+        table = torch.randn(buckets.num_buckets, H, device="cuda", generator=g).requires_grad_(True)
+        gate = torch.randn(H * 64, device="cuda", generator=g).requires_grad_(True)
+        a = fa.window_attn_rel_bias_qkvpacked(qkv, H, table, buckets, group_ids=ids, output_layout="bnc")
+        y, z = fa.block_postnorm_residual_prenorm(a.detach(), a, gate=gate)
+        return y, z, *torch.autograd.grad((y, z), (qkv, table, gate), (y.detach(), z.detach()))
+
+    alone = [step(s) for s in (0, 1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = step(i)
+    torch.cuda.synchronize()
+    for a, b in zip(alone, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_captured_block_with_a_bias():
+    blk, x, c = _block("bf16_mixed", RES)
+    with torch.no_grad():
+        want = blk(x, c, RES)
+        static = torch.zeros_like(x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            blk(static, c, RES)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = blk(static, c, RES)
+        static.copy_(x)
+        graph.replay()
+        assert torch.equal(out, want)
