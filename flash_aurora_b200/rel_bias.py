@@ -189,23 +189,24 @@ class _Call:
 
 
 def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool):
-    """Launch the forward kernels into the operand ``out``; returns the state that the backward pass reads, and the
-    row statistics when asked for."""
+    """Launch the forward kernels into the operand ``out``; returns the state that the backward pass reads, with the
+    row statistics in it when asked for."""
     Bwin, H, N = call.shape
     dev = call.device
     with _lib.on_device(dev):
-        stats = torch.empty(Bwin, H, _MAX_TOKENS, 2, device=dev, dtype=torch.float32) if want_stats else None
         n = _bytes("state", dev.index, call.precision, H, call.nW if call.kind == "group_ids" else 0)
-        state = torch.empty(n, dtype=torch.uint8, device=dev)
+        at = (n + 15) // 16 * 16  # of the row statistics, in the same buffer
+        state = torch.empty(at + Bwin * H * _MAX_TOKENS * 8 if want_stats else n, dtype=torch.uint8, device=dev)
         rc = _lib.load().fa_window_attention_rel_bias(
             call.precision, Bwin, H, N, _HEAD_DIM, q[0], k[0], v[0], out[0], _strides(q, k, v, out), table.data_ptr(),
             _lib.dtype_code(table.dtype), call.buckets.index.data_ptr(), *call.masks(mask), state.data_ptr(),
-            _ptr(stats), _lib.stream_ptr(dev))
+            state.data_ptr() + at if want_stats else None, _lib.stream_ptr(dev))
         _lib.check(rc, "window_attn_rel_bias")
-    return state, stats
+    call.stats_at = at
+    return state
 
 
-def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, state, stats, table_dtype) -> Optional[torch.Tensor]:
+def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, state, table_dtype) -> Optional[torch.Tensor]:
     """Launch the backward kernels into the operands ``dq``, ``dk``, ``dv``; returns the table's gradient, in
     ``table_dtype`` (None: not asked for)."""
     Bwin, H, N = call.shape
@@ -217,8 +218,8 @@ def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, state, stats, table_
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         rc = _lib.load().fa_window_attention_rel_bias_backward(
             call.precision, Bwin, H, N, _HEAD_DIM, q[0], k[0], v[0], dout[0], dq[0], dk[0], dv[0],
-            _strides(q, k, v, dout, dq, dk, dv), *call.masks(mask), state.data_ptr(), stats.data_ptr(),
-            b.order.data_ptr(), b.offsets.data_ptr(), b.num_buckets, _ptr(dtable),
+            _strides(q, k, v, dout, dq, dk, dv), *call.masks(mask), state.data_ptr(),
+            state.data_ptr() + call.stats_at, b.order.data_ptr(), b.offsets.data_ptr(), b.num_buckets, _ptr(dtable),
             _lib.dtype_code(table_dtype or torch.float32), ws.data_ptr(), n, _lib.stream_ptr(dev))
         _lib.check(rc, "window_attn_rel_bias backward")
     return dtable
@@ -229,18 +230,18 @@ class _Attn(torch.autograd.Function):
     def forward(ctx, q, k, v, table, mask, call):
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         state = _forward(_heads(q), _heads(k), _heads(v), _heads(out), table, mask, call, True)
-        ctx.save_for_backward(q, k, v, mask, *state)
+        ctx.save_for_backward(q, k, v, mask, state)
         ctx.call, ctx.table_dtype = call, table.dtype
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, mask, state, stats = ctx.saved_tensors
+        q, k, v, mask, state = ctx.saved_tensors
         need = ctx.needs_input_grad
         dout = _strided(dout)
         dq, dk, dv = (torch.empty_like(q, memory_format=torch.contiguous_format) for _ in range(3))
-        dtable = _backward(*(_heads(t) for t in (q, k, v, dout, dq, dk, dv)), mask, ctx.call, state, stats,
+        dtable = _backward(*(_heads(t) for t in (q, k, v, dout, dq, dk, dv)), mask, ctx.call, state,
                            ctx.table_dtype if need[3] else None)
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None
 
@@ -249,21 +250,21 @@ class _AttnPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, table, mask, call, bnc):
         out, state = _packed_forward(qkv, table, mask, call, bnc, True)
-        ctx.save_for_backward(qkv, mask, *state)
+        ctx.save_for_backward(qkv, mask, state)
         ctx.call, ctx.table_dtype, ctx.bnc = call, table.dtype, bnc
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, mask, state, stats = ctx.saved_tensors
+        qkv, mask, state = ctx.saved_tensors
         dqkv = torch.empty_like(qkv)
         if ctx.bnc:
             dout = dout.contiguous()
             dout = dout if dout.data_ptr() % 16 == 0 else dout.clone()
         else:
             dout = _strided(dout)
-        dtable = _backward(*_qkv(qkv), _bnc(dout) if ctx.bnc else _heads(dout), *_qkv(dqkv), mask, ctx.call, state, stats,
+        dtable = _backward(*_qkv(qkv), _bnc(dout) if ctx.bnc else _heads(dout), *_qkv(dqkv), mask, ctx.call, state,
                            ctx.table_dtype if ctx.needs_input_grad[1] else None)
         return dqkv if ctx.needs_input_grad[0] else None, dtable, None, None, None
 
