@@ -294,6 +294,7 @@ extern "C" int fa_window_attention_rel_bias_backward(
   cudaStream_t s = (cudaStream_t)stream;
   const int64_t need = fa_window_attention_rel_bias_workspace(Bwin, H, N);
   FA_REQUIRE(Bwin == 0 || (workspace && workspace_bytes >= need), FA_ERR_INVALID, "workspace too small");
+  FA_REQUIRE(Bwin == 0 || aligned16(workspace), FA_ERR_INVALID, "the workspace must be 16-byte aligned");
   const int grid = grid_of(Bwin * H);
   if (Bwin > 0) {
     Params p{};
