@@ -189,7 +189,7 @@ __device__ __forceinline__ void param8(const float* p, int t, int tpr, int D, in
 // ------------------------------------------------------------------------------------------
 struct Group {
   int tpr, id, t;  // threads per row, row group in the block, thread in the group
-  float* buf;      // 2 x 2 x (tpr / 32) floats of this group
+  float2* buf;     // two buffers of (tpr / 32) partial sums of this group, read in pairs
   int par;
 };
 
@@ -204,7 +204,7 @@ __device__ __forceinline__ void group_sum(Group& g, float (&v)[kVals]) {
   }
   if (g.tpr > 32) {
     const int warps = g.tpr >> 5;
-    float* b = g.buf + g.par * kVals * warps;
+    float* b = reinterpret_cast<float*>(g.buf) + g.par * kVals * warps;
     g.par ^= 1;
     if ((g.t & 31) == 0) {
 #pragma unroll
@@ -280,13 +280,13 @@ __global__ void __launch_bounds__(kFwdThreads, kVpt == 2 ? 3 : 2) block_norm_ker
   using ColR = Column<YT, kVec, kN>;
   constexpr int kStage = (ColX::kBytes + (kForm == kBefore ? 0 : ColR::kBytes)) * kFwdThreads;
   extern __shared__ __align__(16) uint8_t ring_mem[];
-  __shared__ float buf[2 * kFwdThreads / 32];
+  __shared__ float2 buf[kFwdThreads / 32];
   const uint32_t ring = smem_addr(ring_mem);
   Group g;
   g.tpr = a.tpr;
   g.id = threadIdx.x / a.tpr;
   g.t = threadIdx.x - g.id * a.tpr;
-  g.buf = buf + 2 * (g.id * a.tpr >> 5);
+  g.buf = buf + (g.id * a.tpr >> 5);
   g.par = 0;
   const int groups = kFwdThreads / a.tpr, D = a.D;
   const int64_t step = (int64_t)gridDim.x * groups;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
   using ColZ = Column<ZT, kVec, 8>;
   constexpr int kX = ColX::kBytes, kR = kForm == kBefore ? 0 : ColY::kBytes, kZ = kForm == kAfter ? 0 : ColZ::kBytes;
   extern __shared__ __align__(16) uint8_t ring_mem[];
-  __shared__ float buf[4 * kBwdMaxThreads / 32];
+  __shared__ float2 buf[2 * kBwdMaxThreads / 32];
   float* comb = reinterpret_cast<float*>(ring_mem);  // after the rows
   const uint32_t ring = smem_addr(ring_mem), stage_bytes = (kX + 2 * kR + kZ) * blockDim.x;
   // After the ring (or the sums, whichever is larger): the parameters.
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kBwdMaxThreads, 1) block_norm_bwd_kernel(const
   g.tpr = a.tpr;
   g.id = threadIdx.x / a.tpr;
   g.t = threadIdx.x - g.id * a.tpr;
-  g.buf = buf + 4 * (g.id * a.tpr >> 5);
+  g.buf = buf + 2 * (g.id * a.tpr >> 5);
   g.par = 0;
   const int groups = blockDim.x / a.tpr, D = a.D, threads = blockDim.x;
   const int64_t step = (int64_t)gridDim.x * groups;
