@@ -40,7 +40,8 @@ class RelativeBuckets:
     ``[0, num_buckets)``, with the pairs of each bucket listed for the table's gradient.
 
     Built once per window shape and device (the range check reads the index on the host). The index
-    is copied: changing the given tensor later has no effect.
+    is copied: changing the given tensor later has no effect. Any stream may use it; a captured graph reads it
+    at every replay, so it has to live as long as the graph.
     """
 
     def __init__(self, index: torch.Tensor, num_buckets: int, device: Optional[torch.device] = None) -> None:
@@ -65,8 +66,21 @@ class RelativeBuckets:
         self.index = flat.view(self.tokens, self.tokens).to(torch.int32)
         self.order = order.to(torch.int32)
         self.offsets = torch.searchsorted(values, torch.arange(num_buckets + 1, device=dev)).to(torch.int32)
+        self._stream = None  # of a GPU's lists: the stream (handle) that their memory belongs to
         if dev.type == "cuda":  # ready for every stream from here on
-            torch.cuda.current_stream(dev).synchronize()
+            stream = torch.cuda.current_stream(dev)
+            stream.synchronize()
+            self._stream = stream.cuda_stream
+
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "_stream": None}  # a copy's memory may belong to another stream
+
+    def _used_by(self, stream: torch.cuda.Stream, *tensors: torch.Tensor) -> None:
+        """``stream`` is about to read these tensors: their memory is not given away before it has, even if
+        this object is dropped meanwhile."""
+        if stream.cuda_stream != self._stream:
+            for t in tensors:
+                t.record_stream(stream)
 
     def to(self, device) -> "RelativeBuckets":
         """These buckets on ``device`` (this object if it is there already)."""
@@ -194,13 +208,15 @@ def _forward(q, k, v, out, table, mask, call: _Call, want_stats: bool):
     Bwin, H, N = call.shape
     dev = call.device
     with _lib.on_device(dev):
+        stream = torch.cuda.current_stream(dev)
+        call.buckets._used_by(stream, call.buckets.index)
         n = _bytes("state", dev.index, call.precision, H, call.nW if call.kind == "group_ids" else 0)
         at = (n + 15) // 16 * 16  # of the row statistics, in the same buffer
         state = torch.empty(at + Bwin * H * _MAX_TOKENS * 8 if want_stats else n, dtype=torch.uint8, device=dev)
         rc = _lib.load().fa_window_attention_rel_bias(
             call.precision, Bwin, H, N, _HEAD_DIM, q[0], k[0], v[0], out[0], _strides(q, k, v, out), table.data_ptr(),
             _lib.dtype_code(table.dtype), call.buckets.index.data_ptr(), *call.masks(mask), state.data_ptr(),
-            state.data_ptr() + at if want_stats else None, _lib.stream_ptr(dev))
+            state.data_ptr() + at if want_stats else None, stream.cuda_stream)
         _lib.check(rc, "window_attn_rel_bias")
     call.stats_at = at
     return state
@@ -213,6 +229,8 @@ def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, state, table_dtype) 
     dev = call.device
     b = call.buckets
     with _lib.on_device(dev):
+        stream = torch.cuda.current_stream(dev)
+        b._used_by(stream, b.order, b.offsets)
         dtable = None if table_dtype is None else torch.empty(b.num_buckets, H, device=dev, dtype=table_dtype)
         n = _bytes("workspace", dev.index, Bwin, H, N)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
@@ -220,7 +238,7 @@ def _backward(q, k, v, dout, dq, dk, dv, mask, call: _Call, state, table_dtype) 
             call.precision, Bwin, H, N, _HEAD_DIM, q[0], k[0], v[0], dout[0], dq[0], dk[0], dv[0],
             _strides(q, k, v, dout, dq, dk, dv), *call.masks(mask), state.data_ptr(),
             state.data_ptr() + call.stats_at, b.order.data_ptr(), b.offsets.data_ptr(), b.num_buckets, _ptr(dtable),
-            _lib.dtype_code(table_dtype or torch.float32), ws.data_ptr(), n, _lib.stream_ptr(dev))
+            _lib.dtype_code(table_dtype or torch.float32), ws.data_ptr(), n, stream.cuda_stream)
         _lib.check(rc, "window_attn_rel_bias backward")
     return dtable
 

@@ -2,8 +2,14 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
+from types import SimpleNamespace
 
+import torch
+
+import flash_aurora_b200 as fa
 from flash_aurora_b200 import _lib
 
 P = ctypes.c_void_p(1 << 20)
@@ -30,3 +36,29 @@ def test_workspace_size_is_exact():
     need = (8 + 2) * 144 * 144 * 4
     assert lib.fa_window_attention_rel_bias_workspace(4, 2, 16) == need
     assert _backward(P, need - 1) == _lib.FA_ERR_INVALID and b"workspace" in lib.fa_last_error()
+
+
+class _Recorded:
+    def __init__(self):
+        self.streams = []
+
+    def record_stream(self, s):
+        self.streams.append(s)
+
+
+def test_buckets_are_recorded_with_other_streams():
+    """Only a stream other than the one that the lists' memory belongs to has to be recorded; of a copy the
+    owner is unknown, so every stream is."""
+    b = fa.RelativeBuckets.window((1, 2, 3))
+    own, other = SimpleNamespace(cuda_stream=16), SimpleNamespace(cuda_stream=32)
+    b._stream = 16
+    t, u = _Recorded(), _Recorded()
+    b._used_by(own, t, u)
+    assert t.streams == u.streams == []
+    b._used_by(other, t, u)
+    assert t.streams == u.streams == [other]
+    for c in (copy.copy(b), copy.deepcopy(b), pickle.loads(pickle.dumps(b))):
+        assert torch.equal(c.index, b.index) and c.num_buckets == b.num_buckets
+        t = _Recorded()
+        c._used_by(own, t)
+        assert t.streams == [own]

@@ -1,0 +1,55 @@
+"""Edges of window attention with a relative position bias on the GPU: the calls that its documentation
+allows and that the parity tests leave out."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import flash_aurora_b200 as fa
+from test_rel_bias_gpu import _inputs
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_buckets_dropped_while_another_stream_reads_them(train):
+    """Buckets built on one stream, used on a second whose work is held back, and dropped: the first stream's
+    next allocations must not get their memory. Nothing is written into those allocations."""
+    q, k, v, dout, table, index = _inputs(3, 2, 100, BF16, seed=1)
+    q = q.requires_grad_(train)
+    table = table.requires_grad_(train)
+    builder, user = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def call(buckets):
+        out = fa.window_attn_rel_bias(q, k, v, table, buckets)
+        return torch.autograd.grad(out, (q, table), dout) if train else out
+
+    def ranges(tensors):
+        return [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors]
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(user):
+        call(fa.RelativeBuckets(index, table.shape[0]))  # what is loaded or allocated once
+    torch.cuda.synchronize()
+    with torch.cuda.stream(builder):
+        buckets = fa.RelativeBuckets(index, table.shape[0])
+    read = [buckets.index] + ([buckets.order, buckets.offsets] if train else [])
+    mine = ranges(read)
+    sizes = [t.numel() for t in read]
+    del read
+    with torch.cuda.stream(user):
+        torch.cuda._sleep(400_000_000)  # about a fifth of a second
+        result = call(buckets)
+    del buckets
+    with torch.cuda.stream(builder):
+        fresh = [torch.empty(n, dtype=torch.int32, device="cuda") for n in sizes for _ in range(8)]
+    assert not user.query()  # the calls are still behind the wait
+    for lo, hi in ranges(fresh):
+        assert all(hi <= a or b <= lo for a, b in mine)
+    torch.cuda.synchronize()
+    want = call(fa.RelativeBuckets(index, table.shape[0]))
+    for a, b in zip(result if train else [result], want if train else [want]):
+        assert torch.equal(a, b)
