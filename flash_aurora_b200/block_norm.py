@@ -14,7 +14,8 @@ Tensors are ``(B, L, D)``, float32 or bfloat16, ``D <= 4096``. Scales, shifts, g
 ``None`` counts as zero for a scale or shift and as one for a gate. With ``scale_bias=0`` a scale is
 an ordinary norm weight; with the default of one it is a modulation. Everything is computed in fp32
 and each output is rounded once; sums over rows run in a fixed order, so equal calls give equal bits.
-Gradients of gradients are not available. A step may be captured in a CUDA graph; as for any differentiable
+Gradients of gradients are not available; forward-mode derivatives and calls inside ``torch.func`` transforms
+(``vmap``, ``grad``, ``jvp``) are refused, and ``torch.compile`` is not supported. A step may be captured in a CUDA graph; as for any differentiable
 torch call, no eager autograd graph of the same leaves may be alive then (torch refuses such a capture).
 """
 
@@ -151,6 +152,7 @@ def _check(what: str, x: torch.Tensor, residual: Optional[torch.Tensor], params,
 
 
 def _run(what, call, x, residual, params, norm):
+    _lib.refuse_forward_ad(what, x, residual, *params)
     _check(what, x, residual, params, norm)
     call.norm = _NORMS[norm]
     x = x.contiguous()

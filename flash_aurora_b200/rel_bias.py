@@ -14,7 +14,8 @@ leaves may be alive then (torch refuses such a capture).
 
 Nothing is kept between calls: the backward pass recomputes the probabilities from q, k, the table
 and the row statistics of its own forward call. Sums run in a fixed order, so equal calls give equal
-bits. Gradients of gradients are not available.
+bits. Gradients of gradients are not available; forward-mode derivatives and calls inside ``torch.func``
+transforms (``vmap``, ``grad``, ``jvp``) are refused, and ``torch.compile`` is not supported.
 """
 
 from __future__ import annotations
@@ -331,6 +332,7 @@ def window_attn_rel_bias(
     """Attention on ``q, k, v (Bwin, H, N, 64)`` (bfloat16 or float32, one dtype) with the bias
     ``table[buckets.index, h]`` and an optional mask: ``bias (nW, N, N)`` (below -50 means masked) or
     ``group_ids (nW, N)`` uint8. Window ``b`` reads mask ``b % nW``. Returns ``(Bwin, H, N, 64)``."""
+    _lib.refuse_forward_ad("window_attn_rel_bias", q, k, v, table)
     if q.ndim != 4 or q.shape != k.shape or q.shape != v.shape:
         raise ValueError("q, k, v must all be (Bwin, H, N, Dh)")
     if q.dtype not in (torch.bfloat16, torch.float32):
@@ -367,6 +369,7 @@ def window_attn_rel_bias_qkvpacked(
 ) -> torch.Tensor:
     """:func:`window_attn_rel_bias` on the packed ``Linear(D, 3D)`` output ``(Bwin, N, 3 * H * 64)``,
     contiguous. Returns ``(Bwin, H, N, 64)``, or ``(Bwin, N, H * 64)`` with ``output_layout="bnc"``."""
+    _lib.refuse_forward_ad("window_attn_rel_bias_qkvpacked", qkv, table)
     if qkv.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"qkv-packed path supports bfloat16 and float32; got {qkv.dtype}")
     if qkv.ndim != 3:

@@ -7,7 +7,9 @@ import ctypes
 import pickle
 from types import SimpleNamespace
 
+import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flash_aurora_b200 as fa
 from flash_aurora_b200 import _lib
@@ -62,3 +64,25 @@ def test_buckets_are_recorded_with_other_streams():
         t = _Recorded()
         c._used_by(own, t)
         assert t.streams == [own]
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent would be lost; its primal alone goes on to the next check (CPU tensors)."""
+    b = fa.RelativeBuckets.window((1, 2, 4))
+    table, q, qkv = torch.zeros(b.num_buckets, 2), torch.zeros(3, 2, 8, 64), torch.zeros(3, 8, 384)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for i in range(4):
+            args = [dual(t) if i == j else t for j, t in enumerate((q, q, q, table))]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fa.window_attn_rel_bias(*args, b)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            fa.window_attn_rel_bias_qkvpacked(dual(qkv), 2, table, b)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            fa.window_attn_rel_bias_qkvpacked(qkv, 2, dual(table), b)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            fa.window_attn_rel_bias(dual(q), q, q, table, b)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            fa.window_attn_rel_bias(q, q, q, table, b)

@@ -53,3 +53,23 @@ def test_buckets_dropped_while_another_stream_reads_them(train):
     want = call(fa.RelativeBuckets(index, table.shape[0]))
     for a, b in zip(result if train else [result], want if train else [want]):
         assert torch.equal(a, b)
+
+
+def test_transforms_are_refused():
+    from torch.autograd import forward_ad
+    from torch.func import grad, jvp, vmap
+    q, k, v, _, table, index = _inputs(2, 2, 20, FP32, seed=2)
+    b = fa.RelativeBuckets(index, table.shape[0])
+    x, p = torch.randn(2, 5, 64, device="cuda"), torch.randn(64, device="cuda")
+    for f, a in ((lambda t: fa.window_attn_rel_bias(t, k, v, table, b), q),
+                 (lambda t: fa.window_attn_rel_bias(q, k, v, t, b), table),
+                 (lambda t: fa.block_prenorm(t, p), x), (lambda t: fa.block_prenorm(x, t), p)):
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            f(forward_ad.make_dual(a, torch.ones_like(a)))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            jvp(f, (a,), (a,))
+        with pytest.raises(RuntimeError):
+            grad(lambda t: f(t).sum())(a)
+        with pytest.raises((RuntimeError, ValueError)):
+            vmap(f)(torch.stack((a, a)))
+        assert torch.isfinite(f(a)).all()
