@@ -158,7 +158,9 @@ class MLP(nn.Module):
 class WindowAttention(nn.Module):
     """W-MSA / SW-MSA parameters (upstream swin3d.py:112-409): ``qkv`` and ``proj`` linears, and with
     ``rel_pos_bias`` (no upstream counterpart) the learned bias of every window offset and head,
-    ``relative_position_bias_table``, zero at first."""
+    ``relative_position_bias_table``, zero at first. The blocks' forward pass is inference, so no gradient
+    reaches the table through it: it is trained through ``window_attn_rel_bias`` or
+    ``window_attn_rel_bias_qkvpacked``, or loaded."""
 
     def __init__(self, dim: int, window_size, num_heads: int, qkv_bias: bool = True,
                  rel_pos_bias: bool = False) -> None:
@@ -300,8 +302,9 @@ class Swin3DTransformerBlock(nn.Module):
             if table is None:
                 a = window_attn_fwd_cute_qkvpacked(qkv, heads, group_ids=gids, output_layout="bnc")
             else:
-                a = window_attn_rel_bias_qkvpacked(qkv, heads, table.detach(), self.attn.buckets(ws, x.device),
-                                                   group_ids=gids, output_layout="bnc")
+                # Detached: F.linear's output requires grad in grad mode, and the call would keep statistics.
+                a = window_attn_rel_bias_qkvpacked(qkv.detach(), heads, table.detach(),
+                                                   self.attn.buckets(ws, x.device), group_ids=gids, output_layout="bnc")
             Nw = xw.shape[1]
             _rec.end("attention", ev, 4 * T * D * e, 4 * xw.shape[0] * heads * Nw * Nw * (D // heads))
             wp, bp = self._w(self.attn.proj, bf16)

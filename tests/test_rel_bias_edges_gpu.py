@@ -73,3 +73,31 @@ def test_transforms_are_refused():
         with pytest.raises((RuntimeError, ValueError)):
             vmap(f)(torch.stack((a, a)))
         assert torch.isfinite(f(a)).all()
+
+
+def test_block_path_makes_no_graph(monkeypatch):
+    """The block's path is inference: in grad mode too, the attention gets nothing that requires grad, and the
+    output has the bits that it has without grad mode."""
+    from flash_aurora_b200 import swin3d
+    blk = swin3d.Swin3DTransformerBlock(dim=64, num_heads=1, time_dim=32, window_size=(2, 3, 4), shift_size=(1, 1, 2),
+                                        precision="fp32", rel_pos_bias=True)
+    swin3d.init_random_weights_(blk)
+    with torch.no_grad():
+        blk.attn.relative_position_bias_table.normal_()
+    blk = blk.cuda()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, c = torch.randn(1, 4 * 6 * 8, 64, device="cuda", generator=g), torch.randn(1, 32, device="cuda", generator=g)
+    with torch.no_grad():
+        want = blk(x, c, (4, 6, 8))
+    seen = []
+    call = swin3d.window_attn_rel_bias_qkvpacked
+
+    def attention(*args, **kw):
+        seen.append(call(*args, **kw))
+        return seen[-1]
+
+    monkeypatch.setattr(swin3d, "window_attn_rel_bias_qkvpacked", attention)
+    assert torch.is_grad_enabled() and blk.attn.qkv.weight.requires_grad
+    got = blk(x, c, (4, 6, 8))
+    assert len(seen) == 1 and not seen[0].requires_grad
+    assert torch.equal(got, want)
