@@ -2,11 +2,12 @@
 // tensor-core products (m16n8k16). The formulas are in rel_bias.cu.
 //
 // Every operand is a pair of halves: x 2^-e = hi + lo, with a power of two of its row that brings the row's largest
-// magnitude to [2^14, 2^15). The pair holds 22 bits of every element down to 2^-18 of that magnitude, and
-// below it 2^-40 of the magnitude; a product is lo hi + hi lo + hi hi, summed in fp32, so it is good to about
-// 2^-22 of its terms, as 3xTF32 is, at half the instructions (16 deep instead of 8). Scales of rows that are summed
-// over (V in P V, K in dS K, Q and dO in the keys' sums) join the other operand, which lies in registers,
-// before it is scaled and split itself: a row of any size, in a masked place for instance, costs the others nothing.
+// finite magnitude to [2^14, 2^15). The pair holds 22 bits of every element down to 2^-18 of that magnitude, and
+// below it 2^-40 of the magnitude; an infinity or NaN makes NaNs of the sums that it enters and of no others. A
+// product is lo hi + hi lo + hi hi, summed in fp32, so it is good to about 2^-22 of its terms, as 3xTF32 is, at
+// half the instructions (16 deep instead of 8). Scales of rows that are summed over (V in P V, K in dS K, Q and dO
+// in the keys' sums) join the other operand, which lies in registers, before it is scaled and split itself: a row of
+// any size, in a masked place for instance, costs the others nothing.
 // Each group of three products is summed from zero and added in fp32: kept in the tensor core's accumulator,
 // which truncates at every product, the sums had errors of 1e-6 where these kernels are at 1.7e-7 (forward) and
 // 2.5e-7 (gradients) of the outputs' norm. That is why these are not UMMAs, whose accumulators stay in TMEM: every
@@ -90,6 +91,19 @@ struct Share {
         x[i][c] = row(i) < N ? __ldg(reinterpret_cast<const float4*>(base + row(i) * st[2] + 16 * c))
                              : make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  // The largest finite magnitude. An infinity must not set its row's scale: it would make zeros of the row's other
+  // columns, which a product over rows (P V, P^T dO) sums apart from it.
+  __device__ __forceinline__ static float finite_max(const float4 (&v)[4]) {
+    float m = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = fabsf(e == 0 ? v[c].x : e == 1 ? v[c].y : e == 2 ? v[c].z : v[c].w);
+        m = fmaxf(m, a == INFINITY ? 0.f : a);  // a NaN is passed over
+      }
+    return m;
+  }
   // Into shared memory, scaled and split; 16-byte chunk c of row r lies at c ^ (r & 7). Rows past N: zeros.
   __device__ __forceinline__ void put(uint32_t dst, float* down) const {
 #pragma unroll
@@ -98,7 +112,9 @@ struct Share {
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         m = fmaxf(m, fmaxf(fmaxf(fabsf(x[i][c].x), fabsf(x[i][c].y)), fmaxf(fabsf(x[i][c].z), fabsf(x[i][c].w))));
-      const Scale s(quad_max(m));
+      m = quad_max(m);
+      if (__any_sync(0xffffffffu, m == INFINITY)) m = quad_max(finite_max(x[i]));  // rare
+      const Scale s(m);
       const int r = row(i), part = threadIdx.x & 3;
       if (part == 0) down[r] = s.down;
 #pragma unroll

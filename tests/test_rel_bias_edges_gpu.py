@@ -101,3 +101,34 @@ def test_block_path_makes_no_graph(monkeypatch):
     got = blk(x, c, (4, 6, 8))
     assert len(seen) == 1 and not seen[0].requires_grad
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_infinity_in_v_and_dout_reaches_its_own_column_only(dtype, value):
+    """out[:, d] and dv[:, d] sum over column d of v and of dout alone, so every other column has the bits that it
+    has with a zero in that place. The other (window, head) pairs keep all of theirs."""
+    N = 40
+    q, k, v, dout, table, index = _inputs(3, 2, N, dtype, seed=4)
+    ids = torch.zeros(1, N, dtype=torch.uint8, device="cuda")
+    ids[0, 30:] = 1
+    spots = {(0, 1): (3, 5), (2, 0): (N - 1, 63), (1, 1): (35, 0)}  # (window, head): (token, column)
+
+    def run(x):
+        vv, gg = v.clone(), dout.clone()
+        for (w, h), (i, d) in spots.items():
+            vv[w, h, i, d] = x
+            gg[w, h, i, d] = x
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, vv)]
+        out = fa.window_attn_rel_bias(*leaves, table, fa.RelativeBuckets(index, table.shape[0]), group_ids=ids)
+        return (out.detach(), *torch.autograd.grad(out, leaves, gg))
+
+    clean, got = run(0.0), run(value)
+    for name, a, b in (("out", got[0], clean[0]), ("dv", got[3], clean[3])):
+        keep = torch.ones_like(a, dtype=torch.bool)
+        for (w, h), (i, d) in spots.items():
+            keep[w, h, :, d] = False
+            assert not torch.isfinite(a[w, h, i, d]), (name, w, h)  # its own token at least
+        assert torch.equal(a[keep], b[keep]), (name, float((a[keep] - b[keep]).abs().max()))
+    for a, b in zip(got, clean):
+        assert torch.equal(a[0, 0], b[0, 0]) and torch.equal(a[1, 0], b[1, 0]) and torch.equal(a[2, 1], b[2, 1])
