@@ -302,6 +302,11 @@ def _check_window(N: int, Dh: int) -> None:
         raise ValueError(f"window attention supports 1 to {_MAX_TOKENS} tokens per window, got {N}")
 
 
+def _check_mask(bias: Optional[torch.Tensor]) -> None:
+    if bias is not None and not bias.dtype.is_signed:  # none of its values could be below -50: no mask at all
+        raise ValueError(f"bias must hold signed values (masked below -50), got {bias.dtype}")
+
+
 def _call_args(t, Bwin, H, N, table, buckets, bias, group_ids, scale_qk):
     if bias is not None and group_ids is not None:
         raise ValueError("pass at most one of bias / group_ids")
@@ -330,7 +335,7 @@ def window_attn_rel_bias(
     group_ids: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Attention on ``q, k, v (Bwin, H, N, 64)`` (bfloat16 or float32, one dtype) with the bias
-    ``table[buckets.index, h]`` and an optional mask: ``bias (nW, N, N)`` (below -50 means masked) or
+    ``table[buckets.index, h]`` and an optional mask: ``bias (nW, N, N)`` (below -50 means masked, so boolean masks are refused) or
     ``group_ids (nW, N)`` uint8. Window ``b`` reads mask ``b % nW``. Returns ``(Bwin, H, N, 64)``."""
     _lib.refuse_forward_ad("window_attn_rel_bias", q, k, v, table)
     if q.ndim != 4 or q.shape != k.shape or q.shape != v.shape:
@@ -343,6 +348,7 @@ def window_attn_rel_bias(
     _check_window(N, Dh)
     if H < 1:
         raise ValueError("at least one head is needed")
+    _check_mask(bias)
     if not q.is_cuda:
         raise RuntimeError("B200 window attention requires CUDA tensors.")
     if k.device != q.device or v.device != q.device:
@@ -383,6 +389,7 @@ def window_attn_rel_bias_qkvpacked(
     Bwin, N, three_c = qkv.shape
     H = int(num_heads)
     _check_window(N, three_c // (3 * H))
+    _check_mask(bias)
     if not qkv.is_cuda:
         raise RuntimeError("B200 window attention requires CUDA tensors.")
     table, mask, call = _call_args(qkv, Bwin, H, N, table, buckets, bias, group_ids, scale_qk)

@@ -86,3 +86,17 @@ def test_forward_mode_is_refused():
             fa.window_attn_rel_bias(dual(q), q, q, table, b)
         with pytest.raises(RuntimeError, match="CUDA"):
             fa.window_attn_rel_bias(q, q, q, table, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.uint8])
+def test_masks_that_cannot_mask_are_refused(dtype):
+    """A boolean mask is never below -50: it would be taken for "nothing masked"."""
+    b = fa.RelativeBuckets.window((1, 2, 4))
+    table, q = torch.zeros(b.num_buckets, 2), torch.zeros(3, 2, 8, 64)
+    mask = torch.ones(1, 8, 8, dtype=dtype)
+    with pytest.raises(ValueError, match="signed"):
+        fa.window_attn_rel_bias(q, q, q, table, b, mask)
+    with pytest.raises(ValueError, match="signed"):
+        fa.window_attn_rel_bias_qkvpacked(torch.zeros(3, 8, 384), 2, table, b, bias=mask)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fa.window_attn_rel_bias(q, q, q, table, b, mask.float())
