@@ -195,21 +195,12 @@ int check_args(int precision, int64_t Bwin, int64_t H, int64_t N, int64_t Dh, co
   return FA_OK;
 }
 
-// Two bf16 numbers whose product is -100 / scale to 16 bits or better: the first is the significand
-// in [1, 2) that leaves the quotient nearest to a bf16 number (exact for the default scale of 1 / 8).
-void split_mask_value(float scale, uint32_t* a_bits, uint32_t* b_bits) {
+// Two bf16 numbers whose sum is -100 / scale to 2^-17 of it.
+void split_mask_value(float scale, uint32_t* hi_bits, uint32_t* lo_bits) {
   const double want = -100.0 / (double)scale;
-  double best = -1.0;
-  for (int m = 0; m < 128; ++m) {
-    const double a = 1.0 + m / 128.0;
-    const __nv_bfloat16 b = __float2bfloat16((float)(want / a));
-    const double off = fabs(a * (double)__bfloat162float(b) - want);
-    if (best < 0.0 || off < best) {
-      best = off;
-      *a_bits = __nv_bfloat16_raw(__float2bfloat16((float)a)).x;
-      *b_bits = __nv_bfloat16_raw(b).x;
-    }
-  }
+  const __nv_bfloat16 hi = __float2bfloat16((float)want);
+  *hi_bits = __nv_bfloat16_raw(hi).x;
+  *lo_bits = __nv_bfloat16_raw(__float2bfloat16((float)(want - (double)__bfloat162float(hi)))).x;
 }
 
 void copy3(int64_t* dst, const int64_t* src) {
@@ -258,7 +249,7 @@ extern "C" int fa_window_attention_rel_bias(int precision, int64_t Bwin, int64_t
   p.bias = reinterpret_cast<const float4*>(state);
   p.ranks = reinterpret_cast<const uint8_t*>(p.bias + bias_copies(precision) * H * kBiasVecs);
   p.mask = mask_u8 ? mask_u8 : group_ids;
-  if (group_ids) split_mask_value(scale, &p.mask_a, &p.mask_b);
+  if (group_ids) split_mask_value(scale, &p.mask_hi, &p.mask_lo);
   p.stats = reinterpret_cast<float2*>(stats);
   cudaStream_t s = (cudaStream_t)stream;
   const int copies = bias_copies(precision);
@@ -305,9 +296,9 @@ extern "C" int fa_window_attention_rel_bias_backward(
     copy3(p.sq, strides); copy3(p.sk, strides + 3); copy3(p.sv, strides + 6); copy3(p.so, strides + 9);
     copy3(p.sdq, strides + 12); copy3(p.sdk, strides + 15); copy3(p.sdv, strides + 18);
     p.bias = reinterpret_cast<const float4*>(state);
-  p.ranks = reinterpret_cast<const uint8_t*>(p.bias + bias_copies(precision) * H * kBiasVecs);
+    p.ranks = reinterpret_cast<const uint8_t*>(p.bias + bias_copies(precision) * H * kBiasVecs);
     p.mask = mask_u8 ? mask_u8 : group_ids;
-  if (group_ids) split_mask_value(scale, &p.mask_a, &p.mask_b);
+    if (group_ids) split_mask_value(scale, &p.mask_hi, &p.mask_lo);
     p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats));
     p.slots = dtable ? reinterpret_cast<float*>(workspace) : nullptr;
     p.status = attn::status_ptr();

@@ -25,7 +25,7 @@ struct Params {
   const float4* bias;        // the bias in fragment order, see expand_bias_kernel in rel_bias.cu
   const uint8_t* mask;       // (nW, N, N) bytes or (nW, N) region ids, by MaskKind
   const uint8_t* ranks;      // with region ids: (nW, 144) rank of each token's id in its window, kNoRank past N
-  uint32_t mask_a, mask_b;   // bf16 bits: mask_a * mask_b = -100 / scale (region masks, bf16 kernels)
+  uint32_t mask_hi, mask_lo; // bf16 bits: mask_hi + mask_lo = -100 / scale (region masks, bf16 kernels)
   float2* stats;             // (Bwin, H, 144): row maximum and log2 of the row sum, log2 domain
   float* slots;              // backward: (gridDim.x + H - 1) partial bias gradients in fragment order
   int* status;

@@ -11,10 +11,12 @@
 // 144 keys sit in four threads of one warp (16x256b TMEM shape): row maxima and sums take two shuffles.
 // Registers are moved from warps 0..3 to 4..11 (setmaxnreg).
 //
-// Region-id masks go through the tensor cores: with the ids of a window ranked, one K = 16 step adds
+// Region-id masks go through the tensor cores: with the ids of a window ranked, a K = 16 step adds
 //   sum_r onehot(rank of query)[r] * (-c (1 - onehot(rank of key)[r])),  c = 100 / scale,
-// exactly 0 to the raw logit of a pair of one region and -c to the others; a window of R regions
-// takes ceil(R / 16) steps (none for R = 1), whatever its ids are. c is a product of two bf16 numbers.
+// exactly 0 to the raw logit of a pair of one region and -c to the others. c is a sum of two bf16 numbers, each
+// with a column per rank (the best product of two, 16 ranks a step, is off by up to 0.028 of the 100 at scales
+// like 0.39); a window of R regions takes ceil(R / 8) steps (none for R = 1), whatever its ids are. Shifts
+// of all three axes make 8 regions.
 // The per-logit alternative (compare and add in the softmax warps) cost 110 us of 350 on half-masked
 // windows of 144 tokens. Byte masks are applied per logit.
 //
@@ -173,6 +175,7 @@ struct ByteMask {
 // one warp builds the operands, lane holds tokens lane + 32 m.
 // ------------------------------------------------------------------------------------------
 struct Regions {
+  static constexpr uint32_t kOnes = 0x3f803f80u;  // two bf16
   int rank[5];
   int steps;  // mask K-steps: 0 for one region
   __device__ __forceinline__ void read(const uint8_t* ranks, int lane) {
@@ -183,25 +186,27 @@ struct Regions {
       most = max(most, rank[m] == kNoRank ? 0u : (uint32_t)rank[m]);
     }
     most = __reduce_max_sync(0xffffffffu, most);
-    steps = most > 0 ? (int)(most >> 4) + 1 : 0;
+    steps = most > 0 ? (int)(most >> 3) + 1 : 0;
   }
-  // The A and B operands of step `st` (rows of 16 bf16, 32-byte swizzle) at shared address `op`.
-  __device__ __forceinline__ void build(uint32_t op, int st, int lane, uint32_t a_bits, uint32_t b_bits) const {
-    const uint32_t fill = b_bits | (b_bits << 16);
+  // The A and B operands of step `st` (ranks 8 st .. 8 st + 7, a column of the high and one of the low part each;
+  // rows of 16 bf16, 32-byte swizzle) at shared address `op`.
+  __device__ __forceinline__ void build(uint32_t op, int st, int lane, uint32_t hi_bits, uint32_t lo_bits) const {
+    const uint32_t hi2 = hi_bits | (hi_bits << 16), lo2 = lo_bits | (lo_bits << 16);
 #pragma unroll
     for (int m = 0; m < 5; ++m) {
       if (m == 4 && lane >= kMaxN - 128) break;
-      const int r = lane + 32 * m, slot = rank[m] - 16 * st;
-      const uint32_t row = op + (uint32_t)r * 32u, f = rank[m] != kNoRank ? fill : 0u;
-      st_shared_v4(row, 0u, 0u, 0u, 0u);
-      st_shared_v4(row + 16u, 0u, 0u, 0u, 0u);
-      st_shared_v4(row + kRow32, f, f, f, f);
-      st_shared_v4(row + kRow32 + 16u, f, f, f, f);
-      if ((uint32_t)slot < 16u && rank[m] != kNoRank) {
-        const uint32_t hot = row + ((uint32_t)(((slot >> 3) ^ (r >> 2)) & 1) << 4) + (uint32_t)(slot & 7) * 2u;
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(hot), "h"((unsigned short)a_bits) : "memory");
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(hot + kRow32), "h"((unsigned short)0) : "memory");
-      }
+      const int r = lane + 32 * m, slot = rank[m] - 8 * st;
+      const uint32_t row = op + (uint32_t)r * 32u, sw = (uint32_t)((r >> 2) & 1) << 4;
+      const bool in = rank[m] != kNoRank;
+      const uint32_t h = in ? hi2 : 0u, l = in ? lo2 : 0u, half = slot & 1 ? 0xffff0000u : 0x0000ffffu;
+      uint32_t hot[4];  // the rank's column; past N, and outside this step, none
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hot[e] = (slot >> 1) == e ? half : 0u;
+      const uint32_t a0 = hot[0] & kOnes, a1 = hot[1] & kOnes, a2 = hot[2] & kOnes, a3 = hot[3] & kOnes;
+      st_shared_v4(row, a0, a1, a2, a3);  // the halves are alike, whichever the swizzle puts first
+      st_shared_v4(row + 16u, a0, a1, a2, a3);
+      st_shared_v4(row + kRow32 + sw, h & ~hot[0], h & ~hot[1], h & ~hot[2], h & ~hot[3]);
+      st_shared_v4(row + kRow32 + (sw ^ 16u), l & ~hot[0], l & ~hot[1], l & ~hot[2], l & ~hot[3]);
     }
     fence_proxy_async_shared();
     __syncwarp();
@@ -439,7 +444,7 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
       for (int st = 0; st < reg.steps; ++st, ++jobs) {
         const int b = jobs & 1;
         if (!warp_wait(c.bar(kMaskEmpty + b), (uint32_t)(((jobs >> 1) & 1) ^ 1), c.abort, p.status, 104)) { ok = 0; break; }
-        reg.build(c.sbase + kOffMask + b * kMaskOpBytes, st, lane, p.mask_a, p.mask_b);
+        reg.build(c.sbase + kOffMask + b * kMaskOpBytes, st, lane, p.mask_hi, p.mask_lo);
         if (lane == 0) mbar_arrive(c.bar(kMaskFull + b));
       }
       if (!ok) break;
@@ -897,7 +902,7 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
       // The dS buffer is free once dK of the tile before is done.
       if (now.steps > 0 && i > 0 && !warp_wait(c.bar(kDkFull), (uint32_t)((i - 1) & 1), c.abort, p.status, 133)) break;
       for (int st = 0; st < now.steps && ok; ++st) {
-        if (st > 0 && st % kMaskSlots == 0) {  // more than 64 regions: wait until the slots have been read
+        if (st > 0 && st % kMaskSlots == 0) {  // more than 32 regions: wait until the slots have been read
           if (lane == 0) {
             if (st == kMaskSlots) {
               c.steps[i & 1] = now.steps;
@@ -909,7 +914,7 @@ __device__ __forceinline__ void producer(const Params& p, const Ctx& c, int lane
           ok = warp_wait(c.bar(kMaskEmpty), (uint32_t)(more & 1), c.abort, p.status, 134);
           ++more;
         }
-        if (ok) now.build(c.sbase + kOffDs + (st % kMaskSlots) * kMaskOpBytes, st, lane, p.mask_a, p.mask_b);
+        if (ok) now.build(c.sbase + kOffDs + (st % kMaskSlots) * kMaskOpBytes, st, lane, p.mask_hi, p.mask_lo);
       }
       if (!ok) break;
       if (lane == 0) {

@@ -8,6 +8,8 @@ gradient (of its norm, or of 1).
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -208,6 +210,31 @@ def test_scales(scale, kind, dtype):
     kw = {"group_ids": ids} if mask is None else {"bias": torch.where(mask, -100.0, 0.0)}
     got = _run(q, k, v, table, index, dout, scale_qk=scale, **kw)
     _check(got, reference(q, k, v, table, index, scale, dout, ids, mask), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("scale", [0.125, 0.39, -0.195, 3.0, 1e-4])
+@pytest.mark.parametrize("kind", ["ids", "bytes"])
+def test_masked_logits_get_minus_100_at_any_scale(kind, scale, dtype):
+    """Two keys, the other one masked and its bias 95 or 98 above: its weight w = 1 / (1 + e^5) or 1 / (1 + e^2) shows
+    the -100. The bf16 kernels' region masks add a sum of two bf16 numbers, good to 2^-17 of 100, so to 7.7e-4 of w;
+    P and the output are rounded, 2^-8 each. fp32: three roundings of numbers between 128 and 256, half of 2^-16 each,
+    times ln 2: 1.6e-5 of w, and 1e-6 for the sums."""
+    q = torch.zeros(1, 1, 2, 64, device="cuda", dtype=dtype)
+    v = torch.zeros_like(q)
+    v[0, 0, 0, 0] = v[0, 0, 1, 1] = 1.0
+    b = fa.RelativeBuckets(torch.arange(4, device="cuda").view(2, 2), 4)
+    if kind == "ids":
+        kw = {"group_ids": torch.tensor([[3, 9]], dtype=torch.uint8, device="cuda")}
+    else:
+        kw = {"bias": torch.tensor([[[0.0, -100.0], [-100.0, 0.0]]], device="cuda")}
+    tol = 2 * 2.0 ** -8 + 7.7e-4 if dtype == BF16 else 1.7e-5
+    for lift in (95.0, 98.0):
+        table = torch.tensor([[0.0], [lift], [lift], [0.0]], device="cuda")
+        w = 1.0 / (1.0 + math.exp(100.0 - lift))
+        out = fa.window_attn_rel_bias(q, q, v, table, b, scale_qk=scale, **kw)[0, 0].double()
+        for got, want in ((out[0, 1], w), (out[1, 0], w), (out[0, 0], 1 - w), (out[1, 1], 1 - w)):
+            assert abs(float(got) - want) <= tol * want, (lift, float(got), want)
 
 
 def test_nan_and_infinity_in_bf16_queries():
