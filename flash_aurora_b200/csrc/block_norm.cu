@@ -15,7 +15,11 @@
 // The sums over rows are kept in registers by the threads that own the columns, added over a block's
 // row groups in shared memory, and over blocks by a second kernel in a fixed order (no atomics).
 //
-// All of it is bound by memory: a row is read once, by its group of `tpr` threads. Every thread copies the
+// A row is read once, by its group of `tpr` threads. Forward rows of whole 16-byte units with a residual are bound by
+// memory where their width fills the group's threads (0.83 to 1.0 of the measured copy bandwidth at 512, 1024 and 2048
+// columns; 0.58 and 0.70 for `between` at 520 and 1536, which leave half and a quarter of them idle). `before` is not
+// (0.36 to 0.61): its blocks per SM are those of the forms with five parameter arrays. Rows that go element by element
+// are bound by their instructions, the backward pass by the chain of its two reductions. Every thread copies the
 // elements that it will itself work on into a ring of its own in shared memory, kStages rows ahead
 // (cp.async: no registers, no barrier), so that loads run while rows are reduced; with loads into
 // registers at the top of each row the backward pass of (32400, 2048) rows took 504 us and the forward

@@ -5,9 +5,15 @@
 beside :mod:`flash_aurora_b200.window_attn`, whose kernels take only the 0 / -100 mask. ``table``
 ``(num_buckets, H)`` is the learned parameter (the ``relative_position_bias_table`` of Swin models);
 :class:`RelativeBuckets` says which bucket each (query, key) pair of a window reads. Gradients reach
-q, k, v (or the packed qkv) and the table. Windows hold 1 to 144 tokens, head_dim is 64, tensors are
-bfloat16 or float32 (products of 22-bit operands, fp32 accuracy); masks as in ``window_attn``: region ids or a
-float bias below -50, each adding -100 to a masked logit.
+q, k, v (or the packed qkv) and the table. Windows hold 1 to 144 tokens, head_dim is 64; masks as in
+``window_attn``: region ids or a float bias below -50, each adding -100 to a masked logit. A row whose logits are all
+-inf (a bias of -inf for every key) is NaN, as its softmax is.
+
+The tensors' dtype is the tier. bfloat16: logits, softmax and all sums are fp32; the probabilities, and in the
+backward pass dS, are rounded to bf16 as operands of the products that follow, so the error against exact arithmetic is
+2.1e-3 of the output's norm (2.4e-3 for the gradients) where the output's own rounding makes 1.7e-3. float32: operands
+keep 22 bits, or 2^-40 of the largest of their row of 64 if that is more, and sums are fp32: 1.7e-7 and 2.5e-7 of
+the norm. The table's gradient is summed in fp32 in both.
 
 A step may be captured in a CUDA graph; as for any differentiable torch call, no eager autograd graph of the same
 leaves may be alive then (torch refuses such a capture).
