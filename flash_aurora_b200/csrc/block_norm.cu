@@ -16,7 +16,7 @@
 // row groups in shared memory, and over blocks by a second kernel in a fixed order (no atomics).
 //
 // A row is read once, by its group of `tpr` threads. Forward rows of whole 16-byte units with a residual are bound by
-// memory where their width fills the group's threads (0.83 to 1.0 of the measured copy bandwidth at 512, 1024 and 2048
+// memory where their width fills the group's threads (0.82 to 1.0 of the measured copy bandwidth at 512, 1024 and 2048
 // columns; 0.58 and 0.70 for `between` at 520 and 1536, which leave half and a quarter of them idle). `before` is not
 // (0.36 to 0.61): its blocks per SM are those of the forms with five parameter arrays. Rows that go element by element
 // are bound by their instructions, the backward pass by the chain of its two reductions. Every thread copies the

@@ -21,7 +21,7 @@
 //             P^T and dS^T are at hand as A operands of dV = P^T dO and dK = dS^T Q. The two products computed
 //             again cost 2 of 7 and save 166 KB of shared memory for the pairs of P and dS, and all exchange between
 //             warps but delta.
-// 1024 tiles of 144 tokens take 112 us forward (two blocks an SM; 40 % of issue slots) and 300 us backward (one;
+// 1024 tiles of 144 tokens take 120 us forward (two blocks an SM; 40 % of issue slots) and 300 us backward (one;
 // 32 %), against 23 / 41 us of memory traffic and about 33 / 115 us of products: what bounds them is the latency of
 // dependent instructions with the 9 or 18 warps that registers and shared memory allow.
 #include <cuda_fp16.h>
