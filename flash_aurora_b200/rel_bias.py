@@ -51,6 +51,8 @@ class RelativeBuckets:
     at every replay, so it has to live as long as the graph.
     """
 
+    _stream: Optional[int] = None  # of a GPU's lists: the stream (handle) that their memory belongs to, if known
+
     def __init__(self, index: torch.Tensor, num_buckets: int, device: Optional[torch.device] = None) -> None:
         if index.ndim != 2 or index.shape[0] != index.shape[1] or not 1 <= index.shape[0] <= _MAX_TOKENS:
             raise ValueError(f"index must be (N, N) with 1 <= N <= {_MAX_TOKENS}, got {tuple(index.shape)}")
@@ -73,7 +75,6 @@ class RelativeBuckets:
         self.index = flat.view(self.tokens, self.tokens).to(torch.int32)
         self.order = order.to(torch.int32)
         self.offsets = torch.searchsorted(values, torch.arange(num_buckets + 1, device=dev)).to(torch.int32)
-        self._stream = None  # of a GPU's lists: the stream (handle) that their memory belongs to
         if dev.type == "cuda":  # ready for every stream from here on
             stream = torch.cuda.current_stream(dev)
             stream.synchronize()

@@ -100,3 +100,12 @@ def test_masks_that_cannot_mask_are_refused(dtype):
         fa.window_attn_rel_bias_qkvpacked(torch.zeros(3, 8, 384), 2, table, b, bias=mask)
     with pytest.raises(RuntimeError, match="CUDA"):
         fa.window_attn_rel_bias(q, q, q, table, b, mask.float())
+
+
+def test_buckets_pickled_without_a_stream():
+    """A pickle of the first version's object has no stream: unknown, so every stream is recorded."""
+    b = fa.RelativeBuckets.window((1, 2, 3))
+    b.__dict__.pop("_stream", None)
+    t, s = _Recorded(), SimpleNamespace(cuda_stream=0)
+    b._used_by(s, t)
+    assert t.streams == [s]
